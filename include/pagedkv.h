@@ -58,6 +58,7 @@ extern "C" {
 #define PKV_FLAG_BAD_QUERY_LAYOUT 16
 #define PKV_FLAG_POSITION_OUT_OF_RANGE 32
 #define PKV_FLAG_BAD_SCHEDULE 64 /* a decode schedule built for another batch, grid or table width */
+#define PKV_FLAG_OUT_OF_BLOCKS 128 /* pkv_build_step_tables: the free list ran short */
 
 /* size of the device-resident scratch array behind
  * pkv_paged_decode_attention_noalloc (per GPU, held until the process exits) */
@@ -557,6 +558,132 @@ int pkv_paged_prefill_attention_fp8(void* out, int64_t out_row_stride, const voi
                                     int max_query_len, int n_q_heads, int n_kv_heads, int head_dim,
                                     int block_size, float scale, int dtype, int* err_flags,
                                     pkv_stream_t stream);
+
+/*
+ * The metadata of a step, built on the GPU from request lengths.  Replaces, for
+ * hosts that keep lengths, tables and the free list in device memory, the
+ * per-sequence table growth of mini_engine/scheduler.py:79-156 and the slot
+ * computation of mini_engine/paged/block_manager.py:121-131.
+ *
+ * Request i has num_prior[i] cached and num_new[i] new tokens and owns row i of
+ * block_tables.  It needs ceil((prior + new) / block_size) - ceil(prior /
+ * block_size) new blocks, which are taken from the end of free_blocks[0 ..
+ * *n_free) in request order (the order in which BlockManager.allocate pops its
+ * free list) and written behind its table's ceil(prior / block_size) entries;
+ * *n_free_out = blocks left.  Outputs: context_lens[i] = prior + new,
+ * query_start_loc [n_seqs + 1] (the prefix sum of new), and for each of the
+ * query_start_loc[n_seqs] tokens slot_mapping (table entry * block_size + offset)
+ * and positions; further entries up to n_tokens get slot -1 and position 0.
+ *
+ * Requests are served in order while blocks last.  One that is not (the free
+ * list is short: PKV_FLAG_OUT_OF_BLOCKS; its tokens pass n_tokens:
+ * PKV_FLAG_BAD_QUERY_LAYOUT) keeps its rows of the batch, with slots -1 and
+ * context_lens 0, which every kernel here skips, and takes no block; nor do the
+ * requests after it.  A negative length (PKV_FLAG_BAD_QUERY_LAYOUT) or one past
+ * the table (PKV_FLAG_CONTEXT_EXCEEDS_TABLE) counts as a request without tokens.
+ * n_free_out must not be n_free.  Up to 16,384 requests.
+ */
+int pkv_build_step_tables(int32_t* block_tables, int64_t block_table_stride, int max_blocks_per_seq,
+                          const int32_t* free_blocks, int n_free_blocks, const int32_t* n_free,
+                          int32_t* n_free_out, const int32_t* num_prior, const int32_t* num_new,
+                          int n_seqs, int block_size, int32_t* context_lens,
+                          int32_t* query_start_loc, int64_t* slot_mapping, int64_t* positions,
+                          int n_tokens, int* err_flags, pkv_stream_t stream);
+
+/*
+ * int8 KV pools with one scale per (block, KV head).  No counterpart in the
+ * reference.  Pools hold one signed byte per element in the reference layout
+ * [num_blocks][block_size][n_kv_heads][head_dim]; k_scale / v_scale
+ * [num_blocks][n_kv_heads] fp32.  The scale of a (block, head) is the smallest
+ * power of two s = 2^e, e >= -120, with absmax <= 127 s over the block's rows of
+ * that head; byte = x / s rounded to nearest even; value = byte * s (exact in
+ * fp16 range, bf16 and fp32).  Infinities are stored as +-127 and NaN as 0, and
+ * neither enters absmax.  q, out and new rows are in `dtype` (fp32, fp16 or
+ * bf16).  head_dim 64 or 128, block_size a multiple of 16, pools 16-byte aligned
+ * (else PKV_ERR_UNSUPPORTED / PKV_ERR_MISALIGNED).
+ */
+
+/*
+ * Quantising append: rows query_start_loc[i] .. query_start_loc[i + 1] of k / v
+ * become the last tokens of context i (positions context_lens[i] - n ..
+ * context_lens[i] - 1), through its block table.  A block whose first row is
+ * among them starts anew; one that goes on keeps its rows, and if the new rows
+ * need a larger scale its bytes become rne(byte * old / new).  A context of
+ * length 0 writes nothing.  A block may be written by one sequence per call.
+ * Rows past query_start_loc[n_seqs] belong to no sequence and are not read.
+ */
+int pkv_reshape_and_cache_int8(const void* k, const void* v, int64_t k_row_stride,
+                               int64_t v_row_stride, void* k_pool, void* v_pool, float* k_scale,
+                               float* v_scale, int num_blocks, const int32_t* block_tables,
+                               int64_t block_table_stride, int max_blocks_per_seq,
+                               const int32_t* context_lens, const int32_t* query_start_loc,
+                               int n_seqs, int n_tokens, int n_kv_heads, int head_dim,
+                               int block_size, int dtype, int* err_flags, pkv_stream_t stream);
+
+/*
+ * The last row_start_loc[i + 1] - row_start_loc[i] rows of each context as
+ * values (byte * scale rounded to dtype), packed one sequence behind the other:
+ * the gather of append_and_fetch (mini_engine/paged/block_manager.py:136-141).
+ * k_out / v_out [n_rows][n_kv_heads][head_dim] with row strides in elements.
+ */
+int pkv_fetch_int8(void* k_out, void* v_out, int64_t k_row_stride, int64_t v_row_stride,
+                   const void* k_pool, const void* v_pool, const float* k_scale,
+                   const float* v_scale, int num_blocks, const int32_t* block_tables,
+                   int64_t block_table_stride, int max_blocks_per_seq,
+                   const int32_t* context_lens, const int32_t* row_start_loc, int n_seqs,
+                   int n_rows, int n_kv_heads, int head_dim, int block_size, int dtype,
+                   int* err_flags, pkv_stream_t stream);
+
+/* Split-K scratch of the decode call below (any initial contents; one call at a time). */
+size_t pkv_decode_int8_workspace_bytes(int n_q_heads, int head_dim);
+
+/* pkv_paged_decode_attention over such pools (the new token already appended):
+ * one query row per sequence over its context_lens[s] keys; a context of length
+ * 0 gives a zero row.  Two launches per 1,024 sequences. */
+int pkv_paged_decode_attention_int8(void* out, int64_t out_row_stride, const void* q,
+                                    int64_t q_row_stride, const void* k_pool, const void* v_pool,
+                                    const float* k_scale, const float* v_scale, int num_blocks,
+                                    const int32_t* block_tables, int64_t block_table_stride,
+                                    int max_blocks_per_seq, const int32_t* context_lens,
+                                    int n_seqs, int n_q_heads, int n_kv_heads, int head_dim,
+                                    int block_size, float scale, int dtype, void* workspace,
+                                    size_t workspace_bytes, int* err_flags, pkv_stream_t stream);
+
+/* Scratch of the chunked prefill below: the visible rows of every sequence as values. */
+size_t pkv_prefill_int8_scratch_bytes(int n_seqs, int max_blocks_per_seq, int n_kv_heads,
+                                      int head_dim, int block_size, int dtype);
+
+/* pkv_paged_prefill_attention over such pools (the chunk already appended): query
+ * i of sequence s sees keys 0 .. num_prior[s] + i.  One pass lays the visible
+ * rows out in the scratch (256-byte aligned), then the packed attention runs over
+ * it.  scale > 0. */
+int pkv_paged_prefill_attention_int8(void* out, int64_t out_row_stride, const void* q,
+                                     int64_t q_row_stride, const void* k_pool, const void* v_pool,
+                                     const float* k_scale, const float* v_scale, int num_blocks,
+                                     const int32_t* block_tables, int64_t block_table_stride,
+                                     int max_blocks_per_seq, const int32_t* query_start_loc,
+                                     const int32_t* num_prior, int n_seqs, int n_tokens,
+                                     int n_q_heads, int n_kv_heads, int head_dim, int block_size,
+                                     float scale, int dtype, void* scratch, size_t scratch_bytes,
+                                     int* err_flags, pkv_stream_t stream);
+
+/*
+ * Causal attention with grouped heads over whole prompts packed one behind the
+ * other, without a cache: row i of sequence s (rows query_start_loc[s] ..
+ * query_start_loc[s + 1]) sees rows 0 .. i of its own sequence.  Replaces
+ * Qwen2Model._attention (mini_engine/model/qwen2.py:98-128) for callers that
+ * score prompts.  q, out [n_tokens][n_q_heads][head_dim], k, v
+ * [n_tokens][n_kv_heads][head_dim] with row strides in elements (views of one
+ * fused projection will do); out must not overlap k or v.  head_dim 64 or 128,
+ * scale > 0.  Rows past query_start_loc[n_seqs] are neither read nor written.  A
+ * key that a row must not see never enters it, whatever it holds.
+ */
+int pkv_packed_prompt_attention(void* out, int64_t out_row_stride, const void* q,
+                                int64_t q_row_stride, const void* k, int64_t k_row_stride,
+                                const void* v, int64_t v_row_stride, const int32_t* query_start_loc,
+                                int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads,
+                                int head_dim, float scale, int dtype, int* err_flags,
+                                pkv_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,710 @@
+// pkv_decode_int8.cu -- decode attention (one query row per sequence) over int8
+// pools with one power-of-two scale per (block, KV head).
+//
+// Replaces the gather of append_and_fetch and _attention with num_new == 1 of
+// the reference (mini_engine/paged/block_manager.py:136-141,
+// mini_engine/model/qwen2.py:98-128) for such pools.
+//
+// Mathematics.  With k_j = 2^a_b K_j and v_j = 2^c_b V_j (K, V integers, b the
+// block of token j), x_j = (scale 2^a_b) (q . K_j) and
+//   o = sum_j softmax(x)_j 2^c_b V_j.
+// The integers are exact in fp16, so the products run on the tensor cores
+// (m16n8k16, fp32 sums): S^T = K Q^T with 16 tokens as M and 8 query heads of
+// the GQA group as N, O^T += V^T P^T.  The K scale multiplies the fp32 scores.
+// The V scale goes into P as 2^(c_b - E), E the largest exponent seen so far (a
+// larger one rescales O, exactly), and 2^E into O at the end; the row sum takes
+// the unscaled p.  Running maximum, sums and O are fp32.  q is fp16; bf16 rows
+// are brought into fp16 range by the power of two of their largest value (8 bits
+// fit exactly but for elements 2^-16 below the row's largest, whose error is
+// 2^-25 of it).  fp32 rows, and the P that go with them, are split into two fp16
+// parts (22 bits) and each product is two MMAs.
+//
+// Converting a byte costs no conversion instruction: x ^ 0x80 = x + 128 becomes
+// the low byte of the fp16 1024 + 128 + x (a byte permute), and subtracting 1152
+// is exact.  fp8 bytes need the conversion pipe, which bounds the fp8 kernel at
+// about half of the HBM rate.
+//
+// Work split.  The 16-token tiles of all sequences are cut into one contiguous
+// range per CTA and the range into one sub-range per team of warps (one warp per
+// KV head and chunk of query heads, so the heads of a token are read at about
+// the same time).  Each warp streams its tiles through its own ring of
+// shared-memory stages with 16-byte cp.async (no barrier between warps: a warp
+// waits only for its own copies).  Partial (m, l, O) of a sequence that several
+// teams share meet in shared memory at the end of the CTA, those of a sequence
+// that several CTAs share in the workspace, joined in CTA order by a second
+// launch.
+#include <algorithm>
+#include <type_traits>
+
+#include "pkv_common.cuh"
+#include "pkv_internal.h"
+
+namespace pkv {
+
+namespace {
+
+constexpr int kD8MaxSeqs = 1024;   // per launch
+constexpr int kD8MaxCtas = 296;    // per launch and head group
+constexpr float kD8Log2e = 1.4426950408889634f;
+constexpr float kD8Slack = 8.f;    // the reference maximum moves by more than this (log2)
+
+struct D8Params {
+  void* out;
+  const void* q;
+  int64_t out_stride, q_stride;
+  const int8_t* k_pool;
+  const int8_t* v_pool;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* block_tables;
+  int64_t bt_stride;
+  const int32_t* context_lens;
+  int n_seqs, max_blocks, num_blocks, tiles_per_block;
+  int n_q_heads, n_kv_heads, group, chunks;  // chunks of 8 NT query heads per KV head
+  int n_groups;                              // n_kv_heads * chunks
+  int teams;                                 // per CTA
+  int per_cta;                               // head groups per CTA
+  float scale_log2;
+  float* part_o;   // [2 * grid][n_q_heads][D]
+  float* part_ml;  // [2 * grid][n_q_heads][2]
+  int* err;
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// bytes (biased by 128) -> fp16 pairs; magic = 0x64646464
+__device__ __forceinline__ uint32_t sub1152(uint32_t h) {
+  const __half2 c = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+  const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&h), c);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t i8_lo(uint32_t biased) { return sub1152(__byte_perm(biased, 0x64646464u, 0x4140)); }
+__device__ __forceinline__ uint32_t i8_hi(uint32_t biased) { return sub1152(__byte_perm(biased, 0x64646464u, 0x4342)); }
+
+__device__ __forceinline__ uint4 flip(uint4 w) {
+  return make_uint4(w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u);
+}
+
+// last s in [0, n) with prefix[s] <= x
+__device__ __forceinline__ int d8_find(const int* prefix, int n, int x) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (prefix[mid] <= x) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// stage: K tile, V tile (16 rows x D bytes each), K scale, V scale
+template <int D> __host__ __device__ constexpr int d8_stage() { return 2 * 16 * D + 16; }
+// Position of the 16-byte chunk c of row r.  K is read 16 bytes a lane (row g,
+// chunk t), V 8 bytes a lane (rows 2t + {0, 1, 8, 9} in an order that depends on
+// t's parity): both orders fill all banks.
+template <int D> __device__ __forceinline__ int k_chunk(int r, int c) {
+  return D == 64 ? r * 64 + c * 16 : r * 128 + ((c ^ ((r & 1) << 2)) << 4);
+}
+template <int D> __device__ __forceinline__ int v_chunk(int r, int c) {
+  return D == 64 ? r * 64 + ((c ^ (((r >> 2) & 1) << 1)) << 4) : r * 128 + ((c ^ (r & 6)) << 4);
+}
+
+template <typename T, int D, int NT, int LIMBS, int WARPS, int STAGES>
+__global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Params p) {
+  constexpr int KS = D / 16;          // k-steps of the scores, and m-tiles of O
+  constexpr int kHeads = 8 * NT;      // query heads of a warp
+  constexpr int kSlot = kHeads * (D + 2);  // floats of a partial: O, then (m, l)
+  constexpr int kStage = d8_stage<D>();
+  constexpr int kRing = STAGES * kStage;
+  static_assert(kRing >= kSlot * 4, "a warp's ring holds its last partial");
+  extern __shared__ __align__(128) uint8_t d8_smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int B = p.n_seqs;
+  uint8_t* ring = d8_smem + warp * kRing;
+  float* heads_part = reinterpret_cast<float*>(d8_smem + WARPS * kRing);  // [WARPS][kSlot]
+  int* prefix = reinterpret_cast<int*>(heads_part + WARPS * kSlot);       // [B + 1] tiles before each sequence
+  int* ctxs = prefix + B + 1;                                             // [B]
+  __shared__ int wsum[WARPS];
+  __shared__ int slot_seq[2 * WARPS];  // sequence of each team's partials (-1: none)
+
+  pdl_trigger();
+  pdl_wait();  // the metadata, q and the pools may come from the kernel before this one
+
+  // ---- tiles of each sequence, and their prefix
+  {
+    const int64_t room = static_cast<int64_t>(p.max_blocks) * p.tiles_per_block * 16;
+    const int per = (B + WARPS * 32 - 1) / (WARPS * 32);
+    const int lo = min(B, tid * per), hi = min(B, lo + per);
+    int sum = 0;
+    for (int i = lo; i < hi; ++i) {
+      int c = max(p.context_lens[i], 0);
+      if (c > room) {
+        if (blockIdx.x == 0 && blockIdx.y == 0) raise_flag(p.err, PKV_FLAG_CONTEXT_EXCEEDS_TABLE);
+        c = static_cast<int>(room);
+      }
+      ctxs[i] = c;
+      sum += (c + 15) >> 4;
+    }
+    int x = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) wsum[warp] = x;
+    __syncthreads();
+    int run = x - sum;
+    for (int w = 0; w < warp; ++w) run += wsum[w];
+    for (int i = lo; i < hi; ++i) {
+      prefix[i] = run;
+      run += (ctxs[i] + 15) >> 4;
+    }
+    if (hi == B && lo < B) prefix[B] = run;
+    if (tid < 2 * WARPS) slot_seq[tid] = -1;
+    __syncthreads();
+  }
+  const int total = prefix[B];
+  const int per = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), p.teams);
+  const int c0 = min(total, static_cast<int>(blockIdx.x) * per), c1 = min(total, c0 + per);
+  const int team = warp / p.per_cta;
+  const int hg = blockIdx.y * p.per_cta + (warp - team * p.per_cta);
+  const int sub = (c1 - c0 + p.teams - 1) / p.teams;
+  const bool works = team < p.teams && hg < p.n_groups;
+  const int r0 = works ? min(c1, c0 + team * sub) : c1, r1 = works ? min(c1, r0 + sub) : c1;
+  const int kvh = hg / p.chunks, head0 = kvh * p.group + (hg - kvh * p.chunks) * kHeads;
+  const int nh = works ? min(kHeads, (kvh + 1) * p.group - head0) : 0;  // this warp's query heads
+
+  if (r0 < r1) {
+    // ---- the ring: tile i of the range (i from 0) sits in stage i % STAGES
+    const int n_tiles = r1 - r0;
+    const int64_t pitch = static_cast<int64_t>(p.n_kv_heads) * D;
+    const uint32_t ring_a = smem_u32(ring);
+    int ids = 0, ids_next = 0;  // lane l: first pool row / 16 of tile 32 b + l
+    auto load_ids = [&](int b) {
+      const int i = b * 32 + lane;
+      int row16 = 0;
+      if (i < n_tiles) {
+        const int s = d8_find(prefix, B, r0 + i);
+        const int tile = r0 + i - prefix[s];
+        const int jb = tile / p.tiles_per_block;
+        int id = p.block_tables[static_cast<int64_t>(s) * p.bt_stride + jb];
+        if (id < 0 || id >= p.num_blocks) {
+          raise_flag(p.err, PKV_FLAG_BLOCK_OUT_OF_RANGE);
+          id = 0;
+        }
+        row16 = id * p.tiles_per_block + (tile - jb * p.tiles_per_block);
+      }
+      return row16;
+    };
+    auto issue = [&](int i) {
+      if ((i & 31) == 0) {
+        ids = i == 0 ? load_ids(0) : ids_next;
+        ids_next = load_ids((i >> 5) + 1);
+      }
+      const int row16 = __shfl_sync(0xffffffffu, ids, i & 31);
+      if (i < n_tiles) {
+        const uint32_t st = ring_a + (i % STAGES) * kStage;
+        const int64_t src = static_cast<int64_t>(row16) * 16 * pitch + static_cast<int64_t>(kvh) * D;
+        constexpr int cpr = D / 16;
+#pragma unroll
+        for (int c0_ = 0; c0_ < 16 * cpr; c0_ += 32) {
+          const int c = c0_ + lane, r = c / cpr, ch = c % cpr;
+          cp_async16(st + k_chunk<D>(r, ch), p.k_pool + src + r * pitch + ch * 16);
+          cp_async16(st + 16 * D + v_chunk<D>(r, ch), p.v_pool + src + r * pitch + ch * 16);
+        }
+        if (lane < 2)
+          cp_async4(st + 32 * D + lane * 4, (lane ? p.v_scale : p.k_scale) +
+                    static_cast<int64_t>(row16 / p.tiles_per_block) * p.n_kv_heads + kvh);
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) issue(i);
+
+    int s = d8_find(prefix, B, r0), pos = r0, i = 0;
+    while (pos < r1) {
+      const int seg_end = min(prefix[s + 1], r1);
+      const int ctx = ctxs[s];
+      const bool first = pos == r0;  // the range's first segment
+      // ---- Q^T fragments: column n = g is head head0 + 8 nt + g; k-step kk's
+      // indices 2t, 2t + 1, 2t + 8, 2t + 9 are dims d0 .. d0 + 3
+      uint32_t qb[NT][LIMBS][KS][2];
+      float c_head[NT][2];  // score factor of heads 2t, 2t + 1
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const bool on = 8 * nt + g < nh;
+        const T* row = static_cast<const T*>(p.q) + static_cast<int64_t>(s) * p.q_stride +
+                       static_cast<int64_t>(head0 + 8 * nt + g) * D;
+        float f[KS][4];
+        float amax = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+          const int d0 = (kk >> 2) * 64 + 16 * t + 4 * (kk & 3);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            f[kk][e] = on ? Elem<T>::to_f(row[d0 + e]) : 0.f;
+            amax = fmaxf(amax, fabsf(f[kk][e]));
+          }
+        }
+        float back = 1.f, inv = 1.f;
+        if (!std::is_same<T, __half>::value) {
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+          // 2^E with 2^E <= amax < 2^(E+1) (1 for zero, subnormal or not finite rows)
+          const uint32_t ex = __float_as_uint(amax) >> 23;
+          if (ex >= 2 && ex <= 252) {
+            back = __uint_as_float(ex << 23);
+            inv = __uint_as_float((254u - ex) << 23);
+          }
+        }
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = f[kk][e] * inv;
+          qb[nt][0][kk][0] = pack2<__half>(v[0], v[1]);
+          qb[nt][0][kk][1] = pack2<__half>(v[2], v[3]);
+          if constexpr (LIMBS == 2) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] -= __half2float(__float2half_rn(v[e]));
+            qb[nt][LIMBS - 1][kk][0] = pack2<__half>(v[0], v[1]);
+            qb[nt][LIMBS - 1][kk][1] = pack2<__half>(v[2], v[3]);
+          }
+        }
+        // lanes 4n .. hold head n's factor
+        c_head[nt][0] = p.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * t);
+        c_head[nt][1] = p.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * t + 4);
+      }
+      float m[NT][2], mu[NT][2], l[NT][2], o[NT][KS][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          m[nt][c] = -INFINITY;
+          mu[nt][c] = l[nt][c] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < KS; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+      }
+      float v_ref = 0.f, v_inv = 0.f;  // 2^E and 2^-E (0: no tile yet)
+
+      int left = ctx - (pos - prefix[s]) * 16;  // tokens from this tile on
+      for (; pos < seg_end; ++pos, ++i, left -= 16) {
+        cp_wait<STAGES - 2>();
+        __syncwarp();  // every lane's copies of tile i are in, and every lane is done with tile i - 1
+        issue(i + STAGES - 1);
+        const uint8_t* st = ring + (i % STAGES) * kStage;
+        const float ks = *reinterpret_cast<const float*>(st + 32 * D);
+        const float vs = *reinterpret_cast<const float*>(st + 32 * D + 4);
+        const int valid = min(16, left);
+        // ---- S^T = K Q^T
+        float sc[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+        for (int half = 0; half < D / 64; ++half) {
+          const uint4 k0 = flip(*reinterpret_cast<const uint4*>(st + k_chunk<D>(g, half * 4 + t)));
+          const uint4 k1 = flip(*reinterpret_cast<const uint4*>(st + k_chunk<D>(g + 8, half * 4 + t)));
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+          for (int k4 = 0; k4 < 4; ++k4) {
+            const uint32_t a[4] = {i8_lo(w0[k4]), i8_lo(w1[k4]), i8_hi(w0[k4]), i8_hi(w1[k4])};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int lb = 0; lb < LIMBS; ++lb)
+                mma16816<__half>(sc[nt], a, qb[nt][lb][half * 4 + k4][0], qb[nt][lb][half * 4 + k4][1]);
+          }
+        }
+        // ---- online softmax (exp2), P scaled by V's scale over 2^E
+        bool grow = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float f0 = c_head[nt][0] * ks, f1 = c_head[nt][1] * ks;
+          sc[nt][0] = g < valid ? sc[nt][0] * f0 : -INFINITY;
+          sc[nt][1] = g < valid ? sc[nt][1] * f1 : -INFINITY;
+          sc[nt][2] = g + 8 < valid ? sc[nt][2] * f0 : -INFINITY;
+          sc[nt][3] = g + 8 < valid ? sc[nt][3] * f1 : -INFINITY;
+        }
+        float mx[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mx[nt][0] = fmaxf(sc[nt][0], sc[nt][2]);
+          mx[nt][1] = fmaxf(sc[nt][1], sc[nt][3]);
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) {
+            mx[nt][0] = fmaxf(mx[nt][0], __shfl_xor_sync(0xffffffffu, mx[nt][0], off));
+            mx[nt][1] = fmaxf(mx[nt][1], __shfl_xor_sync(0xffffffffu, mx[nt][1], off));
+          }
+          grow = grow || mx[nt][0] > m[nt][0] + kD8Slack || mx[nt][1] > m[nt][1] + kD8Slack;
+        }
+        const bool wider = vs > v_ref;  // warp-uniform
+        if (wider || __any_sync(0xffffffffu, grow)) {
+          const float vf = wider ? v_ref * (1.f / vs) : 1.f;  // exact
+          if (wider) {
+            v_ref = vs;
+            v_inv = 1.f / vs;
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float cf[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float mn = fmaxf(m[nt][c], mx[nt][c]);
+              const float mun = mn == -INFINITY ? 0.f : mn;
+              cf[c] = ex2_approx(m[nt][c] - mun);
+              m[nt][c] = mn;
+              mu[nt][c] = mun;
+              l[nt][c] *= cf[c];
+              cf[c] *= vf;
+            }
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+              o[nt][j][0] *= cf[0];
+              o[nt][j][1] *= cf[1];
+              o[nt][j][2] *= cf[0];
+              o[nt][j][3] *= cf[1];
+            }
+          }
+        }
+        const float vfac = vs * v_inv;
+        uint32_t pb[NT][LIMBS][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float e[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) e[c] = ex2_approx(sc[nt][c] - mu[nt][c & 1]);
+          l[nt][0] += e[0] + e[2];
+          l[nt][1] += e[1] + e[3];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) e[c] *= vfac;
+          pb[nt][0][0] = movmatrix_t(pack2<__half>(e[0], e[1]));
+          pb[nt][0][1] = movmatrix_t(pack2<__half>(e[2], e[3]));
+          if constexpr (LIMBS == 2) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) e[c] -= __half2float(__float2half_rn(e[c]));
+            pb[nt][LIMBS - 1][0] = movmatrix_t(pack2<__half>(e[0], e[1]));
+            pb[nt][LIMBS - 1][1] = movmatrix_t(pack2<__half>(e[2], e[3]));
+          }
+        }
+        // ---- O^T += V^T P^T: row g of m-tile mt is dim 8g + 2mt (of a half of 64), row g + 8 the next
+        const int sw = t & 1;
+        const uint32_t flip_sel = sw ? 0x4444u : 0u;
+#pragma unroll
+        for (int half = 0; half < D / 64; ++half) {
+          uint2 r[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int row = 2 * t + (k >> 1) * 8 + ((k & 1) ^ sw);
+            r[k] = *reinterpret_cast<const uint2*>(st + 16 * D + v_chunk<D>(row, half * 4 + (g >> 1)) + (g & 1) * 8);
+            r[k].x ^= 0x80808080u;
+            r[k].y ^= 0x80808080u;
+          }
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) {
+            const uint32_t sel = ((mt & 1) ? 0x7362u : 0x5140u) ^ flip_sel;
+            const uint32_t x01 = __byte_perm(mt < 2 ? r[0].x : r[0].y, mt < 2 ? r[1].x : r[1].y, sel);
+            const uint32_t x23 = __byte_perm(mt < 2 ? r[2].x : r[2].y, mt < 2 ? r[3].x : r[3].y, sel);
+            const uint32_t a[4] = {i8_lo(x01), i8_hi(x01), i8_lo(x23), i8_hi(x23)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int lb = 0; lb < LIMBS; ++lb)
+                mma16816<__half>(o[nt][half * 4 + mt], a, pb[nt][lb][0], pb[nt][lb][1]);
+          }
+        }
+      }
+
+      // ---- segment end
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], off);
+      const bool complete = prefix[s] >= r0 && prefix[s + 1] <= r1;
+      if (complete) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int hh = 8 * nt + 2 * t + c;
+            if (hh >= nh) continue;
+            const float f = v_ref / l[nt][c];
+            T* orow = static_cast<T*>(p.out) + static_cast<int64_t>(s) * p.out_stride +
+                      static_cast<int64_t>(head0 + hh) * D;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+              const int d = (j >> 2) * 64 + 8 * g + 2 * (j & 3);
+              orow[d] = Elem<T>::from_f(o[nt][j][c] * f);
+              orow[d + 1] = Elem<T>::from_f(o[nt][j][c + 2] * f);
+            }
+          }
+      } else {
+        // the range's first partial goes to its own slot, a later (last) one
+        // into the ring, which no copy in flight uses any more
+        float* slot = first ? heads_part + warp * kSlot : reinterpret_cast<float*>(ring);
+        if (!first) {
+          cp_wait<0>();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int hh = 8 * nt + 2 * t + c;
+            const float f = v_ref / l[nt][c];  // a partial holds its own softmax's O
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+              const int d = (j >> 2) * 64 + 8 * g + 2 * (j & 3);
+              slot[hh * D + d] = o[nt][j][c] * f;
+              slot[hh * D + d + 1] = o[nt][j][c + 2] * f;
+            }
+            if (g == 0) {
+              slot[kHeads * D + 2 * hh] = m[nt][c];
+              slot[kHeads * D + 2 * hh + 1] = l[nt][c];
+            }
+          }
+        if (lane == 0 && warp == team * p.per_cta) slot_seq[2 * team + (first ? 0 : 1)] = s;
+      }
+      ++s;
+      while (s < B && prefix[s + 1] == prefix[s]) ++s;  // empty sequences
+    }
+    cp_wait<0>();
+  }
+  __syncthreads();
+
+  // ---- join the teams' partials: runs of slots of one sequence, in order
+  const int n_slots = 2 * p.teams;
+  for (int a = 0; a < n_slots;) {
+    const int s = slot_seq[a];
+    if (s < 0) {
+      ++a;
+      continue;
+    }
+    int b = a + 1;
+    while (b < n_slots && (slot_seq[b] == s || slot_seq[b] < 0)) ++b;
+    const bool complete = prefix[s] >= c0 && prefix[s + 1] <= c1;
+    const int64_t part = prefix[s] > c0 ? 2 * blockIdx.x + 1 : 2 * blockIdx.x;
+    const int n_out = p.per_cta * kHeads * D;
+    for (int e = tid; e < n_out; e += WARPS * 32) {
+      const int w = e / (kHeads * D), hh = (e - w * kHeads * D) / D, d = e % D;
+      const int hgw = blockIdx.y * p.per_cta + w;
+      if (hgw >= p.n_groups) continue;
+      const int kv = hgw / p.chunks, hd0 = kv * p.group + (hgw - kv * p.chunks) * kHeads;
+      if (hd0 + hh >= (kv + 1) * p.group) continue;
+      auto slot_of = [&](int k) {
+        const int wp = (k >> 1) * p.per_cta + w;
+        return (k & 1) ? reinterpret_cast<const float*>(d8_smem + wp * kRing) : heads_part + wp * kSlot;
+      };
+      float mm = -INFINITY;
+      for (int k = a; k < b; ++k)
+        if (slot_seq[k] >= 0) mm = fmaxf(mm, slot_of(k)[kHeads * D + 2 * hh]);
+      const float base = mm == -INFINITY ? 0.f : mm;
+      float ll = 0.f, oo = 0.f;
+      for (int k = a; k < b; ++k)
+        if (slot_seq[k] >= 0) {
+          const float* sl = slot_of(k);
+          const float f = ex2_approx(sl[kHeads * D + 2 * hh] - base) * sl[kHeads * D + 2 * hh + 1];
+          ll += f;
+          oo += f * sl[hh * D + d];
+        }
+      const int head = hd0 + hh;
+      if (complete) {
+        static_cast<T*>(p.out)[static_cast<int64_t>(s) * p.out_stride + static_cast<int64_t>(head) * D + d] =
+            Elem<T>::from_f(oo / ll);
+      } else {
+        p.part_o[(part * p.n_q_heads + head) * D + d] = oo / ll;
+        if (d == 0) {
+          p.part_ml[(part * p.n_q_heads + head) * 2] = mm;
+          p.part_ml[(part * p.n_q_heads + head) * 2 + 1] = ll;
+        }
+      }
+    }
+    a = b;
+  }
+}
+
+// Joins the CTAs' partials of sequence blockIdx.x (heads blockIdx.y * heads_per ..):
+// O = sum_c w_c O_c / sum_c w_c, w_c = 2^(m_c - M) l_c, over the CTAs that share it, in
+// order.  16 lanes of partials per head element group; empty sequences get zeros.
+constexpr int kM8Threads = 256;
+template <typename T, int D>
+__global__ void __launch_bounds__(kM8Threads) merge_int8_kernel(const D8Params p, int grid, int heads_per) {
+  constexpr int kVec = D / 4, kLanes = kM8Threads / kVec;  // partials read side by side
+  __shared__ float4 s_o[kLanes][kVec];
+  __shared__ float s_m[kLanes], s_l[kLanes];
+  __shared__ int red[2][kM8Threads / 32];
+  const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  const int64_t room = static_cast<int64_t>(p.max_blocks) * p.tiles_per_block * 16;
+  auto tiles_of = [&](int i) {
+    return static_cast<int>((min(static_cast<int64_t>(max(p.context_lens[i], 0)), room) + 15) >> 4);
+  };
+  int before = 0, total = 0;
+  for (int i = tid; i < p.n_seqs; i += kM8Threads) {
+    const int n = tiles_of(i);
+    total += n;
+    if (i < s) before += n;
+  }
+  before = __reduce_add_sync(0xffffffffu, before);
+  total = __reduce_add_sync(0xffffffffu, total);
+  if (lane == 0) { red[0][warp] = before; red[1][warp] = total; }
+  __syncthreads();
+  before = total = 0;
+#pragma unroll
+  for (int w = 0; w < kM8Threads / 32; ++w) { before += red[0][w]; total += red[1][w]; }
+  const int mine = tiles_of(s);
+  const int per = max((total + grid - 1) / grid, p.teams);
+  const int h0 = blockIdx.y * heads_per, h1 = min(p.n_q_heads, h0 + heads_per);
+  T* orow = static_cast<T*>(p.out) + static_cast<int64_t>(s) * p.out_stride;
+  if (mine == 0) {
+    for (int e = h0 * D + tid; e < h1 * D; e += kM8Threads) orow[e] = Elem<T>::from_f(0.f);
+    return;
+  }
+  const int first = before / per, last = (before + mine - 1) / per;
+  if (first == last) return;  // one CTA had it all and wrote it
+  const int v = tid % kVec, k0 = tid / kVec;
+  for (int h = h0; h < h1; ++h) {
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = first + k0; c <= last; c += kLanes) {
+      const int64_t part = before > c * per ? 2 * static_cast<int64_t>(c) + 1 : 2 * static_cast<int64_t>(c);
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (part * p.n_q_heads + h) * 2);
+      const float4 x = reinterpret_cast<const float4*>(p.part_o + (part * p.n_q_heads + h) * D)[v];
+      const float mn = fmaxf(m, ml.x), base = mn == -INFINITY ? 0.f : mn;
+      const float fa = ex2_approx(m - base), fb = ex2_approx(ml.x - base) * ml.y;
+      m = mn;
+      l = l * fa + fb;
+      o = make_float4(o.x * fa + x.x * fb, o.y * fa + x.y * fb, o.z * fa + x.z * fb, o.w * fa + x.w * fb);
+    }
+    s_o[k0][v] = o;
+    if (v == 0) { s_m[k0] = m; s_l[k0] = l; }
+    __syncthreads();
+    if (k0 == 0) {
+      float mm = -INFINITY;
+      for (int k = 0; k < kLanes; ++k) mm = fmaxf(mm, s_m[k]);
+      const float base = mm == -INFINITY ? 0.f : mm;
+      float ll = 0.f;
+      o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < kLanes; ++k) {
+        const float f = ex2_approx(s_m[k] - base);
+        const float4 x = s_o[k][v];
+        ll += f * s_l[k];
+        o = make_float4(o.x + f * x.x, o.y + f * x.y, o.z + f * x.z, o.w + f * x.w);
+      }
+      T* op = orow + static_cast<int64_t>(h) * D + 4 * v;
+      op[0] = Elem<T>::from_f(o.x / ll);
+      op[1] = Elem<T>::from_f(o.y / ll);
+      op[2] = Elem<T>::from_f(o.z / ll);
+      op[3] = Elem<T>::from_f(o.w / ll);
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, int D, int NT, int WARPS, int STAGES>
+cudaError_t launch_d8(const AttnArgs& a, void* workspace, cudaStream_t stream) {
+  constexpr int LIMBS = std::is_same<T, float>::value ? 2 : 1;
+  auto kern = decode_int8_kernel<T, D, NT, LIMBS, WARPS, STAGES>;
+  constexpr int kFixed = WARPS * (STAGES * d8_stage<D>() + 8 * NT * (D + 2) * 4);
+  constexpr int kMost = kFixed + (2 * kD8MaxSeqs + 1) * 4;
+  static_assert(kMost + 1024 <= 232448, "the rings and partials fit the 227 KB of shared memory");
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+  if (e != cudaSuccess) return e;
+  D8Params p{};
+  p.k_pool = static_cast<const int8_t*>(a.k_pool);
+  p.v_pool = static_cast<const int8_t*>(a.v_pool);
+  p.k_scale = a.k_scale;
+  p.v_scale = a.v_scale;
+  p.bt_stride = a.bt_stride;
+  p.max_blocks = a.max_blocks;
+  p.num_blocks = a.num_blocks;
+  p.tiles_per_block = a.block_size / 16;
+  p.n_q_heads = a.n_q_heads;
+  p.n_kv_heads = a.n_kv_heads;
+  p.group = a.n_q_heads / a.n_kv_heads;
+  p.chunks = (p.group + 8 * NT - 1) / (8 * NT);
+  p.n_groups = p.n_kv_heads * p.chunks;
+  p.per_cta = std::min(p.n_groups, 8);
+  p.teams = WARPS / p.per_cta;
+  p.scale_log2 = a.scale * kD8Log2e;
+  p.out_stride = a.out_stride;
+  p.q_stride = a.q_stride;
+  p.err = a.err;
+  p.part_ml = static_cast<float*>(workspace);
+  p.part_o = p.part_ml + static_cast<size_t>(2) * kD8MaxCtas * p.n_q_heads * 2;
+  const int gy = (p.n_groups + p.per_cta - 1) / p.per_cta;
+  const int gx = std::max(1, std::min(sms, kD8MaxCtas) / gy);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.stream = stream;
+  const int es = sizeof(T);
+  for (int s0 = 0; s0 < a.n_seqs; s0 += kD8MaxSeqs) {
+    p.n_seqs = std::min(kD8MaxSeqs, a.n_seqs - s0);
+    p.out = static_cast<uint8_t*>(a.out) + s0 * a.out_stride * es;
+    p.q = static_cast<const uint8_t*>(a.q) + s0 * a.q_stride * es;
+    p.block_tables = a.block_tables + s0 * a.bt_stride;
+    p.context_lens = a.context_lens + s0;
+    cfg.gridDim = dim3(gx, gy);
+    cfg.blockDim = dim3(WARPS * 32);
+    cfg.dynamicSmemBytes = kFixed + (2 * p.n_seqs + 1) * 4;
+    e = cudaLaunchKernelEx(&cfg, kern, p);
+    if (e != cudaSuccess) return e;
+    const int splits = std::max(1, std::min(p.n_q_heads, 296 / p.n_seqs));
+    const int heads_per = (p.n_q_heads + splits - 1) / splits;
+    cfg.gridDim = dim3(p.n_seqs, (p.n_q_heads + heads_per - 1) / heads_per);
+    cfg.blockDim = dim3(kM8Threads);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, merge_int8_kernel<T, D>, p, gx, heads_per);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+template <typename T>
+cudaError_t launch_d8_t(const AttnArgs& a, void* ws, cudaStream_t stream) {
+  // query heads per warp: 8, or 16 where the group has more (the K and V
+  // fragments are then converted once for both halves)
+  const bool two = a.n_q_heads / a.n_kv_heads > 8;
+  constexpr bool f32 = std::is_same<T, float>::value;
+  if (a.head_dim == 64)
+    return two ? launch_d8<T, 64, 2, f32 ? 8 : 16, f32 ? 6 : 3>(a, ws, stream)
+               : launch_d8<T, 64, 1, 16, 5>(a, ws, stream);
+  return two ? launch_d8<T, 128, 2, 8, 4>(a, ws, stream)
+             : launch_d8<T, 128, 1, f32 ? 8 : 16, f32 ? 4 : 2>(a, ws, stream);
+}
+
+}  // namespace
+
+bool decode_int8_supported(const AttnArgs& a) {
+  return (a.head_dim == 64 || a.head_dim == 128) && a.block_size % 16 == 0;
+}
+
+size_t decode_int8_workspace_bytes(int n_q_heads, int head_dim) {
+  return static_cast<size_t>(2) * kD8MaxCtas * n_q_heads * (head_dim + 2) * 4;
+}
+
+cudaError_t launch_decode_int8(const AttnArgs& a, void* workspace, cudaStream_t stream) {
+  if (a.n_seqs == 0) return cudaSuccess;
+  if (a.dtype == PKV_DTYPE_F16) return launch_d8_t<__half>(a, workspace, stream);
+  if (a.dtype == PKV_DTYPE_BF16) return launch_d8_t<__nv_bfloat16>(a, workspace, stream);
+  return launch_d8_t<float>(a, workspace, stream);
+}
+
+}  // namespace pkv

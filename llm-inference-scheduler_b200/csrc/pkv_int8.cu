@@ -1,0 +1,377 @@
+// pkv_int8.cu -- int8 pools with one power-of-two scale per (block, KV head):
+// the quantising append, the fetch of rows as values, and the pass that lays a
+// step's visible keys and values out for the chunked prefill.
+//
+// The reference keeps 32-bit pools (mini_engine/paged/block_manager.py:37) and
+// names a compact cache as its next step (mini_engine/quant.py); the append
+// replaces the scatter of append_and_fetch (block_manager.py:121-131) and the
+// fetch its gather (block_manager.py:136-141).
+//
+// Format.  Element x of row (block b, offset o, head h) is stored as the integer
+// q = rne(x / s) with s = s[b][h] the smallest power of two 2^e, e >= -120, for
+// which absmax <= 127 s over the block's rows of that head.  With a power of two
+// x / s and q s are exact, so a value is off by at most s / 2 (absmax / 127 at
+// most), dequantising to fp16 / bf16 / fp32 is exact (7 bits), and when a later
+// token needs a larger scale the held integers become rne(q * s_old / s_new),
+// an exact product rounded once; the roundings of a block that grows k times add
+// up to less than one step (1/2 + 1/4 + ...), which no other ratio gives.
+// Infinities are stored as +-127 and do not enter absmax; NaN is stored as 0.
+//
+// Work split of the append and the fetch: one warp per (sequence, touched block,
+// head, K or V), so one warp owns a scale and the rows under it and nothing is
+// atomic.  The host does not know how many blocks each sequence touches, but
+// floor(n / b) + 2 bounds it, so sequence i's units start at
+// floor(start_i / b) + 2 i and a warp finds its sequence by binary search on
+// the start positions: no prefix pass, no scratch.  Bound by the bytes of the
+// rows for prompts, by launch and round trips for decode steps.
+#include <type_traits>
+
+#include "pkv_common.cuh"
+#include "pkv_internal.h"
+
+namespace pkv {
+
+namespace {
+
+constexpr int kI8Warps = 4;
+
+// the block scale for rows of largest finite magnitude amax
+__device__ __forceinline__ float int8_block_scale(float amax) {
+  const uint32_t b = __float_as_uint(amax);
+  // 1.f * 2^E holds amax <= 127 * 2^(E-6) iff 1.f <= 127/64
+  int e = static_cast<int>(b >> 23) - 127 - ((b & 0x7fffffu) <= 0x7e0000u ? 6 : 5);
+  e = max(e, -120);  // zeros and subnormals too
+  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+__device__ __forceinline__ int int8_round(float x, float inv) {
+  return min(127, max(-127, __float2int_rn(x * inv)));  // NaN -> 0, infinities saturate
+}
+__device__ __forceinline__ uint32_t pack_bytes(int a, int b, int c, int d) {
+  return (a & 255) | ((b & 255) << 8) | ((c & 255) << 16) | (static_cast<uint32_t>(d) << 24);
+}
+
+// four consecutive elements; `vec` says whether they may be loaded as one word
+template <typename T>
+__device__ __forceinline__ void load4_any(const T* p, bool vec, float* v) {
+  if (vec) {
+    load4_f<T>(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = Elem<T>::to_f(p[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4_any(T* p, bool vec, const float* v) {
+  if (vec) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = Elem<T>::from_f(v[i]);
+  }
+}
+__device__ __forceinline__ void bytes_to_f(uint32_t w, float* v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
+}
+
+// the sequence and touched-block number of unit u (see the header comment)
+struct Unit {
+  int s, j;        // sequence, number of the touched block
+  int row0, n;     // first packed row of the sequence, rows of the sequence
+  int ctx;         // tokens of the sequence after the call
+};
+__device__ __forceinline__ bool find_unit(const int32_t* start_loc, const int32_t* context_lens,
+                                          int n_seqs, int n_rows, int bs, int64_t u, Unit& w) {
+  int lo = 0, hi = n_seqs - 1;
+  while (lo < hi) {
+    const int m = (lo + hi + 1) >> 1;
+    if (start_loc[m] / bs + 2 * static_cast<int64_t>(m) <= u) lo = m; else hi = m - 1;
+  }
+  w.s = lo;
+  w.row0 = start_loc[lo];
+  w.j = static_cast<int>(u - (w.row0 / bs + 2 * static_cast<int64_t>(lo)));
+  w.n = start_loc[lo + 1] - w.row0;
+  w.ctx = context_lens[lo];
+  return w.row0 >= 0 && w.n > 0 && w.j >= 0 && w.row0 + static_cast<int64_t>(w.n) <= n_rows;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kI8Warps * 32) append_int8_kernel(const Int8RowsArgs a) {
+  pdl_trigger();
+  pdl_wait();  // the metadata and the rows may come from the kernel before this one
+  const int lane = threadIdx.x & 31;
+  const int64_t wid = static_cast<int64_t>(blockIdx.x) * kI8Warps + (threadIdx.x >> 5);
+  const int per_unit = 2 * a.n_kv_heads;
+  const int64_t u = wid / per_unit;
+  const int rem = static_cast<int>(wid - u * per_unit);
+  const bool isv = rem >= a.n_kv_heads;
+  const int h = isv ? rem - a.n_kv_heads : rem;
+  const int bs = a.block_size, D = a.head_dim;
+  if (u >= a.n_units) return;
+  Unit w;
+  if (!find_unit(a.start_loc, a.context_lens, a.n_seqs, a.n_rows, bs, u, w)) {
+    if (w.j == 0 && rem == 0 && lane == 0 &&
+        (w.row0 < 0 || w.n < 0 || w.row0 + static_cast<int64_t>(w.n) > a.n_rows))
+      raise_flag(a.err, PKV_FLAG_BAD_QUERY_LAYOUT);
+    return;
+  }
+  if (w.ctx == 0) return;  // a padding or unserved sequence: nothing is written
+  const int prior = w.ctx - w.n;
+  if (prior < 0) {
+    if (w.j == 0 && rem == 0 && lane == 0) raise_flag(a.err, PKV_FLAG_BAD_QUERY_LAYOUT);
+    return;
+  }
+  const int jb = prior / bs + w.j;  // table column
+  const int64_t blk0 = static_cast<int64_t>(jb) * bs;
+  if (blk0 >= w.ctx) return;
+  if (jb >= a.max_blocks) {
+    if (rem == 0 && lane == 0) raise_flag(a.err, PKV_FLAG_CONTEXT_EXCEEDS_TABLE);
+    return;
+  }
+  const int id = a.block_tables[static_cast<int64_t>(w.s) * a.bt_stride + jb];
+  if (id < 0 || id >= a.num_blocks) {
+    if (rem == 0 && lane == 0) raise_flag(a.err, PKV_FLAG_BLOCK_OUT_OF_RANGE);
+    return;
+  }
+  const int held = max(0, prior - static_cast<int>(blk0));                // rows the block keeps
+  const int end = min(bs, static_cast<int>(w.ctx - blk0));                // rows after the call
+  const int src0 = w.row0 + static_cast<int>(blk0) + held - prior;        // packed row of row `held`
+  const T* src = static_cast<const T*>(isv ? a.v : a.k) +
+                 static_cast<int64_t>(src0) * (isv ? a.v_stride : a.k_stride) + static_cast<int64_t>(h) * D;
+  const int64_t stride = isv ? a.v_stride : a.k_stride;
+  const bool vec = isv ? a.v_vec : a.k_vec;
+  int8_t* dst = static_cast<int8_t*>(isv ? a.v_pool : a.k_pool) +
+                (static_cast<int64_t>(id) * bs * a.n_kv_heads + h) * D;
+  const int64_t pitch = static_cast<int64_t>(a.n_kv_heads) * D;
+  float* scale = (isv ? a.v_scale : a.k_scale) + static_cast<int64_t>(id) * a.n_kv_heads + h;
+
+  // units of four consecutive elements: cpr to a row
+  const int cpr = D / 4, total = (end - held) * cpr;
+  float amax = 0.f;
+  for (int c = lane; c < total; c += 32) {
+    const int r = c / cpr, d = (c - r * cpr) * 4;
+    float v[4];
+    load4_any<T>(src + r * stride + d, vec, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float m = fabsf(v[i]);
+      amax = fmaxf(amax, m < INFINITY ? m : 0.f);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  float sc = int8_block_scale(amax);
+  if (held > 0) {
+    const float old = *scale;
+    sc = fmaxf(sc, old);
+    if (sc != old) {  // the held rows on the larger scale
+      const float ratio = old * (1.f / sc);
+      for (int c = lane; c < held * cpr; c += 32) {
+        const int r = c / cpr, d = (c - r * cpr) * 4;
+        uint32_t* p = reinterpret_cast<uint32_t*>(dst + r * pitch + d);
+        float v[4];
+        bytes_to_f(*p, v);
+        *p = pack_bytes(int8_round(v[0], ratio), int8_round(v[1], ratio), int8_round(v[2], ratio),
+                        int8_round(v[3], ratio));
+      }
+    }
+  }
+  const float inv = 1.f / sc;  // exact: a power of two
+  for (int c = lane; c < total; c += 32) {
+    const int r = c / cpr, d = (c - r * cpr) * 4;
+    float v[4];
+    load4_any<T>(src + r * stride + d, vec, v);
+    *reinterpret_cast<uint32_t*>(dst + (held + r) * pitch + d) =
+        pack_bytes(int8_round(v[0], inv), int8_round(v[1], inv), int8_round(v[2], inv), int8_round(v[3], inv));
+  }
+  __syncwarp();
+  if (lane == 0) *scale = sc;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kI8Warps * 32) fetch_int8_kernel(const Int8RowsArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t wid = static_cast<int64_t>(blockIdx.x) * kI8Warps + (threadIdx.x >> 5);
+  const int per_unit = 2 * a.n_kv_heads;
+  const int64_t u = wid / per_unit;
+  const int rem = static_cast<int>(wid - u * per_unit);
+  const bool isv = rem >= a.n_kv_heads;
+  const int h = isv ? rem - a.n_kv_heads : rem;
+  const int bs = a.block_size, D = a.head_dim;
+  if (u >= a.n_units) return;
+  Unit w;
+  if (!find_unit(a.start_loc, a.context_lens, a.n_seqs, a.n_rows, bs, u, w)) {
+    if (w.j == 0 && rem == 0 && lane == 0 &&
+        (w.row0 < 0 || w.n < 0 || w.row0 + static_cast<int64_t>(w.n) > a.n_rows))
+      raise_flag(a.err, PKV_FLAG_BAD_QUERY_LAYOUT);
+    return;
+  }
+  const int from = w.ctx - w.n;  // first position fetched
+  if (from < 0) {
+    if (w.j == 0 && rem == 0 && lane == 0) raise_flag(a.err, PKV_FLAG_BAD_QUERY_LAYOUT);
+    return;
+  }
+  const int jb = from / bs + w.j;
+  const int64_t blk0 = static_cast<int64_t>(jb) * bs;
+  if (blk0 >= w.ctx) return;
+  if (jb >= a.max_blocks) {
+    if (rem == 0 && lane == 0) raise_flag(a.err, PKV_FLAG_CONTEXT_EXCEEDS_TABLE);
+    return;
+  }
+  const int id = a.block_tables[static_cast<int64_t>(w.s) * a.bt_stride + jb];
+  if (id < 0 || id >= a.num_blocks) {
+    if (rem == 0 && lane == 0) raise_flag(a.err, PKV_FLAG_BLOCK_OUT_OF_RANGE);
+    return;
+  }
+  const int r0 = max(0, from - static_cast<int>(blk0));
+  const int r1 = min(bs, static_cast<int>(w.ctx - blk0));
+  const int64_t out0 = w.row0 + (blk0 + r0 - from);
+  const int64_t stride = isv ? a.v_stride : a.k_stride;
+  T* dst = static_cast<T*>(const_cast<void*>(isv ? a.v : a.k)) + out0 * stride + static_cast<int64_t>(h) * D;
+  const bool vec = isv ? a.v_vec : a.k_vec;
+  const int64_t pitch = static_cast<int64_t>(a.n_kv_heads) * D;
+  const int8_t* src = static_cast<const int8_t*>(isv ? a.v_pool : a.k_pool) +
+                      (static_cast<int64_t>(id) * bs * a.n_kv_heads + h) * D + r0 * pitch;
+  const float sc = (isv ? a.v_scale : a.k_scale)[static_cast<int64_t>(id) * a.n_kv_heads + h];
+  const int cpr = D / 4, total = (r1 - r0) * cpr;
+  for (int c = lane; c < total; c += 32) {
+    const int r = c / cpr, d = (c - r * cpr) * 4;
+    float v[4];
+    bytes_to_f(*reinterpret_cast<const uint32_t*>(src + r * pitch + d), v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] *= sc;
+    store4_any<T>(dst + r * stride + d, vec, v);
+  }
+}
+
+// Rows 16 j .. 16 j + 15 of sequence s (CTA (j, s)) as values, all heads, K and
+// V, into row s * cap + 16 j of k_out / v_out [n_seqs * cap][n_kv_heads][D], so
+// that a sequence's visible keys are consecutive rows.  Rows past its last key
+// are zeros up to the next multiple of 128 (the attention kernel's key tile):
+// a tile holds no stale bytes.
+template <typename T>
+__global__ void __launch_bounds__(128) lay_out_int8_kernel(const Int8LayArgs a) {
+  pdl_trigger();
+  pdl_wait();  // the append before it writes the pools; an earlier layer may still read the scratch
+  const int j = blockIdx.x, s = blockIdx.y, bs = a.block_size;
+  const int new_rows = a.query_start_loc[s + 1] - a.query_start_loc[s];
+  int64_t keys = static_cast<int64_t>(max(a.num_prior[s], 0)) + max(new_rows, 0);
+  if (keys > static_cast<int64_t>(a.max_blocks) * bs) {
+    if (j == 0 && threadIdx.x == 0) raise_flag(a.err, PKV_FLAG_CONTEXT_EXCEEDS_TABLE);
+    keys = static_cast<int64_t>(a.max_blocks) * bs;
+  }
+  const int64_t row0 = static_cast<int64_t>(j) * 16;
+  if (row0 >= (keys + 127) / 128 * 128) return;
+  const int jb = static_cast<int>(row0 / bs);
+  int id = -1;
+  if (row0 < keys) {
+    id = a.block_tables[static_cast<int64_t>(s) * a.bt_stride + jb];
+    if (id < 0 || id >= a.num_blocks) {
+      if (threadIdx.x == 0) raise_flag(a.err, PKV_FLAG_BLOCK_OUT_OF_RANGE);
+      id = -1;
+    }
+  }
+  const int valid = id < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(16), keys - row0));
+  const int pitch = a.n_kv_heads * a.head_dim;       // elements of a row
+  const int chunks = pitch / 16;                     // 16 elements at a time
+  const int64_t src0 = (static_cast<int64_t>(id < 0 ? 0 : id) * bs + row0 % bs) * pitch;
+  const int64_t dst0 = (static_cast<int64_t>(s) * a.cap + row0) * pitch;
+  for (int c = threadIdx.x; c < 2 * 16 * chunks; c += blockDim.x) {
+    const bool isv = c >= 16 * chunks;
+    const int cc = isv ? c - 16 * chunks : c;
+    const int r = cc / chunks, e = (cc - r * chunks) * 16;
+    T* dst = static_cast<T*>(isv ? a.v_out : a.k_out) + dst0 + static_cast<int64_t>(r) * pitch + e;
+    float v[16];
+    if (r < valid) {
+      const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const int8_t*>(isv ? a.v_pool : a.k_pool) +
+                                                      src0 + static_cast<int64_t>(r) * pitch + e);
+      const float sc = (isv ? a.v_scale : a.k_scale)[static_cast<int64_t>(id) * a.n_kv_heads + e / a.head_dim];
+      bytes_to_f(w.x, v), bytes_to_f(w.y, v + 4), bytes_to_f(w.z, v + 8), bytes_to_f(w.w, v + 12);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] *= sc;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = 0.f;
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        reinterpret_cast<uint4*>(dst)[i] =
+            make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
+                       pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
+    }
+  }
+}
+
+template <typename K>
+cudaError_t launch_rows(K f16, K bf16, K f32, Int8RowsArgs a, cudaStream_t stream) {
+  const int64_t warps = a.n_units * 2 * a.n_kv_heads;
+  const int64_t grid = (warps + kI8Warps - 1) / kI8Warps;
+  if (grid == 0) return cudaSuccess;
+  if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kI8Warps * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  K kern = a.dtype == PKV_DTYPE_F16 ? f16 : a.dtype == PKV_DTYPE_BF16 ? bf16 : f32;
+  return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+// may four consecutive elements of these rows be one access?
+bool rows_vec(const void* p, int64_t stride, int esize) {
+  return ((reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride * esize)) & (4 * esize - 1)) == 0;
+}
+
+void fill_rows(Int8RowsArgs& a) {
+  const int es = a.dtype == PKV_DTYPE_F32 ? 4 : 2;
+  a.k_vec = rows_vec(a.k, a.k_stride, es);
+  a.v_vec = rows_vec(a.v, a.v_stride, es);
+  a.n_units = a.n_rows / a.block_size + 2 * static_cast<int64_t>(a.n_seqs);
+}
+
+}  // namespace
+
+cudaError_t launch_append_int8(Int8RowsArgs a, cudaStream_t stream) {
+  fill_rows(a);
+  return launch_rows(append_int8_kernel<__half>, append_int8_kernel<__nv_bfloat16>,
+                     append_int8_kernel<float>, a, stream);
+}
+
+cudaError_t launch_fetch_int8(Int8RowsArgs a, cudaStream_t stream) {
+  fill_rows(a);
+  return launch_rows(fetch_int8_kernel<__half>, fetch_int8_kernel<__nv_bfloat16>,
+                     fetch_int8_kernel<float>, a, stream);
+}
+
+cudaError_t launch_lay_out_int8(const Int8LayArgs& a, int dtype, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.cap / 16, a.n_seqs);
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (dtype == PKV_DTYPE_F16) return cudaLaunchKernelEx(&cfg, lay_out_int8_kernel<__half>, a);
+  if (dtype == PKV_DTYPE_BF16) return cudaLaunchKernelEx(&cfg, lay_out_int8_kernel<__nv_bfloat16>, a);
+  return cudaLaunchKernelEx(&cfg, lay_out_int8_kernel<float>, a);
+}
+
+}  // namespace pkv

@@ -165,6 +165,94 @@ cudaError_t launch_prefill_fast(const AttnArgs& a, const CUtensorMap* qmap, cons
 int encode_q_tensormap(CUtensorMap* map, const void* q, int64_t q_stride, int n_tokens,
                        int n_q_heads, int head_dim, int dtype);
 
+// ---- step tables (pkv_step_tables.cu)
+constexpr int kStepTablesMaxSeqs = 16384;
+struct StepTablesArgs {
+  int32_t* block_tables;  // [n_seqs][bt_stride], new entries written
+  int64_t bt_stride;
+  int max_blocks;
+  const int32_t* free_blocks;  // [free_capacity], taken from the end
+  int free_capacity;
+  const int32_t* n_free;
+  int32_t* n_free_out;
+  const int32_t* num_prior;
+  const int32_t* num_new;
+  int n_seqs, block_size;
+  int32_t* context_lens;
+  int32_t* query_start_loc;  // [n_seqs + 1]
+  int64_t* slot_mapping;     // [n_tokens]
+  int64_t* positions;        // [n_tokens]
+  int n_tokens;
+  int* err;
+  int vec_ok;  // slot_mapping and positions take 16-byte stores (set by the launcher)
+};
+cudaError_t launch_step_tables(StepTablesArgs a, cudaStream_t stream);
+
+// ---- int8 pools with a scale per (block, KV head) (pkv_int8.cu, pkv_decode_int8.cu)
+struct Int8RowsArgs {
+  const void* k;  // append: the new rows; fetch: the output rows
+  const void* v;
+  int64_t k_stride, v_stride;  // elements between rows
+  void* k_pool;
+  void* v_pool;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* block_tables;
+  int64_t bt_stride;
+  int max_blocks;
+  const int32_t* context_lens;
+  const int32_t* start_loc;  // [n_seqs + 1]: the last start_loc[i + 1] - start_loc[i] rows of context i
+  int n_seqs, n_rows, num_blocks, block_size, n_kv_heads, head_dim, dtype;
+  int* err;
+  int k_vec, v_vec;  // set by the launcher
+  int64_t n_units;
+};
+cudaError_t launch_append_int8(Int8RowsArgs a, cudaStream_t stream);
+cudaError_t launch_fetch_int8(Int8RowsArgs a, cudaStream_t stream);
+struct Int8LayArgs {
+  const void* k_pool;
+  const void* v_pool;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* block_tables;
+  int64_t bt_stride;
+  int max_blocks;
+  const int32_t* query_start_loc;
+  const int32_t* num_prior;
+  int n_seqs, num_blocks, block_size, n_kv_heads, head_dim;
+  void* k_out;
+  void* v_out;
+  int cap;  // rows per sequence in k_out / v_out, a multiple of 128
+  int* err;
+};
+cudaError_t launch_lay_out_int8(const Int8LayArgs& a, int dtype, cudaStream_t stream);
+// AttnArgs with k_scale / v_scale per (block, KV head); decode form
+bool decode_int8_supported(const AttnArgs& a);
+size_t decode_int8_workspace_bytes(int n_q_heads, int head_dim);
+cudaError_t launch_decode_int8(const AttnArgs& a, void* workspace, cudaStream_t stream);
+
+// ---- causal attention over consecutive rows (pkv_packed.cu)
+struct PackedArgs {
+  void* out;
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t out_stride, q_stride, k_stride, v_stride;  // elements between token rows
+  const int32_t* query_start_loc;
+  // NULL: the keys of sequence s are its own rows query_start_loc[s] .. (a
+  // whole prompt).  Otherwise they are rows s * key_cap .. of k / v, num_prior[s]
+  // of them before the first query.
+  const int32_t* num_prior;
+  int key_cap;
+  int key_limit;   // keys a sequence's table can hold
+  int n_key_rows;  // rows of k / v
+  int n_seqs, n_tokens, n_q_heads, n_kv_heads, head_dim;
+  float scale;
+  int dtype;
+  int* err;
+};
+cudaError_t launch_packed_attention(const PackedArgs& a, cudaStream_t stream);
+
 // Argument checks, TMA-descriptor cache and kernel selection of pkv_abi.cu,
 // reused by the allocation-free decode entry point.
 int validate_attention_args(const void* out, int64_t out_stride, const void* q, int64_t q_stride,

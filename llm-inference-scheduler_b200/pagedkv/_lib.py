@@ -37,6 +37,7 @@ FLAG_PIPELINE_TIMEOUT = 8
 FLAG_BAD_QUERY_LAYOUT = 16
 FLAG_POSITION_OUT_OF_RANGE = 32
 FLAG_BAD_SCHEDULE = 64
+FLAG_OUT_OF_BLOCKS = 128
 
 DECODE_AUTO = 0
 DECODE_GENERIC = 1
@@ -99,6 +100,20 @@ SIGNATURES: dict = {
                                                             _P, _I64, _I64, _I64, _P, _P, _I64, _I, _P,
                                                             _I64, _I, _P, _I, _I, _I, _I, _I, _F, _I,
                                                             _P, _SZ, _P, _P, _P, _P, _I]),
+    "pkv_build_step_tables": (_I, [_P, _I64, _I, _P, _I, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _I,
+                                   _P, _P]),
+    "pkv_reshape_and_cache_int8": (_I, [_P, _P, _I64, _I64, _P, _P, _P, _P, _I, _P, _I64, _I, _P, _P,
+                                        _I, _I, _I, _I, _I, _I, _P, _P]),
+    "pkv_fetch_int8": (_I, [_P, _P, _I64, _I64, _P, _P, _P, _P, _I, _P, _I64, _I, _P, _P, _I, _I, _I,
+                            _I, _I, _I, _P, _P]),
+    "pkv_decode_int8_workspace_bytes": (_SZ, [_I, _I]),
+    "pkv_paged_decode_attention_int8": (_I, [_P, _I64, _P, _I64, _P, _P, _P, _P, _I, _P, _I64, _I, _P,
+                                             _I, _I, _I, _I, _I, _F, _I, _P, _SZ, _P, _P]),
+    "pkv_prefill_int8_scratch_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
+    "pkv_paged_prefill_attention_int8": (_I, [_P, _I64, _P, _I64, _P, _P, _P, _P, _I, _P, _I64, _I, _P,
+                                              _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _SZ, _P, _P]),
+    "pkv_packed_prompt_attention": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I, _I, _I, _I, _I,
+                                         _F, _I, _P, _P]),
 }
 
 

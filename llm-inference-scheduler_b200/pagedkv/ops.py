@@ -10,6 +10,7 @@ pagedkv._lib.FLAG_*), which callers check with `check_flags` after a sync.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -997,3 +998,321 @@ def bind_paged_decode_attention_fp8(q, k_pool, v_pool, k_scale, v_scale, block_t
                        _sched_args(args, schedule), "pkv_paged_decode_attention_fp8",
                        (q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, workspace,
                         out, err, schedule))
+
+
+# ---------------------------------------------------------------- step tables on the GPU
+
+def _call(name: str, t: torch.Tensor, *args) -> None:
+    """One C call on t's device and its current stream (the last argument)."""
+    fn = getattr(_lib.load(), name)
+    dev = t.get_device()
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(t))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(t))
+    if rc:
+        _lib.check(rc, name)
+
+
+def _same_device(t: torch.Tensor, **others) -> None:
+    """Every tensor on t's CUDA device (None entries are skipped)."""
+    for name, o in others.items():
+        if o is not None and _cuda(o, name).device != t.device:
+            raise ValueError(f"pagedkv: `{name}` is on {o.device}, expected {t.device}")
+
+
+def _check_err(err: torch.Tensor | None) -> None:
+    if err is not None and (err.dtype != torch.int32 or err.numel() < 1):
+        raise TypeError("pagedkv: err must be an int32 tensor of one element")
+
+
+def _int_row(t: torch.Tensor, name: str, n: int, dtype=torch.int32) -> None:
+    """t is a contiguous 1-D tensor of at least n elements of dtype."""
+    if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous():
+        raise TypeError(f"pagedkv: {name} must be a contiguous {str(dtype)[6:]} tensor")
+    if t.shape[0] < n:
+        raise ValueError(f"pagedkv: {name} has {t.shape[0]} entries, {n} are needed")
+
+
+class StepTables(NamedTuple):
+    """A step's metadata as build_step_tables writes it (device tensors)."""
+
+    context_lens: torch.Tensor     # int32 [B]: prior + new (0: not served)
+    query_start_loc: torch.Tensor  # int32 [B + 1]
+    slot_mapping: torch.Tensor     # int64 [n_tokens], -1 where no token is stored
+    positions: torch.Tensor        # int64 [n_tokens]
+    n_free: torch.Tensor           # int32 [1]: blocks left in the free list
+
+
+def new_step_tables(n_seqs: int, n_tokens: int, device) -> StepTables:
+    """Buffers of build_step_tables for up to n_seqs requests and n_tokens
+    tokens, for a caller that fills the same ones every step (a captured one)."""
+    return StepTables(torch.empty(n_seqs, dtype=torch.int32, device=device),
+                      torch.empty(n_seqs + 1, dtype=torch.int32, device=device),
+                      torch.empty(n_tokens, dtype=torch.int64, device=device),
+                      torch.empty(n_tokens, dtype=torch.int64, device=device),
+                      torch.empty(1, dtype=torch.int32, device=device))
+
+
+def build_step_tables(block_tables: torch.Tensor, free_blocks: torch.Tensor, n_free: torch.Tensor,
+                      num_prior: torch.Tensor, num_new: torch.Tensor, block_size: int,
+                      n_tokens: int, out: StepTables | None = None,
+                      err: torch.Tensor | None = None) -> StepTables:
+    """The step's block tables, slot map, positions and lengths from request
+    lengths that live on the GPU (pkv_build_step_tables, one launch).
+
+    block_tables: int32 [B, W], request i's blocks in row i; the blocks that
+    its new tokens open are written into it.  free_blocks: int32 ids, the first
+    n_free[0] of them free, taken from the end in request order (the order in
+    which BlockManager.allocate pops).  num_prior, num_new: int32 [B].
+    n_tokens: rows of the batch (at least the sum of num_new; further rows get
+    slot -1).  The free count after the step is in the result's n_free, another
+    tensor than the one passed in; pass it to the next step.
+
+    A request the free list is too short for sets PKV_FLAG_OUT_OF_BLOCKS in
+    err; it and those after it get slots -1 and context length 0 and take no
+    block.  Reference: scheduler.py:79-156 and block_manager.py:121-131 (host)."""
+    _check_tables(block_tables)
+    _same_device(block_tables, free_blocks=free_blocks, n_free=n_free, num_prior=num_prior,
+                 num_new=num_new, err=err)
+    _check_err(err)
+    B = num_prior.shape[0]
+    _int_row(num_prior, "num_prior", B), _int_row(num_new, "num_new", B)
+    if num_new.shape[0] != B or block_tables.shape[0] < B:
+        raise ValueError("pagedkv: num_prior, num_new and block_tables disagree on the requests")
+    _int_row(free_blocks, "free_blocks", 0), _int_row(n_free, "n_free", 1)
+    if out is None:
+        out = new_step_tables(B, n_tokens, block_tables.device)
+    else:
+        _same_device(block_tables, **out._asdict())
+        _int_row(out.context_lens, "context_lens", B)
+        _int_row(out.query_start_loc, "query_start_loc", B + 1)
+        _int_row(out.slot_mapping, "slot_mapping", n_tokens, torch.int64)
+        _int_row(out.positions, "positions", n_tokens, torch.int64)
+        _int_row(out.n_free, "out.n_free", 1)
+        if out.n_free.data_ptr() == n_free.data_ptr():
+            raise ValueError("pagedkv: the new free count needs a tensor of its own")
+    _call("pkv_build_step_tables", block_tables, block_tables.data_ptr(), block_tables.stride(0),
+          block_tables.shape[1], free_blocks.data_ptr(), free_blocks.shape[0], n_free.data_ptr(),
+          out.n_free.data_ptr(), num_prior.data_ptr(), num_new.data_ptr(), B, int(block_size),
+          out.context_lens.data_ptr(), out.query_start_loc.data_ptr(), out.slot_mapping.data_ptr(),
+          out.positions.data_ptr(), int(n_tokens), _ptr(err))
+    return out
+
+
+# ---------------------------------------------------------------- int8 pools, a scale per (block, KV head)
+
+def _check_int8_pools(k_pool, v_pool, k_scale, v_scale, **others):
+    """Shapes, types and devices of int8 pools and their scales; returns
+    (num_blocks, block_size, n_kv_heads, head_dim)."""
+    _cuda(k_pool, "k_pool")
+    _same_device(k_pool, v_pool=v_pool, k_scale=k_scale, v_scale=v_scale, **others)
+    if k_pool.dtype != torch.int8 or v_pool.dtype != torch.int8:
+        raise TypeError("pagedkv: int8 pools are int8 tensors")
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise TypeError("pagedkv: int8 pool scales are float32")
+    if not all(t.is_contiguous() for t in (k_pool, v_pool, k_scale, v_scale)):
+        raise ValueError("pagedkv: pools and scales must be contiguous")
+    if k_pool.dim() != 4 or k_pool.shape != v_pool.shape:
+        raise ValueError("pagedkv: pools must be [num_blocks, block_size, n_kv_heads, head_dim]")
+    nb, bs, hkv, d = k_pool.shape
+    if tuple(k_scale.shape) != (nb, hkv) or tuple(v_scale.shape) != (nb, hkv):
+        raise ValueError("pagedkv: int8 pool scales must be [num_blocks, n_kv_heads]")
+    return nb, bs, hkv, d
+
+
+def _check_rows_of(block_tables, context_lens, start_loc, name):
+    """Block tables, context lengths and row starts of the same sequences."""
+    _check_tables(block_tables)
+    n_seqs = start_loc.shape[0] - 1
+    if n_seqs < 0:
+        raise ValueError(f"pagedkv: {name} holds n_seqs + 1 entries")
+    _int_row(start_loc, name, n_seqs + 1), _int_row(context_lens, "context_lens", n_seqs)
+    if block_tables.shape[0] < n_seqs:
+        raise ValueError("pagedkv: block_tables has fewer rows than sequences")
+    return n_seqs
+
+
+def reshape_and_cache_int8(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor,
+                           v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                           block_tables: torch.Tensor, context_lens: torch.Tensor,
+                           query_start_loc: torch.Tensor, err: torch.Tensor | None = None) -> None:
+    """Append k, v [T, Hkv, D] to int8 pools with one power-of-two scale per
+    (block, KV head): rows query_start_loc[i] .. query_start_loc[i + 1] become
+    the last tokens of context i (context_lens counts them).
+
+    k_pool, v_pool: int8 [NB, bs, Hkv, D]; k_scale, v_scale: float32 [NB, Hkv].
+    scale = the smallest 2^e (e >= -120) with absmax <= 127 * 2^e over the
+    block's rows of the head, byte = round(x / scale).  A block that goes on
+    keeps its rows, requantised when the new ones need a larger scale.
+    Reference: block_manager.py:121-131 (unquantised)."""
+    nb, bs, hkv, d = _check_int8_pools(k_pool, v_pool, k_scale, v_scale, k=k, v=v, err=err,
+                                       block_tables=block_tables, context_lens=context_lens,
+                                       query_start_loc=query_start_loc)
+    _check_err(err)
+    n_seqs = _check_rows_of(block_tables, context_lens, query_start_loc, "query_start_loc")
+    if k.dtype != v.dtype:
+        raise TypeError("pagedkv: k and v must share one dtype")
+    T = k.shape[0]
+    if tuple(k.shape[1:]) != (hkv, d) or k.shape != v.shape:
+        raise ValueError("pagedkv: k / v must be [tokens, n_kv_heads, head_dim] as the pools")
+    code = dtype_code(k.dtype)
+    if T == 0 or n_seqs == 0:
+        return
+    _call("pkv_reshape_and_cache_int8", k, k.data_ptr(), v.data_ptr(), _row_stride(k, "k"),
+          _row_stride(v, "v"), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
+          v_scale.data_ptr(), nb, block_tables.data_ptr(), block_tables.stride(0),
+          block_tables.shape[1], context_lens.data_ptr(), query_start_loc.data_ptr(), n_seqs, T, hkv,
+          d, bs, code, _ptr(err))
+
+
+def fetch_int8(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
+               v_scale: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
+               row_start_loc: torch.Tensor, n_rows: int, dtype: torch.dtype,
+               err: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The last row_start_loc[i + 1] - row_start_loc[i] rows of each context as
+    values of `dtype`: (K, V), each [n_rows, Hkv, D], one sequence behind the
+    other (rows past row_start_loc[-1] are left as allocated).  Reference: the
+    gather of append_and_fetch, block_manager.py:136-141."""
+    nb, bs, hkv, d = _check_int8_pools(k_pool, v_pool, k_scale, v_scale, err=err,
+                                       block_tables=block_tables, context_lens=context_lens,
+                                       row_start_loc=row_start_loc)
+    _check_err(err)
+    n_seqs = _check_rows_of(block_tables, context_lens, row_start_loc, "row_start_loc")
+    code = dtype_code(dtype)
+    k = torch.empty((n_rows, hkv, d), dtype=dtype, device=k_pool.device)
+    v = torch.empty((n_rows, hkv, d), dtype=dtype, device=k_pool.device)
+    if n_rows == 0 or n_seqs == 0:
+        return k, v
+    _call("pkv_fetch_int8", k, k.data_ptr(), v.data_ptr(), hkv * d, hkv * d, k_pool.data_ptr(),
+          v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), nb, block_tables.data_ptr(),
+          block_tables.stride(0), block_tables.shape[1], context_lens.data_ptr(),
+          row_start_loc.data_ptr(), n_seqs, int(n_rows), hkv, d, bs, code, _ptr(err))
+    return k, v
+
+
+def decode_int8_workspace_bytes(n_q_heads: int, head_dim: int) -> int:
+    return int(_lib.load().pkv_decode_int8_workspace_bytes(n_q_heads, head_dim))
+
+
+def _bytes_of(t: torch.Tensor, name: str) -> int:
+    if not t.is_contiguous():
+        raise ValueError(f"pagedkv: {name} must be contiguous")
+    return t.numel() * t.element_size()
+
+
+def _like_q(out, q):
+    """The output rows: allocated, or the caller's checked against q."""
+    if out is None:
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
+    if out.dtype != q.dtype or out.shape != q.shape:
+        raise ValueError("pagedkv: out must have q's shape and dtype")
+    return out
+
+
+def paged_decode_attention_int8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                                k_scale: torch.Tensor, v_scale: torch.Tensor,
+                                block_tables: torch.Tensor, context_lens: torch.Tensor, scale: float,
+                                workspace: torch.Tensor | None = None,
+                                out: torch.Tensor | None = None,
+                                err: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_decode_attention over int8 pools with a scale per (block, KV
+    head): q [B, Hq, D] in float32, float16 or bfloat16 -> [B, Hq, D]; a
+    context of length 0 gives a zero row.  workspace: a byte buffer of
+    decode_int8_workspace_bytes (any contents; allocated here when None).
+    Reference: block_manager.py:136-141 + qwen2.py:98-128 (num_new == 1)."""
+    nb, bs, hkv, d = _check_int8_pools(k_pool, v_pool, k_scale, v_scale, q=q, err=err, out=out,
+                                       block_tables=block_tables, context_lens=context_lens,
+                                       workspace=workspace)
+    _check_tables(block_tables), _check_err(err)
+    B, hq, dq = q.shape
+    _int_row(context_lens, "context_lens", B)
+    if dq != d or hq % hkv or block_tables.shape[0] < B:
+        raise ValueError("pagedkv: q / pools / block_tables shapes disagree")
+    code = dtype_code(q.dtype)
+    out = _like_q(out, q)
+    if B == 0:
+        return out
+    if workspace is None:
+        workspace = torch.empty(decode_int8_workspace_bytes(hq, d), dtype=torch.uint8, device=q.device)
+    _call("pkv_paged_decode_attention_int8", q, out.data_ptr(), _row_stride(out, "out"), q.data_ptr(),
+          _row_stride(q, "q"), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
+          v_scale.data_ptr(), nb, block_tables.data_ptr(), block_tables.stride(0),
+          block_tables.shape[1], context_lens.data_ptr(), B, hq, hkv, d, bs, float(scale), code,
+          workspace.data_ptr(), _bytes_of(workspace, "workspace"), _ptr(err))
+    return out
+
+
+def prefill_int8_scratch_bytes(n_seqs: int, max_blocks_per_seq: int, n_kv_heads: int, head_dim: int,
+                               block_size: int, dtype: torch.dtype) -> int:
+    return int(_lib.load().pkv_prefill_int8_scratch_bytes(n_seqs, max_blocks_per_seq, n_kv_heads,
+                                                          head_dim, block_size, dtype_code(dtype)))
+
+
+def paged_prefill_attention_int8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                                 k_scale: torch.Tensor, v_scale: torch.Tensor,
+                                 block_tables: torch.Tensor, query_start_loc: torch.Tensor,
+                                 num_prior: torch.Tensor, max_query_len: int, scale: float,
+                                 out: torch.Tensor | None = None, err: torch.Tensor | None = None,
+                                 scratch: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_prefill_attention over int8 pools with a scale per (block, KV
+    head): query i of sequence s sees keys 0 .. num_prior[s] + i.  The visible
+    rows are laid out as values of q's dtype in `scratch`
+    (prefill_int8_scratch_bytes; allocated here when None), which the packed
+    attention kernel then reads.  max_query_len is taken as the other prefill
+    calls take it; this path does not need it."""
+    nb, bs, hkv, d = _check_int8_pools(k_pool, v_pool, k_scale, v_scale, q=q, err=err, out=out,
+                                       block_tables=block_tables, query_start_loc=query_start_loc,
+                                       num_prior=num_prior, scratch=scratch)
+    _check_err(err)
+    n_seqs = _check_rows_of(block_tables, num_prior, query_start_loc, "query_start_loc")
+    T, hq, dq = q.shape
+    if dq != d or hq % hkv:
+        raise ValueError("pagedkv: q / pools shapes disagree")
+    out = _like_q(out, q)
+    if T == 0 or n_seqs == 0:
+        return out
+    if scratch is None:
+        scratch = torch.empty(prefill_int8_scratch_bytes(n_seqs, block_tables.shape[1], hkv, d, bs, q.dtype),
+                              dtype=torch.uint8, device=q.device)
+    _call("pkv_paged_prefill_attention_int8", q, out.data_ptr(), _row_stride(out, "out"), q.data_ptr(),
+          _row_stride(q, "q"), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
+          v_scale.data_ptr(), nb, block_tables.data_ptr(), block_tables.stride(0),
+          block_tables.shape[1], query_start_loc.data_ptr(), num_prior.data_ptr(), n_seqs, T, hq, hkv,
+          d, bs, float(scale), dtype_code(q.dtype), scratch.data_ptr(), _bytes_of(scratch, "scratch"),
+          _ptr(err))
+    return out
+
+
+# ---------------------------------------------------------------- packed prompts, no cache
+
+def packed_prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                            query_start_loc: torch.Tensor, scale: float,
+                            out: torch.Tensor | None = None,
+                            err: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention with grouped heads over whole prompts packed one
+    behind the other, without a cache: row i of sequence s (rows
+    query_start_loc[s] .. query_start_loc[s + 1]) sees rows 0 .. i of its
+    sequence.  q [T, Hq, D], k, v [T, Hkv, D] (views of a fused projection will
+    do), D 64 or 128; query_start_loc int32 [n_seqs + 1].  Rows past the last
+    sequence are left as they are.  Reference: qwen2.py:98-128."""
+    _cuda(q, "q")
+    _same_device(q, k=k, v=v, query_start_loc=query_start_loc, out=out, err=err)
+    _check_err(err)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("pagedkv: q, k and v must share one dtype")
+    code = dtype_code(q.dtype)
+    T, hq, d = q.shape
+    hkv = k.shape[1]
+    if k.shape != v.shape or k.shape[0] != T or k.shape[2] != d or hq % hkv:
+        raise ValueError("pagedkv: q / k / v shapes disagree")
+    n_seqs = query_start_loc.shape[0] - 1
+    _int_row(query_start_loc, "query_start_loc", 1)
+    out = _like_q(out, q)
+    if T == 0 or n_seqs == 0:
+        return out
+    _call("pkv_packed_prompt_attention", q, out.data_ptr(), _row_stride(out, "out"), q.data_ptr(),
+          _row_stride(q, "q"), k.data_ptr(), _row_stride(k, "k"), v.data_ptr(), _row_stride(v, "v"),
+          query_start_loc.data_ptr(), n_seqs, T, hq, hkv, d, float(scale), code, _ptr(err))
+    return out
