@@ -191,6 +191,24 @@ int encode_q_tensormap(CUtensorMap* map, const void* q, int64_t q_stride, int n_
   return r == CUDA_SUCCESS ? 0 : PKV_ERR_DRIVER;
 }
 
+int encode_rows_tensormap(CUtensorMap* map, const void* rows, int64_t row_stride, int n_rows,
+                          int n_heads, int head_dim, int dtype, int box_heads, int box_rows) {
+  auto enc = encoder();
+  if (enc == nullptr) return PKV_ERR_DRIVER;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(n_heads),
+                              static_cast<cuuint64_t>(n_rows)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_dim) * 2,
+                                 static_cast<cuuint64_t>(row_stride) * 2};
+  const cuuint32_t box[3] = {64u, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[3] = {1u, 1u, 1u};
+  const CUtensorMapDataType dt =
+      dtype == PKV_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = enc(map, dt, 3, const_cast<void*>(rows), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : PKV_ERR_DRIVER;
+}
+
 }  // namespace pkv
 
 using namespace pkv;

@@ -253,6 +253,12 @@ struct PackedArgs {
 };
 cudaError_t launch_packed_attention(const PackedArgs& a, cudaStream_t stream);
 
+// TMA descriptor for rows [n_rows][n_heads][head_dim] of 16-bit values (row stride
+// in elements) with a box of 64 dims x box_heads x box_rows, 128-byte swizzle.
+// Returns 0 or PKV_ERR_DRIVER.
+int encode_rows_tensormap(CUtensorMap* map, const void* rows, int64_t row_stride, int n_rows,
+                          int n_heads, int head_dim, int dtype, int box_heads, int box_rows);
+
 // Argument checks, TMA-descriptor cache and kernel selection of pkv_abi.cu,
 // reused by the allocation-free decode entry point.
 int validate_attention_args(const void* out, int64_t out_stride, const void* q, int64_t q_stride,

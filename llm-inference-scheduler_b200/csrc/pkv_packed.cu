@@ -3,6 +3,7 @@
 // were laid out row by row.
 #include <float.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "pkv_common.cuh"
@@ -254,12 +255,629 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, packed_cores_kernel<T, D>, a);
 }
 
+
+// ---- tensor-core tiles (fp16 / bf16)
+//
+// Tile rows are (token, query head of one KV head's group) pairs, token-major:
+// 128 / G tokens of all G heads (18 tokens x 7 heads = 126 rows for 14 / 2
+// heads).  One K / V tile then serves the whole group, a prompt of a few tokens
+// fills a tile that would hold 128 rows of one head, and the causal diagonal
+// cuts only the last tokens' worth of a key tile.  A CTA takes items of two such
+// tiles (A and B) of one KV head, which share every K / V tile it loads.
+// 12 warps: two warpgroups of softmax (one thread per row of tile A / B: S from
+// tensor memory, running maximum and sum in registers, P back to tensor memory),
+// a producer (TMA of Q, K, V), one MMA issuer per tile, and the scheduler.
+//   S = Q K^T  (M 128, N 128 keys, K = D, both operands in shared memory)
+//   O += P V   (M 128, N = D, K 128 keys; P from tensor memory)
+// O is rescaled only when the running maximum grows by more than 2^8.
+// D = 64: S, O and P of both tiles fill the 512 tensor-memory columns, and S of
+// the next key tile is issued while the softmax works on this one.  D = 128: O
+// takes twice the columns, so P overwrites S (the MMA pipe runs in order: PV of
+// tile j, then S of tile j + 1 over the P it has read), and one tile's softmax
+// overlaps the other's MMAs.
+//
+// Items are handed out while the kernel runs: a CTA starts with its own block
+// index and then takes the indices of blocks that have not started
+// (clusterlaunchcontrol.try_cancel), one item ahead, so tensor memory, barriers
+// and the item order are set up once per SM.  Indices run from the sequences with
+// the most keys to those with the fewest, the last tokens of each first.
+constexpr int kTcM = 128, kTcN = 128, kTcThreads = 384;
+constexpr int kTcHalf = 128 * 128;  // 16 KB: 128 rows of 64 16-bit values
+constexpr int kTcSchedWarp = 11, kTcProducerWarp = 8, kTcMmaWarp = 9;
+constexpr int kTcRegsSoftmax = 224, kTcRegsOther = 56;
+constexpr int kTcRegSplit = 256 * kTcRegsSoftmax + 128 * kTcRegsOther;
+constexpr int kTcMaxSorted = 384;   // sequences ordered by their keys (more: taken as they come)
+constexpr int kTcItemInts = 8;
+constexpr uint32_t kTcTmemCols = 512;
+
+template <int D> struct TcShape {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kStages = D == 64 ? 4 : 2;
+  static constexpr int kTile = kHalves * kTcHalf;       // Q, K or V tile
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffK = 2 * kTile;
+  static constexpr int kOffV = kOffK + kStages * kTile;
+  static constexpr int kOffBar = kOffV + kStages * kTile;
+  // q_full, q_empty, kv_full/kv_empty [stages], s_full, s_empty, p_full, o_done [2], item_full, item_empty [2], clc
+  static constexpr int kBars = 2 + 2 * kStages + 8 + 4 + 1;
+  static constexpr int kOffClc = (kOffBar + kBars * 8 + 15) / 16 * 16;
+  static constexpr int kOffItem = kOffClc + 16;
+  static constexpr int kOffTmem = kOffItem + 2 * kTcItemInts * 4;
+  static constexpr int kOffOrder = kOffTmem + 16;        // sorted sequences, then item prefix
+  static constexpr int kBytes = 1024 + kOffOrder + (2 * kTcMaxSorted + 1) * 4;
+  static constexpr uint32_t kColS = 0, kColO = 256, kColP = D == 64 ? 384 : 0;
+  static constexpr uint32_t kPStep = D == 64 ? 64 : 128; // columns between P_A and P_B
+};
+static_assert(TcShape<64>::kBytes <= 232448 && TcShape<128>::kBytes <= 232448, "tiles fit the shared memory of an SM");
+
+struct TcParams {
+  PackedArgs a;
+  int group, tokens;   // query heads per KV head, tokens per tile
+  int sorted;
+  float scale_log2;
+};
+
+__device__ __forceinline__ void clc_try_cancel(void* result, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(result)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// the cancelled block's x index, or -1
+__device__ __forceinline__ int clc_index(const void* result) {
+  uint32_t x = 0, ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %1, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n\t}"
+      : "+r"(x), "=r"(ok)
+      : "r"(smem_u32(result))
+      : "memory");
+  return ok ? static_cast<int>(x) : -1;
+}
+
+// an item: two tiles of one (sequence, KV head)
+struct TcItem {
+  int s, g, tok0, q_begin, n_new, prior, keys;
+  int row0;  // first key row
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    packed_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                     const __grid_constant__ CUtensorMap vmap, const TcParams p) {
+  using Sh = TcShape<D>;
+  constexpr int kStages = Sh::kStages, kHalves = Sh::kHalves;
+  extern __shared__ uint8_t tc_smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t raw = smem_u32(tc_smem);
+  uint8_t* base = tc_smem + ((1024u - (raw & 1023u)) & 1023u);
+  const uint32_t sbase = smem_u32(base);
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(base + Sh::kOffBar);
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* kv_full = q_empty + 1;
+  uint64_t* kv_empty = kv_full + kStages;
+  uint64_t* s_full = kv_empty + kStages;
+  uint64_t* s_empty = s_full + 2;
+  uint64_t* p_full = s_empty + 2;
+  uint64_t* o_done = p_full + 2;
+  uint64_t* item_full = o_done + 2;
+  uint64_t* item_empty = item_full + 2;
+  uint64_t* clc_bar = item_empty + 2;
+  int* items = reinterpret_cast<int*>(base + Sh::kOffItem);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + Sh::kOffTmem);
+  int* order = reinterpret_cast<int*>(base + Sh::kOffOrder);
+  int* first_item = order + kTcMaxSorted;
+  const PackedArgs& a = p.a;
+  const int G = p.group, TT = p.tokens, B = a.n_seqs;
+
+  if (warp == 0 && elect_one()) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 2);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 2);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 128);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_done[i], 1);
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 11);
+    }
+    mbar_init(clc_bar, 1);
+    fence_barrier_init();
+  }
+  if (warp == kTcMmaWarp) tmem_alloc(tmem_slot, kTcTmemCols);
+  if (warp == kTcProducerWarp && elect_one()) {
+    prefetch_tensormap(&qmap);
+    prefetch_tensormap(&kmap);
+    prefetch_tensormap(&vmap);
+  }
+  if (tid == 0) pdl_trigger();
+  pdl_wait();  // the starts, q, k and v may come from the kernel before this one
+  const int per_item = 2 * TT;
+  if (blockIdx.x == 0)
+    for (int t = tid; t < B; t += kTcThreads) {
+      const int b = a.query_start_loc[t], n = a.query_start_loc[t + 1] - b;
+      if (b < 0 || n < 0 || b + static_cast<int64_t>(n) > a.n_tokens) raise_flag(a.err, PKV_FLAG_BAD_QUERY_LAYOUT);
+    }
+  if (p.sorted) {
+    // sequences by decreasing number of keys (ties by index), then the items before each
+    int* keys = first_item;
+    int mine = 0;
+    if (tid < B) {
+      mine = a.query_start_loc[tid + 1] - a.query_start_loc[tid] + (a.num_prior ? max(a.num_prior[tid], 0) : 0);
+      keys[tid] = mine;
+    }
+    __syncthreads();
+    int rank = 0;
+    if (tid < B)
+      for (int u = 0; u < B; ++u) rank += keys[u] > mine || (keys[u] == mine && u < tid);
+    __syncthreads();
+    if (tid < B) order[rank] = tid;
+    __syncthreads();
+    if (warp == 0) {
+      int run = 0;
+      for (int b0 = 0; b0 < B; b0 += 32) {
+        const int i = b0 + lane;
+        int n = 0;
+        if (i < B) {
+          const int len = a.query_start_loc[order[i] + 1] - a.query_start_loc[order[i]];
+          n = (min(max(len, 0), a.n_tokens) + per_item - 1) / per_item;
+        }
+        int x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        if (i < B) first_item[i] = run + x - n;
+        run += __shfl_sync(0xffffffffu, x, 31);
+      }
+      if (lane == 0) first_item[B] = run;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tmem_slot;
+
+  // the item of block index idx; false if there is none
+  auto find_item = [&](int idx, TcItem& it) -> bool {
+    const int u = idx / a.n_kv_heads;
+    it.g = idx - u * a.n_kv_heads;
+    int tile;
+    if (p.sorted) {
+      int lo = 0, hi = B - 1;
+      if (u >= first_item[B]) return false;
+      while (lo < hi) {
+        const int m = (lo + hi + 1) >> 1;
+        if (first_item[m] <= u) lo = m; else hi = m - 1;
+      }
+      it.s = order[lo];
+      tile = first_item[lo + 1] - 1 - u;  // last tokens first
+      it.q_begin = a.query_start_loc[it.s];
+      it.n_new = a.query_start_loc[it.s + 1] - it.q_begin;
+    } else {
+      int lo = 0, hi = B - 1;
+      while (lo < hi) {
+        const int m = (lo + hi + 1) >> 1;
+        if (a.query_start_loc[m] / per_item + static_cast<int64_t>(m) <= u) lo = m; else hi = m - 1;
+      }
+      it.s = lo;
+      it.q_begin = a.query_start_loc[lo];
+      it.n_new = a.query_start_loc[lo + 1] - it.q_begin;
+      const int k = static_cast<int>(u - (it.q_begin / per_item + static_cast<int64_t>(lo)));
+      tile = (it.n_new + per_item - 1) / per_item - 1 - k;
+    }
+    if (it.q_begin < 0 || it.n_new < 0 || it.q_begin + static_cast<int64_t>(it.n_new) > a.n_tokens) return false;  // flagged above
+    if (tile < 0 || tile >= (it.n_new + per_item - 1) / per_item) return false;
+    it.tok0 = tile * per_item;
+    const KeySpan k = key_span(a, it.s, it.q_begin, it.n_new);
+    it.prior = k.prior;
+    it.keys = k.keys;
+    it.row0 = static_cast<int>(k.row0);
+    return true;
+  };
+  // item `k` (counted per CTA) as the scheduler published it; tok0 < 0: no more
+  auto take_item = [&](int k, TcItem& it) -> bool {
+    const int sl = k & 1;
+    bool ok = mbar_wait(&item_full[sl], (k >> 1) & 1);
+    ok = __all_sync(0xffffffffu, ok);
+    const int* w = items + sl * kTcItemInts;
+    it.s = w[0], it.g = w[1], it.tok0 = w[2], it.q_begin = w[3], it.n_new = w[4], it.prior = w[5], it.keys = w[6], it.row0 = w[7];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty[sl]);
+    if (!ok && lane == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
+    return ok && it.tok0 >= 0;
+  };
+  // keys visible to tile x's last row, key tiles
+  auto tile_keys = [&](const TcItem& it, int x) {
+    const int t0 = it.tok0 + x * TT;
+    const int n = min(max(it.n_new - t0, 0), TT);
+    return n > 0 ? min(it.prior + t0 + n, it.keys) : 0;
+  };
+
+  if (warp >= 8) {
+    setmaxnreg_dec<kTcRegsOther>();
+    if (warp == kTcSchedWarp) {
+      // ======================= scheduler (one lane) =======================
+      if (lane == 0) {
+        int idx = blockIdx.x;
+        bool more = true;
+        uint32_t clc_phase = 0;
+        for (int k = 0;; ++k) {
+          TcItem it;
+          bool have = false;
+          while (more) {
+            if (idx >= 0) have = find_item(idx, it);
+            if (have) break;
+            // the next block that has not started, if there is one
+            mbar_arrive_expect_tx(clc_bar, 16);
+            clc_try_cancel(base + Sh::kOffClc, clc_bar);
+            if (!mbar_wait(clc_bar, clc_phase)) {
+              raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
+              more = false;
+              break;
+            }
+            clc_phase ^= 1;
+            idx = clc_index(base + Sh::kOffClc);
+            fence_proxy_async_smem();  // the response was read before the next one is written
+            if (idx < 0) more = false;
+          }
+          idx = -1;
+          const int sl = k & 1;
+          if (k >= 2 && !mbar_wait(&item_empty[sl], ((k >> 1) & 1) ^ 1)) {
+            raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
+            have = false;
+          }
+          int* w = items + sl * kTcItemInts;
+          w[0] = it.s, w[1] = it.g, w[2] = have ? it.tok0 : -1, w[3] = it.q_begin, w[4] = it.n_new, w[5] = it.prior, w[6] = it.keys,
+          w[7] = it.row0;
+          mbar_arrive(&item_full[sl]);
+          if (!have) break;
+        }
+      }
+      __syncwarp();
+    } else if (warp == kTcProducerWarp) {
+      // ======================= producer =======================
+      int c = 0;  // K / V tiles loaded so far
+      TcItem it;
+      for (int k = 0; take_item(k, it); ++k) {
+        const int n_tiles = (max(tile_keys(it, 0), tile_keys(it, 1)) + kTcN - 1) / kTcN;
+        if (k >= 1 && !__all_sync(0xffffffffu, mbar_wait(q_empty, (k - 1) & 1))) {
+          if (lane == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
+          break;
+        }
+        const bool two = it.tok0 + TT < it.n_new;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(q_full, (two ? 2 : 1) * kHalves * G * TT * 128);
+          for (int x = 0; x < (two ? 2 : 1); ++x)
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+              tma_load_3d(base + Sh::kOffQ + x * Sh::kTile + h * kTcHalf, &qmap, q_full, h * 64, it.g * G,
+                          it.q_begin + it.tok0 + x * TT);
+        }
+        __syncwarp();
+        bool dead = false;
+        for (int j = 0; j < n_tiles; ++j, ++c) {
+          const int st = c % kStages;
+          if (!__all_sync(0xffffffffu, mbar_wait(&kv_empty[st], ((c / kStages) & 1) ^ 1))) {
+            if (lane == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
+            dead = true;
+            break;
+          }
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&kv_full[st], 2 * Sh::kTile);
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) {
+              tma_load_3d(base + Sh::kOffK + st * Sh::kTile + h * kTcHalf, &kmap, &kv_full[st], h * 64, it.g, it.row0 + j * kTcN);
+              tma_load_3d(base + Sh::kOffV + st * Sh::kTile + h * kTcHalf, &vmap, &kv_full[st], h * 64, it.g, it.row0 + j * kTcN);
+            }
+          }
+          __syncwarp();
+        }
+        if (dead) break;
+      }
+    } else {
+      // ======================= MMA issuers (warp 9: tile A, warp 10: tile B) =======================
+      // Every issuer waits for every key tile and releases every stage, also
+      // those its tile does not reach, so a release always follows the load.
+      const int x = warp - kTcMmaWarp;
+      constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      constexpr uint32_t idesc_s = mma_idesc_f16(fmt, 0, 0, kTcN, kTcM);
+      constexpr uint32_t idesc_o = mma_idesc_f16(fmt, 0, 1, 64, kTcM);
+      const uint32_t t_s = tbase + Sh::kColS + x * 128, t_o = tbase + Sh::kColO + x * D, t_p = tbase + Sh::kColP + x * Sh::kPStep;
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
+      auto issue_qk = [&](int st) {
+        uint64_t ad[4 * kHalves], bd[4 * kHalves];
+#pragma unroll
+        for (int kk = 0; kk < 4 * kHalves; ++kk) {
+          const uint32_t off = (kk >> 2) * kTcHalf + (kk & 3) * 32;
+          ad[kk] = smem_desc(sbase + Sh::kOffQ + x * Sh::kTile + off, 16, 1024);
+          bd[kk] = smem_desc(sbase + Sh::kOffK + st * Sh::kTile + off, 16, 1024);
+        }
+        if (elect_one()) {
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 4 * kHalves; ++kk) tc_mma_f16(t_s, ad[kk], bd[kk], idesc_s, kk > 0 ? 1u : 0u);
+          tc_commit(&s_full[x]);
+        }
+        __syncwarp();
+      };
+      auto issue_pv = [&](int st, bool fresh) {
+        uint64_t bd[8 * kHalves];
+#pragma unroll
+        for (int kk = 0; kk < 8 * kHalves; ++kk)
+          bd[kk] = smem_desc(sbase + Sh::kOffV + st * Sh::kTile + (kk >> 3) * kTcHalf + (kk & 7) * 2048, 16, 1024);
+        if (elect_one()) {
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 8 * kHalves; ++kk)
+            tc_mma_f16_ts(t_o + (kk >> 3) * 64, t_p + (kk & 7) * 8, bd[kk], idesc_o, (!fresh || (kk & 7) > 0) ? 1u : 0u);
+          tc_commit(&o_done[x]);
+        }
+        __syncwarp();
+      };
+      int c = 0, cx = 0;  // key tiles seen, key tiles of this query tile
+      bool dead = false;
+      TcItem it;
+      for (int k = 0; !dead && take_item(k, it); ++k) {
+        const int mine = (tile_keys(it, x) + kTcN - 1) / kTcN;
+        const int n_tiles = max(mine, (tile_keys(it, 1 - x) + kTcN - 1) / kTcN);
+        if (!wait_all(q_full, k & 1)) { dead = true; break; }
+        // S of the first key tile, once the softmax has read the last S
+        if (!wait_all(&kv_full[c % kStages], (c / kStages) & 1)) { dead = true; break; }
+        if (mine > 0) {
+          if (D == 64 && cx > 0 && !wait_all(&s_empty[x], (cx - 1) & 1)) { dead = true; break; }
+          issue_qk(c % kStages);
+        }
+        for (int j = 0; j < n_tiles; ++j, ++c) {
+          const int st = c % kStages, nx = (c + 1) % kStages;
+          if (D == 64 && j + 1 < n_tiles) {
+            if (!wait_all(&kv_full[nx], ((c + 1) / kStages) & 1)) { dead = true; break; }
+            if (j + 1 < mine) {
+              if (!wait_all(&s_empty[x], (cx + j) & 1)) { dead = true; break; }
+              issue_qk(nx);
+            }
+          }
+          if (j < mine) {
+            if (!wait_all(&p_full[x], (cx + j) & 1)) { dead = true; break; }
+            issue_pv(st, j == 0);
+          }
+          if (D != 64 && j + 1 < n_tiles) {
+            if (!wait_all(&kv_full[nx], ((c + 1) / kStages) & 1)) { dead = true; break; }
+            if (j + 1 < mine) issue_qk(nx);
+          }
+          if (elect_one()) {
+            // (D = 128: this also waits for S of the next tile, which was issued before it)
+            tc_commit(&kv_empty[st]);
+            if (j + 1 == n_tiles) tc_commit(q_empty);
+          }
+          __syncwarp();
+        }
+        cx += mine;
+      }
+      if (dead && lane == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
+    }
+  } else {
+    setmaxnreg_inc<kTcRegsSoftmax>();
+    // ======================= softmax and epilogue (thread = row of tile x) =======================
+    const int x = warp >> 2, r = tid & 127;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tbase + Sh::kColS + x * 128 + lane_off;
+    const uint32_t t_o = tbase + Sh::kColO + x * D + lane_off;
+    const uint32_t t_p = tbase + Sh::kColP + x * Sh::kPStep + lane_off;
+    const int rtok = r / G, rhead = r - rtok * G;
+    const float sl2 = p.scale_log2;
+    int cx = 0;
+    bool dead = false;
+    TcItem it;
+    for (int k = 0; take_item(k, it); ++k) {
+      const int kvx = tile_keys(it, x), ntx = (kvx + kTcN - 1) / kTcN;
+      const int tok = it.tok0 + x * TT + rtok;
+      const bool row_valid = rtok < TT && tok < it.n_new;
+      const int lim = row_valid ? min(it.prior + tok + 1, kvx) : 0;
+      float m_used = -INFINITY, l = 0.f;
+      for (int j = 0; j < ntx; ++j) {
+        if (!dead && !mbar_wait(&s_full[x], (cx + j) & 1)) dead = true;
+        __syncwarp();
+        tc_fence_after();
+        uint32_t sr[4][32];
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4) tmem_ld32(t_s + c4 * 32, sr[c4]);
+        tmem_wait_ld_regs(sr[0]);
+        reg_after_wait(sr[1]);
+        reg_after_wait(sr[2]);
+        reg_after_wait(sr[3]);
+        if (D == 64) {
+          tc_fence_before();
+          mbar_arrive(&s_empty[x]);
+        }
+        const int kbase = j * kTcN;
+        if (kbase + kTcN > lim) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (kbase + c >= lim) sr[c >> 5][c & 31] = __float_as_uint(-INFINITY);
+        }
+        float m8[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) m8[q] = fmaxf(__uint_as_float(sr[0][q]), __uint_as_float(sr[0][q + 8]));
+#pragma unroll
+        for (int c = 16; c < 128; c += 16) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            m8[q] = fmax3(m8[q], __uint_as_float(sr[c >> 5][(c & 31) + q]), __uint_as_float(sr[(c + 8) >> 5][((c + 8) & 31) + q]));
+        }
+        const float mt = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7])) * sl2;
+        float factor = 1.f;
+        if (mt > m_used + 8.f) {
+          factor = exp2f(m_used - mt);
+          m_used = mt;
+          l *= factor;
+        }
+        const bool rescale = __any_sync(0xffffffffu, factor != 1.f) && j > 0;
+        const float nm = (m_used == -INFINITY) ? 0.f : -m_used;
+        float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        const float2 sl2v = make_float2(sl2, sl2), nmv = make_float2(nm, nm);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int c2 = half * 32 + i, c = 2 * c2;
+            const float2 xs = __ffma2_rn(make_float2(__uint_as_float(sr[c >> 5][c & 31]), __uint_as_float(sr[(c + 1) >> 5][(c + 1) & 31])),
+                                         sl2v, nmv);
+            const float2 pp = c2 % 3 == 2 ? exp2_poly3x2(xs) : make_float2(ex2_approx(xs.x), ex2_approx(xs.y));
+            ls[i & 1] = __fadd2_rn(ls[i & 1], pp);
+            pk[i] = pack2<T>(pp.x, pp.y);
+          }
+          if (half == 0) {
+            // D = 64: PV of tile j - 1 has read P and written O (D = 128: S of tile j came after it)
+            if (D == 64 && j >= 1 && !dead && !mbar_wait(&o_done[x], (cx + j - 1) & 1)) dead = true;
+            __syncwarp();
+            tc_fence_after();
+            if (rescale) {
+#pragma unroll
+              for (int c2 = 0; c2 < D / 32; ++c2) {
+                uint32_t orr[32];
+                tmem_ld32(t_o + c2 * 32, orr);
+                tmem_wait_ld_regs(orr);
+#pragma unroll
+                for (int c = 0; c < 32; ++c) orr[c] = __float_as_uint(__uint_as_float(orr[c]) * factor);
+                tmem_st32(t_o + c2 * 32, orr);
+              }
+            }
+          }
+          tmem_st32(t_p + half * 32, pk);
+        }
+        l += (ls[0].x + ls[1].x) + (ls[0].y + ls[1].y);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[x]);
+      }
+      // ---- epilogue: O / l -> out
+      bool fine = true;
+      const int64_t row = static_cast<int64_t>(it.q_begin) + tok;
+      const int head = it.g * G + rhead;
+      if (ntx > 0) {
+        if (!dead && !mbar_wait(&o_done[x], (cx + ntx - 1) & 1)) dead = true;
+        __syncwarp();
+        tc_fence_after();
+        const float inv = l > 0.f ? 1.f / l : l;  // NaN stays
+        float fsum = l;
+        T* orow = static_cast<T*>(a.out) + row * a.out_stride + static_cast<int64_t>(head) * D;
+#pragma unroll
+        for (int c2 = 0; c2 < D / 32; ++c2) {
+          uint32_t o[32];
+          tmem_ld32(t_o + c2 * 32, o);
+          tmem_wait_ld_regs(o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) fsum += fabsf(__uint_as_float(o[i]));
+          if (row_valid) {
+#pragma unroll
+            for (int c8 = 0; c8 < 4; ++c8) {
+              float f[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[c8 * 8 + i]) * inv;
+              uint4 v;
+              v.x = pack2<T>(f[0], f[1]);
+              v.y = pack2<T>(f[2], f[3]);
+              v.z = pack2<T>(f[4], f[5]);
+              v.w = pack2<T>(f[6], f[7]);
+              *reinterpret_cast<uint4*>(orow + c2 * 32 + c8 * 8) = v;
+            }
+          }
+        }
+        tc_fence_before();  // O is read before the next item's PV (ordered by p_full)
+        fine = !row_valid || fsum < INFINITY;
+      }
+      cx += ntx;
+      unsigned bad = __ballot_sync(0xffffffffu, !fine);
+      while (bad) {  // rows that a key they must not see may have spoiled
+        const int b = __ffs(bad) - 1;
+        bad &= bad - 1;
+        const int64_t brow = __shfl_sync(0xffffffffu, row, b);
+        const int bhead = __shfl_sync(0xffffffffu, head, b), blim = __shfl_sync(0xffffffffu, lim, b);
+        __syncwarp();
+        packed_row_alone<T, D>(a, brow, bhead, it.row0, blim);
+      }
+    }
+    if (dead && r == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kTcMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tbase, kTcTmemCols);
+  }
+}
+
+bool tc_supported(const PackedArgs& a) {
+  auto al = [](const void* q, int64_t stride) { return ((reinterpret_cast<uintptr_t>(q) | static_cast<uintptr_t>(stride * 2)) & 15) == 0; };
+  return a.dtype != PKV_DTYPE_F32 && a.n_q_heads / a.n_kv_heads <= 64 && al(a.q, a.q_stride) && al(a.k, a.k_stride) &&
+         al(a.v, a.v_stride) && al(a.out, a.out_stride);
+}
+
+template <typename T, int D>
+cudaError_t launch_tc(const PackedArgs& a, cudaStream_t stream) {
+  auto kern = packed_tc_kernel<T, D>;
+  static std::atomic<int> ready[64];  // per device: 0 not asked, 1 ready, -1 the register split does not fit
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  int state = dev < 64 ? ready[dev].load() : 0;
+  if (state == 0) {
+    cudaFuncAttributes fa;
+    e = cudaFuncGetAttributes(&fa, kern);
+    if (e != cudaSuccess) return e;
+    state = fa.numRegs * kTcThreads >= kTcRegSplit ? 1 : -1;
+    if (state == 1) {
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<D>::kBytes);
+      if (e != cudaSuccess) return e;
+    }
+    if (dev < 64) ready[dev].store(state);
+  }
+  if (state != 1) return launch_cores<T, D>(a, stream);
+  TcParams p{};
+  p.a = a;
+  p.group = a.n_q_heads / a.n_kv_heads;
+  p.tokens = kTcM / p.group;
+  p.sorted = a.n_seqs <= kTcMaxSorted;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  CUtensorMap qm, km, vm;
+  int rc = encode_rows_tensormap(&qm, a.q, a.q_stride, a.n_tokens, a.n_q_heads, D, a.dtype, p.group, p.tokens);
+  if (rc == 0) rc = encode_rows_tensormap(&km, a.k, a.k_stride, a.n_key_rows, a.n_kv_heads, D, a.dtype, 1, kTcN);
+  if (rc == 0) rc = encode_rows_tensormap(&vm, a.v, a.v_stride, a.n_key_rows, a.n_kv_heads, D, a.dtype, 1, kTcN);
+  if (rc != 0) return cudaErrorNotSupported;
+  const int64_t items = (a.n_tokens / (2 * p.tokens) + static_cast<int64_t>(a.n_seqs)) * a.n_kv_heads;
+  if (items > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(items));
+  cfg.blockDim = dim3(kTcThreads);
+  cfg.dynamicSmemBytes = TcShape<D>::kBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, qm, km, vm, p);
+}
+
 }  // namespace
 
 cudaError_t launch_packed_attention(const PackedArgs& a, cudaStream_t stream) {
   if (a.n_tokens == 0 || a.n_seqs == 0) return cudaSuccess;
   auto go = [&](auto tag) {
     using T = decltype(tag);
+    if constexpr (sizeof(T) == 2) {
+      if (tc_supported(a)) return a.head_dim == 64 ? launch_tc<T, 64>(a, stream) : launch_tc<T, 128>(a, stream);
+    }
     return a.head_dim == 64 ? launch_cores<T, 64>(a, stream) : launch_cores<T, 128>(a, stream);
   };
   if (a.dtype == PKV_DTYPE_F16) return go(__half{});
