@@ -266,15 +266,20 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
 // tiles (A and B) of one KV head, which share every K / V tile it loads.
 // 12 warps: two warpgroups of softmax (one thread per row of tile A / B: S from
 // tensor memory, running maximum and sum in registers, P back to tensor memory),
-// a producer (TMA of Q, K, V), one MMA issuer per tile, and the scheduler.
+// a producer (TMA of Q, K, V), one MMA issuer and the scheduler.
 //   S = Q K^T  (M 128, N 128 keys, K = D, both operands in shared memory)
 //   O += P V   (M 128, N = D, K 128 keys; P from tensor memory)
 // O is rescaled only when the running maximum grows by more than 2^8.
-// D = 64: S, O and P of both tiles fill the 512 tensor-memory columns, and S of
-// the next key tile is issued while the softmax works on this one.  D = 128: O
-// takes twice the columns, so P overwrites S (the MMA pipe runs in order: PV of
-// tile j, then S of tile j + 1 over the P it has read), and one tile's softmax
-// overlaps the other's MMAs.
+//
+// Steps A(0), B(0), A(1), B(1), .. (query tile, key tile) go through a ring of S
+// buffers in tensor memory (three for D = 64, two for D = 128, where O takes the
+// columns of the third).  P of a step overwrites its own S, and S of a step goes
+// into the buffer whose P the PV issued before it reads: the MMA pipe runs in
+// issue order, so the issuer alone orders the buffers.  One issuer for both tiles
+// also keeps them apart: PV and the next S of tile A, then those of tile B, so
+// one tile's softmax runs while the other's MMAs do.  (With an issuer each, both
+// tiles fell into step, 4,200 cycles a pair of steps at D = 128 where the MMAs
+// take 2,048.)  With three buffers S is always two steps ahead of the softmax.
 //
 // Items are handed out while the kernel runs: a CTA starts with its own block
 // index and then takes the indices of blocks that have not started
@@ -283,7 +288,7 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
 // the most keys to those with the fewest, the last tokens of each first.
 constexpr int kTcM = 128, kTcN = 128, kTcThreads = 384;
 constexpr int kTcHalf = 128 * 128;  // 16 KB: 128 rows of 64 16-bit values
-constexpr int kTcSchedWarp = 11, kTcProducerWarp = 8, kTcMmaWarp = 9;
+constexpr int kTcProducerWarp = 8, kTcMmaWarp = 9, kTcSchedWarp = 10;
 constexpr int kTcRegsSoftmax = 224, kTcRegsOther = 56;
 constexpr int kTcRegSplit = 256 * kTcRegsSoftmax + 128 * kTcRegsOther;
 constexpr int kTcMaxSorted = 384;   // sequences ordered by their keys (more: taken as they come)
@@ -292,21 +297,21 @@ constexpr uint32_t kTcTmemCols = 512;
 
 template <int D> struct TcShape {
   static constexpr int kHalves = D / 64;
-  static constexpr int kStages = D == 64 ? 4 : 2;
+  static constexpr int kStages = D == 64 ? 4 : 2;       // of K and of V
+  static constexpr int kBufs = D == 64 ? 3 : 2;         // of S / P in tensor memory
   static constexpr int kTile = kHalves * kTcHalf;       // Q, K or V tile
   static constexpr int kOffQ = 0;
   static constexpr int kOffK = 2 * kTile;
   static constexpr int kOffV = kOffK + kStages * kTile;
   static constexpr int kOffBar = kOffV + kStages * kTile;
-  // q_full, q_empty, kv_full/kv_empty [stages], s_full, s_empty, p_full, o_done [2], item_full, item_empty [2], clc
-  static constexpr int kBars = 2 + 2 * kStages + 8 + 4 + 1;
+  // q_full, q_empty, K and V full / empty [stages], S full [2 tiles][bufs], P full [bufs], o_done [2 tiles][2], item_full, item_empty [2], clc
+  static constexpr int kBars = 2 + 4 * kStages + 3 * kBufs + 4 + 4 + 1;
   static constexpr int kOffClc = (kOffBar + kBars * 8 + 15) / 16 * 16;
   static constexpr int kOffItem = kOffClc + 16;
   static constexpr int kOffTmem = kOffItem + 2 * kTcItemInts * 4;
   static constexpr int kOffOrder = kOffTmem + 16;        // sorted sequences, then item prefix
   static constexpr int kBytes = 1024 + kOffOrder + (2 * kTcMaxSorted + 1) * 4;
-  static constexpr uint32_t kColS = 0, kColO = 256, kColP = D == 64 ? 384 : 0;
-  static constexpr uint32_t kPStep = D == 64 ? 64 : 128; // columns between P_A and P_B
+  static constexpr uint32_t kColO = kBufs * 128;        // O_A, O_B behind the S buffers
 };
 static_assert(TcShape<64>::kBytes <= 232448 && TcShape<128>::kBytes <= 232448, "tiles fit the shared memory of an SM");
 
@@ -349,7 +354,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     packed_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                      const __grid_constant__ CUtensorMap vmap, const TcParams p) {
   using Sh = TcShape<D>;
-  constexpr int kStages = Sh::kStages, kHalves = Sh::kHalves;
+  constexpr int kStages = Sh::kStages, kHalves = Sh::kHalves, kBufs = Sh::kBufs;
   extern __shared__ uint8_t tc_smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t raw = smem_u32(tc_smem);
@@ -357,13 +362,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t sbase = smem_u32(base);
   uint64_t* q_full = reinterpret_cast<uint64_t*>(base + Sh::kOffBar);
   uint64_t* q_empty = q_full + 1;
-  uint64_t* kv_full = q_empty + 1;
-  uint64_t* kv_empty = kv_full + kStages;
-  uint64_t* s_full = kv_empty + kStages;
-  uint64_t* s_empty = s_full + 2;
-  uint64_t* p_full = s_empty + 2;
-  uint64_t* o_done = p_full + 2;
-  uint64_t* item_full = o_done + 2;
+  uint64_t* k_full = q_empty + 1;
+  uint64_t* k_empty = k_full + kStages;
+  uint64_t* v_full = k_empty + kStages;
+  uint64_t* v_empty = v_full + kStages;
+  uint64_t* s_full = v_empty + kStages;
+  uint64_t* p_full = s_full + 2 * kBufs;
+  uint64_t* o_done = p_full + kBufs;
+  uint64_t* item_full = o_done + 4;
   uint64_t* item_empty = item_full + 2;
   uint64_t* clc_bar = item_empty + 2;
   int* items = reinterpret_cast<int*>(base + Sh::kOffItem);
@@ -375,18 +381,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (warp == 0 && elect_one()) {
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 2);
+    mbar_init(q_empty, 1);
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 2);
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
     }
+    for (int i = 0; i < 2 * kBufs; ++i) mbar_init(&s_full[i], 1);
+    for (int i = 0; i < kBufs; ++i) mbar_init(&p_full[i], 128);
+    for (int i = 0; i < 4; ++i) mbar_init(&o_done[i], 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_empty[i], 128);
-      mbar_init(&p_full[i], 128);
-      mbar_init(&o_done[i], 1);
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], 11);
+      mbar_init(&item_empty[i], 10);  // 8 softmax warps, producer, MMA issuer
     }
     mbar_init(clc_bar, 1);
     fence_barrier_init();
@@ -566,101 +573,149 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         bool dead = false;
         for (int j = 0; j < n_tiles; ++j, ++c) {
           const int st = c % kStages;
-          if (!__all_sync(0xffffffffu, mbar_wait(&kv_empty[st], ((c / kStages) & 1) ^ 1))) {
-            if (lane == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
-            dead = true;
-            break;
-          }
-          if (elect_one()) {
-            mbar_arrive_expect_tx(&kv_full[st], 2 * Sh::kTile);
+          // K is free again once S of its tile is done, V once its PV is: each has a ring of its own
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h) {
-              tma_load_3d(base + Sh::kOffK + st * Sh::kTile + h * kTcHalf, &kmap, &kv_full[st], h * 64, it.g, it.row0 + j * kTcN);
-              tma_load_3d(base + Sh::kOffV + st * Sh::kTile + h * kTcHalf, &vmap, &kv_full[st], h * 64, it.g, it.row0 + j * kTcN);
+          for (int kv = 0; kv < 2; ++kv) {
+            uint64_t* full = kv ? &v_full[st] : &k_full[st];
+            if (!__all_sync(0xffffffffu, mbar_wait(kv ? &v_empty[st] : &k_empty[st], ((c / kStages) & 1) ^ 1))) {
+              if (lane == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
+              dead = true;
+              break;
             }
+            if (elect_one()) {
+              mbar_arrive_expect_tx(full, Sh::kTile);
+#pragma unroll
+              for (int h = 0; h < kHalves; ++h)
+                tma_load_3d(base + (kv ? Sh::kOffV : Sh::kOffK) + st * Sh::kTile + h * kTcHalf, kv ? &vmap : &kmap, full, h * 64, it.g,
+                            it.row0 + j * kTcN);
+            }
+            __syncwarp();
           }
-          __syncwarp();
+          if (dead) break;
         }
         if (dead) break;
       }
-    } else {
-      // ======================= MMA issuers (warp 9: tile A, warp 10: tile B) =======================
-      // Every issuer waits for every key tile and releases every stage, also
-      // those its tile does not reach, so a release always follows the load.
-      const int x = warp - kTcMmaWarp;
+    } else if (warp == kTcMmaWarp) {
+      // ======================= MMA issuer =======================
+      // Two cursors over the steps: S of step qn is issued up to kBufs - 1 steps
+      // ahead of the PV of step pn (never waiting for it ahead of time), so the
+      // buffer it goes into has been read by a PV issued before.
       constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
       constexpr uint32_t idesc_s = mma_idesc_f16(fmt, 0, 0, kTcN, kTcM);
-      constexpr uint32_t idesc_o = mma_idesc_f16(fmt, 0, 1, 64, kTcM);
-      const uint32_t t_s = tbase + Sh::kColS + x * 128, t_o = tbase + Sh::kColO + x * D, t_p = tbase + Sh::kColP + x * Sh::kPStep;
+      constexpr uint32_t idesc_o = mma_idesc_f16(fmt, 0, 1, D, kTcM);
       auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
-      auto issue_qk = [&](int st) {
-        uint64_t ad[4 * kHalves], bd[4 * kHalves];
-#pragma unroll
-        for (int kk = 0; kk < 4 * kHalves; ++kk) {
-          const uint32_t off = (kk >> 2) * kTcHalf + (kk & 3) * 32;
-          ad[kk] = smem_desc(sbase + Sh::kOffQ + x * Sh::kTile + off, 16, 1024);
-          bd[kk] = smem_desc(sbase + Sh::kOffK + st * Sh::kTile + off, 16, 1024);
-        }
-        if (elect_one()) {
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < 4 * kHalves; ++kk) tc_mma_f16(t_s, ad[kk], bd[kk], idesc_s, kk > 0 ? 1u : 0u);
-          tc_commit(&s_full[x]);
-        }
-        __syncwarp();
+      auto is_done = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)); };
+      struct Cursor {
+        int k = -1;              // item
+        int nt0 = 0, nt1 = 0;    // its key tiles of A and B
+        int j = 0, x = 0;        // the step
+        int c0 = 0, n = 0;       // K / V tiles before the item, steps before this one
+        bool more = true;        // there is a step
       };
-      auto issue_pv = [&](int st, bool fresh) {
-        uint64_t bd[8 * kHalves];
-#pragma unroll
-        for (int kk = 0; kk < 8 * kHalves; ++kk)
-          bd[kk] = smem_desc(sbase + Sh::kOffV + st * Sh::kTile + (kk >> 3) * kTcHalf + (kk & 7) * 2048, 16, 1024);
-        if (elect_one()) {
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < 8 * kHalves; ++kk)
-            tc_mma_f16_ts(t_o + (kk >> 3) * 64, t_p + (kk & 7) * 8, bd[kk], idesc_o, (!fresh || (kk & 7) > 0) ? 1u : 0u);
-          tc_commit(&o_done[x]);
-        }
-        __syncwarp();
+      // the next item's first step
+      auto open = [&](Cursor& u, const TcItem& it) {
+        u.c0 += max(u.nt0, u.nt1);
+        u.nt0 = (tile_keys(it, 0) + kTcN - 1) / kTcN;
+        u.nt1 = (tile_keys(it, 1) + kTcN - 1) / kTcN;
+        u.j = u.x = 0;
+        ++u.k;
       };
-      int c = 0, cx = 0;  // key tiles seen, key tiles of this query tile
-      bool dead = false;
-      TcItem it;
-      for (int k = 0; !dead && take_item(k, it); ++k) {
-        const int mine = (tile_keys(it, x) + kTcN - 1) / kTcN;
-        const int n_tiles = max(mine, (tile_keys(it, 1 - x) + kTcN - 1) / kTcN);
-        if (!wait_all(q_full, k & 1)) { dead = true; break; }
-        // S of the first key tile, once the softmax has read the last S
-        if (!wait_all(&kv_full[c % kStages], (c / kStages) & 1)) { dead = true; break; }
-        if (mine > 0) {
-          if (D == 64 && cx > 0 && !wait_all(&s_empty[x], (cx - 1) & 1)) { dead = true; break; }
-          issue_qk(c % kStages);
+      // past this step; true if it was the item's last
+      auto advance = [&](Cursor& u) {
+        ++u.n;
+        if (u.x == 0 && u.j < u.nt1) {
+          u.x = 1;
+        } else {
+          ++u.j;
+          u.x = u.j < u.nt0 ? 0 : 1;
         }
-        for (int j = 0; j < n_tiles; ++j, ++c) {
-          const int st = c % kStages, nx = (c + 1) % kStages;
-          if (D == 64 && j + 1 < n_tiles) {
-            if (!wait_all(&kv_full[nx], ((c + 1) / kStages) & 1)) { dead = true; break; }
-            if (j + 1 < mine) {
-              if (!wait_all(&s_empty[x], (cx + j) & 1)) { dead = true; break; }
-              issue_qk(nx);
-            }
+        return u.j >= max(u.nt0, u.nt1);
+      };
+      // does no later step use key tile j?
+      auto last_use = [&](const Cursor& u) { return u.x == 1 || u.j >= u.nt1; };
+      TcItem it;  // the S cursor's item: the PV cursor's or the one after it
+      Cursor q, pv;
+      bool dead = false, item_over = false;
+      int made0 = 0, made1 = 0;  // S of tile A, of tile B
+      int done0 = 0, done1 = 0;  // PVs of tile A, of tile B
+      q.more = take_item(0, it);
+      if (q.more) open(q, it);
+      pv = q;
+      while (pv.more && !dead) {
+        while (q.more && q.n < pv.n + kBufs) {
+          if (item_over) {
+            if (q.k > pv.k) break;
+            item_over = false;
+            q.more = take_item(q.k + 1, it);
+            if (!q.more) break;
+            open(q, it);
           }
-          if (j < mine) {
-            if (!wait_all(&p_full[x], (cx + j) & 1)) { dead = true; break; }
-            issue_pv(st, j == 0);
+          const int st = (q.c0 + q.j) % kStages;
+          const uint32_t kpar = ((q.c0 + q.j) / kStages) & 1;
+          if (q.n == pv.n) {  // the softmax waits for this one
+            if ((q.j == 0 && q.x == 0 && !wait_all(q_full, q.k & 1)) || !wait_all(&k_full[st], kpar)) { dead = true; break; }
+          } else if ((q.j == 0 && q.x == 0 && !is_done(q_full, q.k & 1)) || !is_done(&k_full[st], kpar)) {
+            break;
           }
-          if (D != 64 && j + 1 < n_tiles) {
-            if (!wait_all(&kv_full[nx], ((c + 1) / kStages) & 1)) { dead = true; break; }
-            if (j + 1 < mine) issue_qk(nx);
+          const uint32_t qa = sbase + Sh::kOffQ + q.x * Sh::kTile, ka = sbase + Sh::kOffK + st * Sh::kTile;
+          const uint32_t t_s = tbase + (q.n % kBufs) * 128;
+          uint64_t ad[4 * kHalves], bd[4 * kHalves];
+#pragma unroll
+          for (int kk = 0; kk < 4 * kHalves; ++kk) {
+            const uint32_t off = (kk >> 2) * kTcHalf + (kk & 3) * 32;
+            ad[kk] = smem_desc(qa + off, 16, 1024);
+            bd[kk] = smem_desc(ka + off, 16, 1024);
           }
+          // S signals a ring of barriers of its own tile: the other tile's softmax
+          // may be items ahead, where it would take an old phase for its own
+          uint64_t* sf = &s_full[q.x * kBufs + (q.x ? made1 : made0) % kBufs];
+          if (q.x) ++made1; else ++made0;
+          const bool last_k = last_use(q);
+          const bool last_q = advance(q);
           if (elect_one()) {
-            // (D = 128: this also waits for S of the next tile, which was issued before it)
-            tc_commit(&kv_empty[st]);
-            if (j + 1 == n_tiles) tc_commit(q_empty);
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < 4 * kHalves; ++kk) tc_mma_f16(t_s, ad[kk], bd[kk], idesc_s, kk > 0 ? 1u : 0u);
+            tc_commit(sf);
+            if (last_k) tc_commit(&k_empty[st]);
+            if (last_q) tc_commit(q_empty);
           }
           __syncwarp();
+          item_over = last_q;
         }
-        cx += mine;
+        if (dead) break;
+        // PV of step pn
+        const int st = (pv.c0 + pv.j) % kStages;
+        if (!wait_all(&v_full[st], ((pv.c0 + pv.j) / kStages) & 1) ||
+            !wait_all(&p_full[pv.n % kBufs], (pv.n / kBufs) & 1)) {
+          dead = true;
+          break;
+        }
+        const uint32_t t_o = tbase + Sh::kColO + pv.x * D, t_p = tbase + (pv.n % kBufs) * 128;
+        // V is the MN-major operand: 8 keys every 1024 bytes, the second 64 dims (D = 128) 16 KB on
+        uint64_t bd[8];
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          bd[kk] = smem_desc(sbase + Sh::kOffV + st * Sh::kTile + kk * 2048, kHalves == 2 ? kTcHalf : 16, 1024);
+        const uint32_t keep = pv.j > 0 ? 1u : 0u;
+        uint64_t* od = &o_done[2 * pv.x + ((pv.x ? done1 : done0) & 1)];
+        if (pv.x) ++done1; else ++done0;
+        const bool last_v = last_use(pv);
+        const bool last = advance(pv);
+        if (elect_one()) {
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) tc_mma_f16_ts(t_o, t_p + kk * 8, bd[kk], idesc_o, kk > 0 ? 1u : keep);
+          tc_commit(od);
+          if (last_v) tc_commit(&v_empty[st]);
+        }
+        __syncwarp();
+        if (last) {
+          // the S cursor, ahead by a step, has opened the next item (and waits in
+          // it for this one) or has found that there is none
+          pv.more = q.k > pv.k;
+          if (pv.more) open(pv, it);
+        }
       }
       if (dead && lane == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
     }
@@ -669,22 +724,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ======================= softmax and epilogue (thread = row of tile x) =======================
     const int x = warp >> 2, r = tid & 127;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_s = tbase + Sh::kColS + x * 128 + lane_off;
     const uint32_t t_o = tbase + Sh::kColO + x * D + lane_off;
-    const uint32_t t_p = tbase + Sh::kColP + x * Sh::kPStep + lane_off;
     const int rtok = r / G, rhead = r - rtok * G;
     const float sl2 = p.scale_log2;
-    int cx = 0;
+    int cx = 0;   // PVs of this tile so far
+    int n0 = 0;   // steps of both tiles so far
     bool dead = false;
     TcItem it;
     for (int k = 0; take_item(k, it); ++k) {
       const int kvx = tile_keys(it, x), ntx = (kvx + kTcN - 1) / kTcN;
+      const int nto = (tile_keys(it, 1 - x) + kTcN - 1) / kTcN;
+      // PV number i of this item and tile has completed.  PVs signal two
+      // barriers in turn: one would tell PV i from PV i - 1 only, and PV i - 2 is
+      // all that S of step i + 1 vouches for.
+      auto wait_pv = [&](int i) {
+        const int w = cx + i;
+        if (!dead && !mbar_wait(&o_done[2 * x + (w & 1)], (w >> 1) & 1)) dead = true;
+      };
       const int tok = it.tok0 + x * TT + rtok;
       const bool row_valid = rtok < TT && tok < it.n_new;
       const int lim = row_valid ? min(it.prior + tok + 1, kvx) : 0;
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < ntx; ++j) {
-        if (!dead && !mbar_wait(&s_full[x], (cx + j) & 1)) dead = true;
+        // this step's number: A(j) and B(j) alternate while both tiles have key tiles
+        const int n = n0 + (x == 0 ? (nto > 0 ? 2 * j : j) : (j < nto ? 2 * j + 1 : nto + j));
+        const uint32_t t_s = tbase + (n % kBufs) * 128 + lane_off;
+        if (!dead && !mbar_wait(&s_full[x * kBufs + (cx + j) % kBufs], ((cx + j) / kBufs) & 1)) dead = true;
         __syncwarp();
         tc_fence_after();
         uint32_t sr[4][32];
@@ -694,10 +759,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         reg_after_wait(sr[1]);
         reg_after_wait(sr[2]);
         reg_after_wait(sr[3]);
-        if (D == 64) {
-          tc_fence_before();
-          mbar_arrive(&s_empty[x]);
-        }
         const int kbase = j * kTcN;
         if (kbase + kTcN > lim) {
 #pragma unroll
@@ -737,11 +798,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             pk[i] = pack2<T>(pp.x, pp.y);
           }
           if (half == 0) {
-            // D = 64: PV of tile j - 1 has read P and written O (D = 128: S of tile j came after it)
-            if (D == 64 && j >= 1 && !dead && !mbar_wait(&o_done[x], (cx + j - 1) & 1)) dead = true;
-            __syncwarp();
-            tc_fence_after();
-            if (rescale) {
+            if (rescale) {  // after the PV before this step
+              wait_pv(j - 1);
+              __syncwarp();
+              tc_fence_after();
 #pragma unroll
               for (int c2 = 0; c2 < D / 32; ++c2) {
                 uint32_t orr[32];
@@ -753,19 +813,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               }
             }
           }
-          tmem_st32(t_p + half * 32, pk);
+          tmem_st32(t_s + half * 32, pk);
         }
         l += (ls[0].x + ls[1].x) + (ls[0].y + ls[1].y);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&p_full[x]);
+        mbar_arrive(&p_full[n % kBufs]);
       }
       // ---- epilogue: O / l -> out
       bool fine = true;
       const int64_t row = static_cast<int64_t>(it.q_begin) + tok;
       const int head = it.g * G + rhead;
       if (ntx > 0) {
-        if (!dead && !mbar_wait(&o_done[x], (cx + ntx - 1) & 1)) dead = true;
+        wait_pv(ntx - 1);
         __syncwarp();
         tc_fence_after();
         const float inv = l > 0.f ? 1.f / l : l;  // NaN stays
@@ -797,6 +857,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         fine = !row_valid || fsum < INFINITY;
       }
       cx += ntx;
+      n0 += ntx + nto;
       unsigned bad = __ballot_sync(0xffffffffu, !fine);
       while (bad) {  // rows that a key they must not see may have spoiled
         const int b = __ffs(bad) - 1;
