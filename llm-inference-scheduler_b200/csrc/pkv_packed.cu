@@ -322,6 +322,43 @@ struct TcParams {
   float scale_log2;
 };
 
+// high word of every shared-memory descriptor here: 1024 bytes between groups of 8
+// rows, descriptor version 1, 128-byte swizzle (smem_desc)
+constexpr uint32_t kSmemDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+// tc_mma_f16 / tc_mma_f16_ts with descriptors given by their low words
+template <uint32_t HI>
+__device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint32_t alo, uint32_t blo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(alo), "r"(blo), "r"(idesc), "r"(accumulate), "n"(HI)
+      : "memory");
+}
+template <uint32_t HI>
+__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t blo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(blo), "r"(idesc), "r"(accumulate), "n"(HI)
+      : "memory");
+}
+// has the phase of this parity completed? (does not wait)
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 __device__ __forceinline__ void clc_try_cancel(void* result, uint64_t* bar) {
   asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
                    smem_u32(result)),
@@ -600,121 +637,134 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // Two cursors over the steps: S of step qn is issued up to kBufs - 1 steps
       // ahead of the PV of step pn (never waiting for it ahead of time), so the
       // buffer it goes into has been read by a PV issued before.
+      // The warp shares its scheduler with two softmax warps, so its own
+      // instructions are dear: descriptors are a constant high word and a low word
+      // that advances by constants, and every ring index is counted, not divided
+      // (with descriptors built per instruction and indices by remainder a step
+      // took 1,830 cycles of this warp, more than the softmax).
       constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
       constexpr uint32_t idesc_s = mma_idesc_f16(fmt, 0, 0, kTcN, kTcM);
       constexpr uint32_t idesc_o = mma_idesc_f16(fmt, 0, 1, D, kTcM);
+      constexpr uint32_t kTileStep = Sh::kTile >> 4;
+      // V is the MN-major operand: 8 keys every 1024 bytes, the second 64 dims (D = 128) 16 KB on
+      const uint32_t q_lo = ((sbase + Sh::kOffQ) >> 4) | (1u << 16);
+      const uint32_t k_lo = ((sbase + Sh::kOffK) >> 4) | (1u << 16);
+      const uint32_t v_lo = ((sbase + Sh::kOffV) >> 4) | (static_cast<uint32_t>(kHalves == 2 ? kTcHalf >> 4 : 1) << 16);
       auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
-      auto is_done = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)); };
       struct Cursor {
-        int k = -1;              // item
-        int nt0 = 0, nt1 = 0;    // its key tiles of A and B
-        int j = 0, x = 0;        // the step
-        int c0 = 0, n = 0;       // K / V tiles before the item, steps before this one
-        bool more = true;        // there is a step
-      };
-      // the next item's first step
-      auto open = [&](Cursor& u, const TcItem& it) {
-        u.c0 += max(u.nt0, u.nt1);
-        u.nt0 = (tile_keys(it, 0) + kTcN - 1) / kTcN;
-        u.nt1 = (tile_keys(it, 1) + kTcN - 1) / kTcN;
-        u.j = u.x = 0;
-        ++u.k;
+        int j = 0, x = 0, nt0 = 0, nt1 = 0;  // the step, key tiles of A and B
+        int st = 0, buf = 0;                 // K / V stage, S buffer
+        uint32_t st_ph = 0, buf_ph = 0;      // their phases
       };
       // past this step; true if it was the item's last
       auto advance = [&](Cursor& u) {
-        ++u.n;
+        if (++u.buf == kBufs) {
+          u.buf = 0;
+          u.buf_ph ^= 1;
+        }
         if (u.x == 0 && u.j < u.nt1) {
           u.x = 1;
-        } else {
-          ++u.j;
-          u.x = u.j < u.nt0 ? 0 : 1;
+          return false;
         }
-        return u.j >= max(u.nt0, u.nt1);
+        if (++u.st == kStages) {
+          u.st = 0;
+          u.st_ph ^= 1;
+        }
+        ++u.j;
+        u.x = u.j < u.nt0 ? 0 : 1;
+        return u.j >= u.nt0 && u.j >= u.nt1;
       };
-      // does no later step use key tile j?
-      auto last_use = [&](const Cursor& u) { return u.x == 1 || u.j >= u.nt1; };
-      TcItem it;  // the S cursor's item: the PV cursor's or the one after it
       Cursor q, pv;
-      bool dead = false, item_over = false;
-      int made0 = 0, made1 = 0;  // S of tile A, of tile B
-      int done0 = 0, done1 = 0;  // PVs of tile A, of tile B
-      q.more = take_item(0, it);
-      if (q.more) open(q, it);
-      pv = q;
-      while (pv.more && !dead) {
-        while (q.more && q.n < pv.n + kBufs) {
+      int qk = -1, pk = 0;            // their items
+      int nt0 = 0, nt1 = 0;           // key tiles of item qk
+      int ahead = 0;                  // S issued whose PV is not
+      int made0 = 0, made1 = 0;       // ring of S barriers, tile A and B
+      uint32_t done = 0;              // bit x: which of the two PV barriers of tile x is next
+      bool dead = false, more = true, item_over = false;
+      auto open_item = [&]() {
+        TcItem it;
+        if (!take_item(qk + 1, it)) return false;
+        ++qk;
+        nt0 = (tile_keys(it, 0) + kTcN - 1) / kTcN;
+        nt1 = (tile_keys(it, 1) + kTcN - 1) / kTcN;
+        q.j = q.x = 0;
+        q.nt0 = nt0;
+        q.nt1 = nt1;
+        return true;
+      };
+      more = open_item();
+      pv.nt0 = nt0;
+      pv.nt1 = nt1;
+      bool work = more;
+      while (work) {
+        while (more && ahead < kBufs) {
           if (item_over) {
-            if (q.k > pv.k) break;
+            if (qk > pk) break;  // two items on: after this one's last PV
             item_over = false;
-            q.more = take_item(q.k + 1, it);
-            if (!q.more) break;
-            open(q, it);
+            more = open_item();
+            if (!more) break;
           }
-          const int st = (q.c0 + q.j) % kStages;
-          const uint32_t kpar = ((q.c0 + q.j) / kStages) & 1;
-          if (q.n == pv.n) {  // the softmax waits for this one
-            if ((q.j == 0 && q.x == 0 && !wait_all(q_full, q.k & 1)) || !wait_all(&k_full[st], kpar)) { dead = true; break; }
-          } else if ((q.j == 0 && q.x == 0 && !is_done(q_full, q.k & 1)) || !is_done(&k_full[st], kpar)) {
-            break;
+          if (q.j == 0 && q.x == 0) {
+            // a new item's Q: waited for only if the softmax has nothing else to do
+            if (ahead > 0 ? !__all_sync(0xffffffffu, mbar_test(q_full, qk & 1)) : false) break;
+            if (!wait_all(q_full, qk & 1)) { dead = true; break; }
           }
-          const uint32_t qa = sbase + Sh::kOffQ + q.x * Sh::kTile, ka = sbase + Sh::kOffK + st * Sh::kTile;
-          const uint32_t t_s = tbase + (q.n % kBufs) * 128;
-          uint64_t ad[4 * kHalves], bd[4 * kHalves];
-#pragma unroll
-          for (int kk = 0; kk < 4 * kHalves; ++kk) {
-            const uint32_t off = (kk >> 2) * kTcHalf + (kk & 3) * 32;
-            ad[kk] = smem_desc(qa + off, 16, 1024);
-            bd[kk] = smem_desc(ka + off, 16, 1024);
-          }
+          if (!wait_all(&k_full[q.st], q.st_ph)) { dead = true; break; }
+          const uint32_t alo = q_lo + q.x * kTileStep, blo = k_lo + q.st * kTileStep;
+          const uint32_t t_s = tbase + q.buf * 128;
           // S signals a ring of barriers of its own tile: the other tile's softmax
           // may be items ahead, where it would take an old phase for its own
-          uint64_t* sf = &s_full[q.x * kBufs + (q.x ? made1 : made0) % kBufs];
-          if (q.x) ++made1; else ++made0;
-          const bool last_k = last_use(q);
-          const bool last_q = advance(q);
+          uint64_t* sf = s_full + (q.x ? kBufs + made1 : made0);
+          uint64_t* ke = (q.x == 1 || q.j >= q.nt1) ? &k_empty[q.st] : nullptr;
+          if (q.x) {
+            if (++made1 == kBufs) made1 = 0;
+          } else {
+            if (++made0 == kBufs) made0 = 0;
+          }
+          item_over = advance(q);
           if (elect_one()) {
             tc_fence_after();
 #pragma unroll
-            for (int kk = 0; kk < 4 * kHalves; ++kk) tc_mma_f16(t_s, ad[kk], bd[kk], idesc_s, kk > 0 ? 1u : 0u);
+            for (int kk = 0; kk < 4 * kHalves; ++kk) {
+              const uint32_t off = (kk >> 2) * (kTcHalf >> 4) + (kk & 3) * 2;
+              tc_mma_ss<kSmemDescHi>(t_s, alo + off, blo + off, idesc_s, kk > 0 ? 1u : 0u);
+            }
             tc_commit(sf);
-            if (last_k) tc_commit(&k_empty[st]);
-            if (last_q) tc_commit(q_empty);
+            if (ke != nullptr) tc_commit(ke);
+            if (item_over) tc_commit(q_empty);
           }
           __syncwarp();
-          item_over = last_q;
+          ++ahead;
         }
         if (dead) break;
-        // PV of step pn
-        const int st = (pv.c0 + pv.j) % kStages;
-        if (!wait_all(&v_full[st], ((pv.c0 + pv.j) / kStages) & 1) ||
-            !wait_all(&p_full[pv.n % kBufs], (pv.n / kBufs) & 1)) {
+        // ---- PV
+        if (!wait_all(&v_full[pv.st], pv.st_ph) || !wait_all(&p_full[pv.buf], pv.buf_ph)) {
           dead = true;
           break;
         }
-        const uint32_t t_o = tbase + Sh::kColO + pv.x * D, t_p = tbase + (pv.n % kBufs) * 128;
-        // V is the MN-major operand: 8 keys every 1024 bytes, the second 64 dims (D = 128) 16 KB on
-        uint64_t bd[8];
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          bd[kk] = smem_desc(sbase + Sh::kOffV + st * Sh::kTile + kk * 2048, kHalves == 2 ? kTcHalf : 16, 1024);
+        const uint32_t t_o = tbase + Sh::kColO + pv.x * D, t_p = tbase + pv.buf * 128, blo = v_lo + pv.st * kTileStep;
         const uint32_t keep = pv.j > 0 ? 1u : 0u;
-        uint64_t* od = &o_done[2 * pv.x + ((pv.x ? done1 : done0) & 1)];
-        if (pv.x) ++done1; else ++done0;
-        const bool last_v = last_use(pv);
+        uint64_t* od = o_done + 2 * pv.x + ((done >> pv.x) & 1);
+        uint64_t* ve = (pv.x == 1 || pv.j >= pv.nt1) ? &v_empty[pv.st] : nullptr;
+        done ^= 1u << pv.x;
         const bool last = advance(pv);
         if (elect_one()) {
           tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) tc_mma_f16_ts(t_o, t_p + kk * 8, bd[kk], idesc_o, kk > 0 ? 1u : keep);
+          for (int kk = 0; kk < 8; ++kk) tc_mma_ts<kSmemDescHi>(t_o, t_p + kk * 8, blo + kk * 128, idesc_o, kk > 0 ? 1u : keep);
           tc_commit(od);
-          if (last_v) tc_commit(&v_empty[st]);
+          if (ve != nullptr) tc_commit(ve);
         }
         __syncwarp();
+        --ahead;
         if (last) {
           // the S cursor, ahead by a step, has opened the next item (and waits in
           // it for this one) or has found that there is none
-          pv.more = q.k > pv.k;
-          if (pv.more) open(pv, it);
+          work = qk > pk;
+          ++pk;
+          pv.j = pv.x = 0;
+          pv.nt0 = nt0;
+          pv.nt1 = nt1;
         }
       }
       if (dead && lane == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
