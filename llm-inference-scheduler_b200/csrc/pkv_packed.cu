@@ -266,20 +266,21 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
 // tiles (A and B) of one KV head, which share every K / V tile it loads.
 // 12 warps: two warpgroups of softmax (one thread per row of tile A / B: S from
 // tensor memory, running maximum and sum in registers, P back to tensor memory),
-// a producer (TMA of Q, K, V), one MMA issuer and the scheduler.
+// a producer (TMA of Q, K, V), an issuer for S, one for O, and the scheduler.
 //   S = Q K^T  (M 128, N 128 keys, K = D, both operands in shared memory)
 //   O += P V   (M 128, N = D, K 128 keys; P from tensor memory)
 // O is rescaled only when the running maximum grows by more than 2^8.
 //
 // Steps A(0), B(0), A(1), B(1), .. (query tile, key tile) go through a ring of S
 // buffers in tensor memory (three for D = 64, two for D = 128, where O takes the
-// columns of the third).  P of a step overwrites its own S, and S of a step goes
-// into the buffer whose P the PV issued before it reads: the MMA pipe runs in
-// issue order, so the issuer alone orders the buffers.  One issuer for both tiles
-// also keeps them apart: PV and the next S of tile A, then those of tile B, so
-// one tile's softmax runs while the other's MMAs do.  (With an issuer each, both
-// tiles fell into step, 4,200 cycles a pair of steps at D = 128 where the MMAs
-// take 2,048.)  With three buffers S is always two steps ahead of the softmax.
+// columns of the third); P of a step overwrites its own S.  Both issuers take the
+// steps in that order, so A and B alternate and one tile's softmax runs while the
+// other's MMAs do: with an issuer per tile both fell into step, 4,200 cycles a
+// pair of steps at D = 128 where the MMAs take 2,048.  One issuer for S and one
+// for O, because the instructions between two batches of MMAs (waits, indices)
+// take a warp that shares its scheduler with two softmax warps about 700 cycles
+// a step, in which the tensor pipe would idle (one issuer for both: 1,780 cycles
+// a step at D = 64, 2,150 at D = 128).
 //
 // Items are handed out while the kernel runs: a CTA starts with its own block
 // index and then takes the indices of blocks that have not started
@@ -288,7 +289,7 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
 // the most keys to those with the fewest, the last tokens of each first.
 constexpr int kTcM = 128, kTcN = 128, kTcThreads = 384;
 constexpr int kTcHalf = 128 * 128;  // 16 KB: 128 rows of 64 16-bit values
-constexpr int kTcProducerWarp = 8, kTcMmaWarp = 9, kTcSchedWarp = 10;
+constexpr int kTcProducerWarp = 8, kTcQkWarp = 9, kTcSchedWarp = 10, kTcPvWarp = 11;
 constexpr int kTcRegsSoftmax = 224, kTcRegsOther = 56;
 constexpr int kTcRegSplit = 256 * kTcRegsSoftmax + 128 * kTcRegsOther;
 constexpr int kTcMaxSorted = 384;   // sequences ordered by their keys (more: taken as they come)
@@ -304,8 +305,8 @@ template <int D> struct TcShape {
   static constexpr int kOffK = 2 * kTile;
   static constexpr int kOffV = kOffK + kStages * kTile;
   static constexpr int kOffBar = kOffV + kStages * kTile;
-  // q_full, q_empty, K and V full / empty [stages], S full [2 tiles][bufs], P full [bufs], o_done [2 tiles][2], item_full, item_empty [2], clc
-  static constexpr int kBars = 2 + 4 * kStages + 3 * kBufs + 4 + 4 + 1;
+  // q_full, q_empty, K and V full / empty [stages], S full [2 tiles][bufs], P full and buffer free [bufs], o_done [2 tiles][2], item_full, item_empty [2], clc
+  static constexpr int kBars = 2 + 4 * kStages + 4 * kBufs + 4 + 4 + 1;
   static constexpr int kOffClc = (kOffBar + kBars * 8 + 15) / 16 * 16;
   static constexpr int kOffItem = kOffClc + 16;
   static constexpr int kOffTmem = kOffItem + 2 * kTcItemInts * 4;
@@ -393,7 +394,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   using Sh = TcShape<D>;
   constexpr int kStages = Sh::kStages, kHalves = Sh::kHalves, kBufs = Sh::kBufs;
   extern __shared__ uint8_t tc_smem[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform for the compiler too
   const uint32_t raw = smem_u32(tc_smem);
   uint8_t* base = tc_smem + ((1024u - (raw & 1023u)) & 1023u);
   const uint32_t sbase = smem_u32(base);
@@ -405,7 +407,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* v_empty = v_full + kStages;
   uint64_t* s_full = v_empty + kStages;
   uint64_t* p_full = s_full + 2 * kBufs;
-  uint64_t* o_done = p_full + kBufs;
+  uint64_t* b_free = p_full + kBufs;
+  uint64_t* o_done = b_free + kBufs;
   uint64_t* item_full = o_done + 4;
   uint64_t* item_empty = item_full + 2;
   uint64_t* clc_bar = item_empty + 2;
@@ -426,16 +429,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&v_empty[i], 1);
     }
     for (int i = 0; i < 2 * kBufs; ++i) mbar_init(&s_full[i], 1);
-    for (int i = 0; i < kBufs; ++i) mbar_init(&p_full[i], 128);
+    for (int i = 0; i < kBufs; ++i) {
+      mbar_init(&p_full[i], 128);
+      mbar_init(&b_free[i], 1);
+    }
     for (int i = 0; i < 4; ++i) mbar_init(&o_done[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], 10);  // 8 softmax warps, producer, MMA issuer
+      mbar_init(&item_empty[i], 11);  // 8 softmax warps, producer, two issuers
     }
     mbar_init(clc_bar, 1);
     fence_barrier_init();
   }
-  if (warp == kTcMmaWarp) tmem_alloc(tmem_slot, kTcTmemCols);
+  if (warp == kTcQkWarp) tmem_alloc(tmem_slot, kTcTmemCols);
   if (warp == kTcProducerWarp && elect_one()) {
     prefetch_tensormap(&qmap);
     prefetch_tensormap(&kmap);
@@ -488,7 +494,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tbase = *tmem_slot;
+  const uint32_t tbase = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   // the item of block index idx; false if there is none
   auto find_item = [&](int idx, TcItem& it) -> bool {
@@ -632,139 +638,106 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (dead) break;
       }
-    } else if (warp == kTcMmaWarp) {
-      // ======================= MMA issuer =======================
-      // Two cursors over the steps: S of step qn is issued up to kBufs - 1 steps
-      // ahead of the PV of step pn (never waiting for it ahead of time), so the
-      // buffer it goes into has been read by a PV issued before.
-      // The warp shares its scheduler with two softmax warps, so its own
-      // instructions are dear: descriptors are a constant high word and a low word
-      // that advances by constants, and every ring index is counted, not divided
-      // (with descriptors built per instruction and indices by remainder a step
-      // took 1,830 cycles of this warp, more than the softmax).
+    } else {
+      // ======================= MMA issuers (warp 9: S, warp 11: O) =======================
+      // Descriptors are a constant high word and a low word that advances by
+      // constants, ring indices are counted, not divided, and what comes from
+      // shared memory is broadcast, so that the compiler knows the loops to be
+      // uniform and keeps the MMAs' operands in uniform registers.
       constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-      constexpr uint32_t idesc_s = mma_idesc_f16(fmt, 0, 0, kTcN, kTcM);
-      constexpr uint32_t idesc_o = mma_idesc_f16(fmt, 0, 1, D, kTcM);
       constexpr uint32_t kTileStep = Sh::kTile >> 4;
-      // V is the MN-major operand: 8 keys every 1024 bytes, the second 64 dims (D = 128) 16 KB on
-      const uint32_t q_lo = ((sbase + Sh::kOffQ) >> 4) | (1u << 16);
-      const uint32_t k_lo = ((sbase + Sh::kOffK) >> 4) | (1u << 16);
-      const uint32_t v_lo = ((sbase + Sh::kOffV) >> 4) | (static_cast<uint32_t>(kHalves == 2 ? kTcHalf >> 4 : 1) << 16);
       auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
-      struct Cursor {
-        int j = 0, x = 0, nt0 = 0, nt1 = 0;  // the step, key tiles of A and B
-        int st = 0, buf = 0;                 // K / V stage, S buffer
-        uint32_t st_ph = 0, buf_ph = 0;      // their phases
-      };
-      // past this step; true if it was the item's last
-      auto advance = [&](Cursor& u) {
-        if (++u.buf == kBufs) {
-          u.buf = 0;
-          u.buf_ph ^= 1;
-        }
-        if (u.x == 0 && u.j < u.nt1) {
-          u.x = 1;
-          return false;
-        }
-        if (++u.st == kStages) {
-          u.st = 0;
-          u.st_ph ^= 1;
-        }
-        ++u.j;
-        u.x = u.j < u.nt0 ? 0 : 1;
-        return u.j >= u.nt0 && u.j >= u.nt1;
-      };
-      Cursor q, pv;
-      int qk = -1, pk = 0;            // their items
-      int nt0 = 0, nt1 = 0;           // key tiles of item qk
-      int ahead = 0;                  // S issued whose PV is not
-      int made0 = 0, made1 = 0;       // ring of S barriers, tile A and B
-      uint32_t done = 0;              // bit x: which of the two PV barriers of tile x is next
-      bool dead = false, more = true, item_over = false;
-      auto open_item = [&]() {
+      int st = 0, buf = 0;                 // K / V stage, S buffer
+      uint32_t st_ph = 0, buf_ph = 0;      // their phases
+      int nt0 = 0, nt1 = 0;                // key tiles of A and B
+      bool dead = false;
+      auto open_item = [&](int k) {
         TcItem it;
-        if (!take_item(qk + 1, it)) return false;
-        ++qk;
-        nt0 = (tile_keys(it, 0) + kTcN - 1) / kTcN;
-        nt1 = (tile_keys(it, 1) + kTcN - 1) / kTcN;
-        q.j = q.x = 0;
-        q.nt0 = nt0;
-        q.nt1 = nt1;
-        return true;
+        const bool ok = __all_sync(0xffffffffu, take_item(k, it));
+        nt0 = __shfl_sync(0xffffffffu, (tile_keys(it, 0) + kTcN - 1) / kTcN, 0);
+        nt1 = __shfl_sync(0xffffffffu, (tile_keys(it, 1) + kTcN - 1) / kTcN, 0);
+        return ok;
       };
-      more = open_item();
-      pv.nt0 = nt0;
-      pv.nt1 = nt1;
-      bool work = more;
-      while (work) {
-        while (more && ahead < kBufs) {
-          if (item_over) {
-            if (qk > pk) break;  // two items on: after this one's last PV
-            item_over = false;
-            more = open_item();
-            if (!more) break;
-          }
-          if (q.j == 0 && q.x == 0) {
-            // a new item's Q: waited for only if the softmax has nothing else to do
-            if (ahead > 0 ? !__all_sync(0xffffffffu, mbar_test(q_full, qk & 1)) : false) break;
-            if (!wait_all(q_full, qk & 1)) { dead = true; break; }
-          }
-          if (!wait_all(&k_full[q.st], q.st_ph)) { dead = true; break; }
-          const uint32_t alo = q_lo + q.x * kTileStep, blo = k_lo + q.st * kTileStep;
-          const uint32_t t_s = tbase + q.buf * 128;
-          // S signals a ring of barriers of its own tile: the other tile's softmax
-          // may be items ahead, where it would take an old phase for its own
-          uint64_t* sf = s_full + (q.x ? kBufs + made1 : made0);
-          uint64_t* ke = (q.x == 1 || q.j >= q.nt1) ? &k_empty[q.st] : nullptr;
-          if (q.x) {
-            if (++made1 == kBufs) made1 = 0;
-          } else {
-            if (++made0 == kBufs) made0 = 0;
-          }
-          item_over = advance(q);
-          if (elect_one()) {
-            tc_fence_after();
+      auto next_buf = [&]() {
+        if (++buf == kBufs) {
+          buf = 0;
+          buf_ph ^= 1;
+        }
+      };
+      auto next_stage = [&]() {
+        if (++st == kStages) {
+          st = 0;
+          st_ph ^= 1;
+        }
+      };
+      if (warp == kTcQkWarp) {
+        constexpr uint32_t idesc = mma_idesc_f16(fmt, 0, 0, kTcN, kTcM);
+        const uint32_t q_lo = ((sbase + Sh::kOffQ) >> 4) | (1u << 16), k_lo = ((sbase + Sh::kOffK) >> 4) | (1u << 16);
+        int made[2] = {0, 0};
+        for (int k = 0; !dead && open_item(k); ++k) {
+          if (!wait_all(q_full, k & 1)) { dead = true; break; }
+          const int n_tiles = max(nt0, nt1);
+          for (int j = 0; j < n_tiles && !dead; ++j) {
+            if (!wait_all(&k_full[st], st_ph)) { dead = true; break; }
+            const uint32_t blo = k_lo + st * kTileStep;
 #pragma unroll
-            for (int kk = 0; kk < 4 * kHalves; ++kk) {
-              const uint32_t off = (kk >> 2) * (kTcHalf >> 4) + (kk & 3) * 2;
-              tc_mma_ss<kSmemDescHi>(t_s, alo + off, blo + off, idesc_s, kk > 0 ? 1u : 0u);
+            for (int x = 0; x < 2; ++x) {
+              if (j >= (x ? nt1 : nt0)) continue;
+              // the PV that read this buffer's P has completed
+              if (!wait_all(&b_free[buf], buf_ph ^ 1)) { dead = true; break; }
+              const uint32_t t_s = tbase + buf * 128;
+              // S signals a ring of barriers of its own tile: the other tile's softmax
+              // may be items ahead, where it would take an old phase for its own
+              uint64_t* sf = s_full + x * kBufs + made[x];
+              const bool last = x == 1 || j >= nt1;
+              if (elect_one()) {
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 0; kk < 4 * kHalves; ++kk) {
+                  const uint32_t off = (kk >> 2) * (kTcHalf >> 4) + (kk & 3) * 2;
+                  tc_mma_ss<kSmemDescHi>(t_s, q_lo + x * kTileStep + off, blo + off, idesc, kk > 0 ? 1u : 0u);
+                }
+                tc_commit(sf);
+                if (last) tc_commit(&k_empty[st]);
+                if (last && j + 1 == n_tiles) tc_commit(q_empty);
+              }
+              __syncwarp();
+              if (++made[x] == kBufs) made[x] = 0;
+              next_buf();
             }
-            tc_commit(sf);
-            if (ke != nullptr) tc_commit(ke);
-            if (item_over) tc_commit(q_empty);
+            next_stage();
           }
-          __syncwarp();
-          ++ahead;
         }
-        if (dead) break;
-        // ---- PV
-        if (!wait_all(&v_full[pv.st], pv.st_ph) || !wait_all(&p_full[pv.buf], pv.buf_ph)) {
-          dead = true;
-          break;
-        }
-        const uint32_t t_o = tbase + Sh::kColO + pv.x * D, t_p = tbase + pv.buf * 128, blo = v_lo + pv.st * kTileStep;
-        const uint32_t keep = pv.j > 0 ? 1u : 0u;
-        uint64_t* od = o_done + 2 * pv.x + ((done >> pv.x) & 1);
-        uint64_t* ve = (pv.x == 1 || pv.j >= pv.nt1) ? &v_empty[pv.st] : nullptr;
-        done ^= 1u << pv.x;
-        const bool last = advance(pv);
-        if (elect_one()) {
-          tc_fence_after();
+      } else {
+        constexpr uint32_t idesc = mma_idesc_f16(fmt, 0, 1, D, kTcM);
+        // V is the MN-major operand: 8 keys every 1024 bytes, the second 64 dims (D = 128) 16 KB on
+        const uint32_t v_lo = ((sbase + Sh::kOffV) >> 4) | (static_cast<uint32_t>(kHalves == 2 ? kTcHalf >> 4 : 1) << 16);
+        int done[2] = {0, 0};  // which of the two barriers of a tile is next
+        for (int k = 0; !dead && open_item(k); ++k) {
+          const int n_tiles = max(nt0, nt1);
+          for (int j = 0; j < n_tiles && !dead; ++j) {
+            if (!wait_all(&v_full[st], st_ph)) { dead = true; break; }
+            const uint32_t blo = v_lo + st * kTileStep;
+            const uint32_t keep = j > 0 ? 1u : 0u;
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) tc_mma_ts<kSmemDescHi>(t_o, t_p + kk * 8, blo + kk * 128, idesc_o, kk > 0 ? 1u : keep);
-          tc_commit(od);
-          if (ve != nullptr) tc_commit(ve);
-        }
-        __syncwarp();
-        --ahead;
-        if (last) {
-          // the S cursor, ahead by a step, has opened the next item (and waits in
-          // it for this one) or has found that there is none
-          work = qk > pk;
-          ++pk;
-          pv.j = pv.x = 0;
-          pv.nt0 = nt0;
-          pv.nt1 = nt1;
+            for (int x = 0; x < 2; ++x) {
+              if (j >= (x ? nt1 : nt0)) continue;
+              if (!wait_all(&p_full[buf], buf_ph)) { dead = true; break; }
+              const uint32_t t_o = tbase + Sh::kColO + x * D, t_p = tbase + buf * 128;
+              if (elect_one()) {
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 0; kk < 8; ++kk) tc_mma_ts<kSmemDescHi>(t_o, t_p + kk * 8, blo + kk * 128, idesc, kk > 0 ? 1u : keep);
+                tc_commit(&b_free[buf]);
+                tc_commit(o_done + 2 * x + done[x]);
+                if (x == 1 || j >= nt1) tc_commit(&v_empty[st]);
+              }
+              __syncwarp();
+              done[x] ^= 1;
+              next_buf();
+            }
+            next_stage();
+          }
         }
       }
       if (dead && lane == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
@@ -784,12 +757,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int k = 0; take_item(k, it); ++k) {
       const int kvx = tile_keys(it, x), ntx = (kvx + kTcN - 1) / kTcN;
       const int nto = (tile_keys(it, 1 - x) + kTcN - 1) / kTcN;
-      // PV number i of this item and tile has completed.  PVs signal two
-      // barriers in turn: one would tell PV i from PV i - 1 only, and PV i - 2 is
-      // all that S of step i + 1 vouches for.
+      // PV number i of this item and tile has completed.  A wait tells a phase
+      // from the one before it only.  PVs signal two barriers in turn, and S of
+      // this tile's step i or i + 1, which the caller has seen, was issued
+      // after PV i - 3 at least: PV i - 1 can be waited for, and then PV i.
       auto wait_pv = [&](int i) {
-        const int w = cx + i;
-        if (!dead && !mbar_wait(&o_done[2 * x + (w & 1)], (w >> 1) & 1)) dead = true;
+#pragma unroll
+        for (int b = 1; b >= 0; --b) {
+          const int w = cx + i - b;
+          if (i >= b && !dead && !mbar_wait(&o_done[2 * x + (w & 1)], (w >> 1) & 1)) dead = true;
+        }
       };
       const int tok = it.tok0 + x * TT + rtok;
       const bool row_valid = rtok < TT && tok < it.n_new;
@@ -922,7 +899,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kTcMmaWarp) {
+  if (warp == kTcQkWarp) {
     tc_fence_after();
     tmem_dealloc(tbase, kTcTmemCols);
   }
