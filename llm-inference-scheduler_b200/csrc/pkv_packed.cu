@@ -2,6 +2,7 @@
 // whole prompts packed one behind the other, or chunks behind cached keys that
 // were laid out row by row.
 #include <float.h>
+#include <limits.h>
 
 #include <atomic>
 #include <type_traits>
@@ -272,24 +273,26 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
 // O is rescaled only when the running maximum grows by more than 2^8.
 //
 // Steps A(0), B(0), A(1), B(1), .. (query tile, key tile) go through a ring of S
-// buffers in tensor memory (three for D = 64, two for D = 128, where O takes the
-// columns of the third); P of a step overwrites its own S.  Both issuers take the
-// steps in that order, so A and B alternate and one tile's softmax runs while the
-// other's MMAs do: with an issuer per tile both fell into step, 4,200 cycles a
-// pair of steps at D = 128 where the MMAs take 2,048.  One issuer for S and one
-// for O, because the instructions between two batches of MMAs (waits, indices)
-// take a warp that shares its scheduler with two softmax warps about 700 cycles
-// a step, in which the tensor pipe would idle (one issuer for both: 1,780 cycles
-// a step at D = 64, 2,150 at D = 128).
+// buffers in tensor memory, which O leaves 384 columns (D = 64) or 256 of: three
+// buffers of 128 keys, or four of 64.  P of a step overwrites its own S, so a
+// buffer is free again when its PV is done, while the softmaxes work on the
+// others.  (D = 64 with P in columns of its own and one S buffer a tile: 189 us
+// against 183 for four prompts of up to 8,191 tokens; key tiles of 64: 216.
+// D = 128 with two buffers of 128 keys: 252 us against 238 for twelve prompts of
+// up to 2,048.)
+// One issuer for S and one for O, both in step order, so A and B alternate: an
+// issuer per tile let both fall into step, and the instructions between two
+// batches of MMAs (waits, indices) take a warp that shares its scheduler with two
+// softmax warps about 700 cycles, in which one issuer for both would leave the
+// tensor pipe idle (1,780 cycles a step at D = 64).
 //
 // Items are handed out while the kernel runs: a CTA starts with its own block
 // index and then takes the indices of blocks that have not started
 // (clusterlaunchcontrol.try_cancel), one item ahead, so tensor memory, barriers
 // and the item order are set up once per SM.  Indices run from the sequences with
 // the most keys to those with the fewest, the last tokens of each first.
-constexpr int kTcM = 128, kTcN = 128, kTcThreads = 384;
-constexpr int kTcHalf = 128 * 128;  // 16 KB: 128 rows of 64 16-bit values
-constexpr int kTcProducerWarp = 8, kTcQkWarp = 9, kTcSchedWarp = 10, kTcPvWarp = 11;
+constexpr int kTcM = 128, kTcThreads = 384;
+constexpr int kTcProducerWarp = 8, kTcQkWarp = 9, kTcSchedWarp = 10;  // warp 11: O
 constexpr int kTcRegsSoftmax = 224, kTcRegsOther = 56;
 constexpr int kTcRegSplit = 256 * kTcRegsSoftmax + 128 * kTcRegsOther;
 constexpr int kTcMaxSorted = 384;   // sequences ordered by their keys (more: taken as they come)
@@ -297,22 +300,26 @@ constexpr int kTcItemInts = 8;
 constexpr uint32_t kTcTmemCols = 512;
 
 template <int D> struct TcShape {
-  static constexpr int kHalves = D / 64;
-  static constexpr int kStages = D == 64 ? 4 : 2;       // of K and of V
-  static constexpr int kBufs = D == 64 ? 3 : 2;         // of S / P in tensor memory
-  static constexpr int kTile = kHalves * kTcHalf;       // Q, K or V tile
+  static constexpr int kN = D == 64 ? 128 : 64;         // keys per tile
+  static constexpr int kStages = 4;                     // of K and of V
+  static constexpr int kBufs = D == 64 ? 3 : 4;         // S buffers
+  static constexpr int kHalves = D / 64;                // 64 dims are a 128-byte swizzled row
+  static constexpr int kQHalf = 128 * 128, kQTile = kHalves * kQHalf;
+  static constexpr int kKHalf = kN * 128, kKTile = kHalves * kKHalf;  // K and V
   static constexpr int kOffQ = 0;
-  static constexpr int kOffK = 2 * kTile;
-  static constexpr int kOffV = kOffK + kStages * kTile;
-  static constexpr int kOffBar = kOffV + kStages * kTile;
-  // q_full, q_empty, K and V full / empty [stages], S full [2 tiles][bufs], P full and buffer free [bufs], o_done [2 tiles][2], item_full, item_empty [2], clc
-  static constexpr int kBars = 2 + 4 * kStages + 4 * kBufs + 4 + 4 + 1;
+  static constexpr int kOffK = 2 * kQTile;
+  static constexpr int kOffV = kOffK + kStages * kKTile;
+  static constexpr int kOffBar = kOffV + kStages * kKTile;
+  // q_full, q_empty, K and V full / empty [stages], S full [2 tiles][bufs], P full and S free [bufs],
+  // o_done [2 tiles][bufs], item_full, item_empty [2], clc
+  static constexpr int kBars = 2 + 4 * kStages + 6 * kBufs + 4 + 1;
   static constexpr int kOffClc = (kOffBar + kBars * 8 + 15) / 16 * 16;
   static constexpr int kOffItem = kOffClc + 16;
   static constexpr int kOffTmem = kOffItem + 2 * kTcItemInts * 4;
   static constexpr int kOffOrder = kOffTmem + 16;        // sorted sequences, then item prefix
-  static constexpr int kBytes = 1024 + kOffOrder + (2 * kTcMaxSorted + 1) * 4;
-  static constexpr uint32_t kColO = kBufs * 128;        // O_A, O_B behind the S buffers
+  static constexpr int kOffOut = (kOffOrder + (2 * kTcMaxSorted + 1) * 4 + 15) / 16 * 16;  // 2 KB per softmax warp
+  static constexpr int kBytes = 1024 + kOffOut + 8 * 2048;
+  static constexpr uint32_t kColO = kBufs * kN;          // O_A, O_B behind the S buffers
 };
 static_assert(TcShape<64>::kBytes <= 232448 && TcShape<128>::kBytes <= 232448, "tiles fit the shared memory of an SM");
 
@@ -347,19 +354,6 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint
       "r"(a_tmem), "r"(blo), "r"(idesc), "r"(accumulate), "n"(HI)
       : "memory");
 }
-// has the phase of this parity completed? (does not wait)
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
 __device__ __forceinline__ void clc_try_cancel(void* result, uint64_t* bar) {
   asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
                    smem_u32(result)),
@@ -392,7 +386,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     packed_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                      const __grid_constant__ CUtensorMap vmap, const TcParams p) {
   using Sh = TcShape<D>;
-  constexpr int kStages = Sh::kStages, kHalves = Sh::kHalves, kBufs = Sh::kBufs;
+  constexpr int kStages = Sh::kStages, kHalves = Sh::kHalves, kBufs = Sh::kBufs, kN = Sh::kN;
   extern __shared__ uint8_t tc_smem[];
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform for the compiler too
@@ -407,9 +401,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* v_empty = v_full + kStages;
   uint64_t* s_full = v_empty + kStages;
   uint64_t* p_full = s_full + 2 * kBufs;
-  uint64_t* b_free = p_full + kBufs;
-  uint64_t* o_done = b_free + kBufs;
-  uint64_t* item_full = o_done + 4;
+  uint64_t* s_free = p_full + kBufs;
+  uint64_t* o_done = s_free + kBufs;
+  uint64_t* item_full = o_done + 2 * kBufs;
   uint64_t* item_empty = item_full + 2;
   uint64_t* clc_bar = item_empty + 2;
   int* items = reinterpret_cast<int*>(base + Sh::kOffItem);
@@ -428,12 +422,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
     }
-    for (int i = 0; i < 2 * kBufs; ++i) mbar_init(&s_full[i], 1);
+    for (int i = 0; i < 2 * kBufs; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&o_done[i], 1);
+    }
     for (int i = 0; i < kBufs; ++i) {
       mbar_init(&p_full[i], 128);
-      mbar_init(&b_free[i], 1);
+      mbar_init(&s_free[i], 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&o_done[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&item_full[i], 1);
       mbar_init(&item_empty[i], 11);  // 8 softmax warps, producer, two issuers
@@ -598,7 +594,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       int c = 0;  // K / V tiles loaded so far
       TcItem it;
       for (int k = 0; take_item(k, it); ++k) {
-        const int n_tiles = (max(tile_keys(it, 0), tile_keys(it, 1)) + kTcN - 1) / kTcN;
+        const int n_tiles = (max(tile_keys(it, 0), tile_keys(it, 1)) + kN - 1) / kN;
         if (k >= 1 && !__all_sync(0xffffffffu, mbar_wait(q_empty, (k - 1) & 1))) {
           if (lane == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
           break;
@@ -609,7 +605,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           for (int x = 0; x < (two ? 2 : 1); ++x)
 #pragma unroll
             for (int h = 0; h < kHalves; ++h)
-              tma_load_3d(base + Sh::kOffQ + x * Sh::kTile + h * kTcHalf, &qmap, q_full, h * 64, it.g * G,
+              tma_load_3d(base + Sh::kOffQ + x * Sh::kQTile + h * Sh::kQHalf, &qmap, q_full, h * 64, it.g * G,
                           it.q_begin + it.tok0 + x * TT);
         }
         __syncwarp();
@@ -626,11 +622,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               break;
             }
             if (elect_one()) {
-              mbar_arrive_expect_tx(full, Sh::kTile);
+              mbar_arrive_expect_tx(full, Sh::kKTile);
 #pragma unroll
               for (int h = 0; h < kHalves; ++h)
-                tma_load_3d(base + (kv ? Sh::kOffV : Sh::kOffK) + st * Sh::kTile + h * kTcHalf, kv ? &vmap : &kmap, full, h * 64, it.g,
-                            it.row0 + j * kTcN);
+                tma_load_3d(base + (kv ? Sh::kOffV : Sh::kOffK) + st * Sh::kKTile + h * Sh::kKHalf, kv ? &vmap : &kmap, full, h * 64, it.g,
+                            it.row0 + j * kN);
             }
             __syncwarp();
           }
@@ -645,20 +641,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // shared memory is broadcast, so that the compiler knows the loops to be
       // uniform and keeps the MMAs' operands in uniform registers.
       constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-      constexpr uint32_t kTileStep = Sh::kTile >> 4;
       auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
       int st = 0, buf = 0;                 // K / V stage, S buffer
       uint32_t st_ph = 0, buf_ph = 0;      // their phases
+      int turn[2] = {0, 0};                // the tile's next barrier of its ring
       int nt0 = 0, nt1 = 0;                // key tiles of A and B
       bool dead = false;
       auto open_item = [&](int k) {
         TcItem it;
         const bool ok = __all_sync(0xffffffffu, take_item(k, it));
-        nt0 = __shfl_sync(0xffffffffu, (tile_keys(it, 0) + kTcN - 1) / kTcN, 0);
-        nt1 = __shfl_sync(0xffffffffu, (tile_keys(it, 1) + kTcN - 1) / kTcN, 0);
+        nt0 = __shfl_sync(0xffffffffu, (tile_keys(it, 0) + kN - 1) / kN, 0);
+        nt1 = __shfl_sync(0xffffffffu, (tile_keys(it, 1) + kN - 1) / kN, 0);
         return ok;
       };
-      auto next_buf = [&]() {
+      // past a step of tile x
+      auto next_step = [&](int x) {
+        if (++turn[x] == kBufs) turn[x] = 0;
         if (++buf == kBufs) {
           buf = 0;
           buf_ph ^= 1;
@@ -671,70 +669,64 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       };
       if (warp == kTcQkWarp) {
-        constexpr uint32_t idesc = mma_idesc_f16(fmt, 0, 0, kTcN, kTcM);
+        constexpr uint32_t idesc = mma_idesc_f16(fmt, 0, 0, kN, kTcM);
         const uint32_t q_lo = ((sbase + Sh::kOffQ) >> 4) | (1u << 16), k_lo = ((sbase + Sh::kOffK) >> 4) | (1u << 16);
-        int made[2] = {0, 0};
         for (int k = 0; !dead && open_item(k); ++k) {
           if (!wait_all(q_full, k & 1)) { dead = true; break; }
           const int n_tiles = max(nt0, nt1);
           for (int j = 0; j < n_tiles && !dead; ++j) {
             if (!wait_all(&k_full[st], st_ph)) { dead = true; break; }
-            const uint32_t blo = k_lo + st * kTileStep;
+            const uint32_t blo = k_lo + st * (Sh::kKTile >> 4);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               if (j >= (x ? nt1 : nt0)) continue;
-              // the PV that read this buffer's P has completed
-              if (!wait_all(&b_free[buf], buf_ph ^ 1)) { dead = true; break; }
-              const uint32_t t_s = tbase + buf * 128;
+              if (!wait_all(&s_free[buf], buf_ph ^ 1)) { dead = true; break; }  // its last P has been read
+              const uint32_t t_s = tbase + buf * kN;
               // S signals a ring of barriers of its own tile: the other tile's softmax
               // may be items ahead, where it would take an old phase for its own
-              uint64_t* sf = s_full + x * kBufs + made[x];
+              uint64_t* sf = s_full + x * kBufs + turn[x];
               const bool last = x == 1 || j >= nt1;
               if (elect_one()) {
                 tc_fence_after();
 #pragma unroll
-                for (int kk = 0; kk < 4 * kHalves; ++kk) {
-                  const uint32_t off = (kk >> 2) * (kTcHalf >> 4) + (kk & 3) * 2;
-                  tc_mma_ss<kSmemDescHi>(t_s, q_lo + x * kTileStep + off, blo + off, idesc, kk > 0 ? 1u : 0u);
-                }
+                for (int kk = 0; kk < 4 * kHalves; ++kk)
+                  tc_mma_ss<kSmemDescHi>(t_s, q_lo + x * (Sh::kQTile >> 4) + (kk >> 2) * (Sh::kQHalf >> 4) + (kk & 3) * 2,
+                                         blo + (kk >> 2) * (Sh::kKHalf >> 4) + (kk & 3) * 2, idesc, kk > 0 ? 1u : 0u);
                 tc_commit(sf);
                 if (last) tc_commit(&k_empty[st]);
                 if (last && j + 1 == n_tiles) tc_commit(q_empty);
               }
               __syncwarp();
-              if (++made[x] == kBufs) made[x] = 0;
-              next_buf();
+              next_step(x);
             }
             next_stage();
           }
         }
       } else {
         constexpr uint32_t idesc = mma_idesc_f16(fmt, 0, 1, D, kTcM);
-        // V is the MN-major operand: 8 keys every 1024 bytes, the second 64 dims (D = 128) 16 KB on
-        const uint32_t v_lo = ((sbase + Sh::kOffV) >> 4) | (static_cast<uint32_t>(kHalves == 2 ? kTcHalf >> 4 : 1) << 16);
-        int done[2] = {0, 0};  // which of the two barriers of a tile is next
+        // V is the MN-major operand: 8 keys every 1024 bytes, the second 64 dims (D = 128) a half tile on
+        const uint32_t v_lo = ((sbase + Sh::kOffV) >> 4) | (static_cast<uint32_t>(kHalves == 2 ? Sh::kKHalf >> 4 : 1) << 16);
         for (int k = 0; !dead && open_item(k); ++k) {
           const int n_tiles = max(nt0, nt1);
           for (int j = 0; j < n_tiles && !dead; ++j) {
             if (!wait_all(&v_full[st], st_ph)) { dead = true; break; }
-            const uint32_t blo = v_lo + st * kTileStep;
+            const uint32_t blo = v_lo + st * (Sh::kKTile >> 4);
             const uint32_t keep = j > 0 ? 1u : 0u;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               if (j >= (x ? nt1 : nt0)) continue;
               if (!wait_all(&p_full[buf], buf_ph)) { dead = true; break; }
-              const uint32_t t_o = tbase + Sh::kColO + x * D, t_p = tbase + buf * 128;
+              const uint32_t t_o = tbase + Sh::kColO + x * D, t_p = tbase + buf * kN;
               if (elect_one()) {
                 tc_fence_after();
 #pragma unroll
-                for (int kk = 0; kk < 8; ++kk) tc_mma_ts<kSmemDescHi>(t_o, t_p + kk * 8, blo + kk * 128, idesc, kk > 0 ? 1u : keep);
-                tc_commit(&b_free[buf]);
-                tc_commit(o_done + 2 * x + done[x]);
+                for (int kk = 0; kk < kN / 16; ++kk) tc_mma_ts<kSmemDescHi>(t_o, t_p + kk * 8, blo + kk * 128, idesc, kk > 0 ? 1u : keep);
+                tc_commit(&s_free[buf]);
+                tc_commit(o_done + x * kBufs + turn[x]);
                 if (x == 1 || j >= nt1) tc_commit(&v_empty[st]);
               }
               __syncwarp();
-              done[x] ^= 1;
-              next_buf();
+              next_step(x);
             }
             next_stage();
           }
@@ -755,48 +747,46 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     bool dead = false;
     TcItem it;
     for (int k = 0; take_item(k, it); ++k) {
-      const int kvx = tile_keys(it, x), ntx = (kvx + kTcN - 1) / kTcN;
-      const int nto = (tile_keys(it, 1 - x) + kTcN - 1) / kTcN;
-      // PV number i of this item and tile has completed.  A wait tells a phase
-      // from the one before it only.  PVs signal two barriers in turn, and S of
-      // this tile's step i or i + 1, which the caller has seen, was issued
-      // after PV i - 3 at least: PV i - 1 can be waited for, and then PV i.
+      const int kvx = tile_keys(it, x), ntx = (kvx + kN - 1) / kN;
+      const int nto = (tile_keys(it, 1 - x) + kN - 1) / kN;
+      // PV number i of this item and tile has completed.  PVs signal a ring of
+      // barriers: a wait tells a phase from the one before it only, and the S
+      // that the caller has seen vouches for the PV a ring's length back.
       auto wait_pv = [&](int i) {
-#pragma unroll
-        for (int b = 1; b >= 0; --b) {
-          const int w = cx + i - b;
-          if (i >= b && !dead && !mbar_wait(&o_done[2 * x + (w & 1)], (w >> 1) & 1)) dead = true;
-        }
+        const int w = cx + i;
+        if (!dead && !mbar_wait(&o_done[x * kBufs + w % kBufs], (w / kBufs) & 1)) dead = true;
       };
       const int tok = it.tok0 + x * TT + rtok;
       const bool row_valid = rtok < TT && tok < it.n_new;
-      const int lim = row_valid ? min(it.prior + tok + 1, kvx) : 0;
+      // rows without a token are not stored, so they need no mask (one of them
+      // would send its warp through the masking code at every step)
+      const int lim = row_valid ? min(it.prior + tok + 1, kvx) : INT_MAX;
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < ntx; ++j) {
-        // this step's number: A(j) and B(j) alternate while both tiles have key tiles
+        // the step's number (A(j) and B(j) alternate while both tiles have key tiles), its S buffer
         const int n = n0 + (x == 0 ? (nto > 0 ? 2 * j : j) : (j < nto ? 2 * j + 1 : nto + j));
-        const uint32_t t_s = tbase + (n % kBufs) * 128 + lane_off;
+        const int b = n % kBufs;
+        const uint32_t t_s = tbase + b * kN + lane_off;
         if (!dead && !mbar_wait(&s_full[x * kBufs + (cx + j) % kBufs], ((cx + j) / kBufs) & 1)) dead = true;
         __syncwarp();
         tc_fence_after();
-        uint32_t sr[4][32];
+        uint32_t sr[kN / 32][32];
 #pragma unroll
-        for (int c4 = 0; c4 < 4; ++c4) tmem_ld32(t_s + c4 * 32, sr[c4]);
+        for (int c4 = 0; c4 < kN / 32; ++c4) tmem_ld32(t_s + c4 * 32, sr[c4]);
         tmem_wait_ld_regs(sr[0]);
-        reg_after_wait(sr[1]);
-        reg_after_wait(sr[2]);
-        reg_after_wait(sr[3]);
-        const int kbase = j * kTcN;
-        if (kbase + kTcN > lim) {
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
+        for (int c4 = 1; c4 < kN / 32; ++c4) reg_after_wait(sr[c4]);
+        const int kbase = j * kN;
+        if (kbase + kN > lim) {
+#pragma unroll
+          for (int c = 0; c < kN; ++c)
             if (kbase + c >= lim) sr[c >> 5][c & 31] = __float_as_uint(-INFINITY);
         }
         float m8[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q) m8[q] = fmaxf(__uint_as_float(sr[0][q]), __uint_as_float(sr[0][q + 8]));
 #pragma unroll
-        for (int c = 16; c < 128; c += 16) {
+        for (int c = 16; c < kN; c += 16) {
 #pragma unroll
           for (int q = 0; q < 8; ++q)
             m8[q] = fmax3(m8[q], __uint_as_float(sr[c >> 5][(c & 31) + q]), __uint_as_float(sr[(c + 8) >> 5][((c + 8) & 31) + q]));
@@ -813,7 +803,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         const float2 sl2v = make_float2(sl2, sl2), nmv = make_float2(nm, nm);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int half = 0; half < kN / 64; ++half) {
           uint32_t pk[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
@@ -824,20 +814,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             ls[i & 1] = __fadd2_rn(ls[i & 1], pp);
             pk[i] = pack2<T>(pp.x, pp.y);
           }
-          if (half == 0) {
-            if (rescale) {  // after the PV before this step
-              wait_pv(j - 1);
-              __syncwarp();
-              tc_fence_after();
+          if (half == 0 && rescale) {  // after the PV before this step
+            wait_pv(j - 1);
+            __syncwarp();
+            tc_fence_after();
 #pragma unroll
-              for (int c2 = 0; c2 < D / 32; ++c2) {
-                uint32_t orr[32];
-                tmem_ld32(t_o + c2 * 32, orr);
-                tmem_wait_ld_regs(orr);
+            for (int c2 = 0; c2 < D / 32; ++c2) {
+              uint32_t orr[32];
+              tmem_ld32(t_o + c2 * 32, orr);
+              tmem_wait_ld_regs(orr);
 #pragma unroll
-                for (int c = 0; c < 32; ++c) orr[c] = __float_as_uint(__uint_as_float(orr[c]) * factor);
-                tmem_st32(t_o + c2 * 32, orr);
-              }
+              for (int c = 0; c < 32; ++c) orr[c] = __float_as_uint(__uint_as_float(orr[c]) * factor);
+              tmem_st32(t_o + c2 * 32, orr);
             }
           }
           tmem_st32(t_s + half * 32, pk);
@@ -845,7 +833,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         l += (ls[0].x + ls[1].x) + (ls[0].y + ls[1].y);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&p_full[n % kBufs]);
+        mbar_arrive(&p_full[b]);
       }
       // ---- epilogue: O / l -> out
       bool fine = true;
@@ -857,7 +845,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_after();
         const float inv = l > 0.f ? 1.f / l : l;  // NaN stays
         float fsum = l;
-        T* orow = static_cast<T*>(a.out) + row * a.out_stride + static_cast<int64_t>(head) * D;
+        // 32 columns at a time through the warp's 2 KB: a store then covers 64
+        // bytes of each of 8 rows (each thread storing its own row, 16 bytes
+        // here and there, took 3,300 cycles an item at D = 64, 5,500 at 128)
+        const int64_t off = row * a.out_stride + static_cast<int64_t>(head) * D;
+        const unsigned rows_ok = __ballot_sync(0xffffffffu, row_valid);
+        uint8_t* mine = base + Sh::kOffOut + warp * 2048;
+        int64_t roff[4];
+#pragma unroll
+        for (int r8 = 0; r8 < 4; ++r8) roff[r8] = __shfl_sync(0xffffffffu, off, r8 * 8 + (lane >> 2));
 #pragma unroll
         for (int c2 = 0; c2 < D / 32; ++c2) {
           uint32_t o[32];
@@ -865,20 +861,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tmem_wait_ld_regs(o);
 #pragma unroll
           for (int i = 0; i < 32; ++i) fsum += fabsf(__uint_as_float(o[i]));
-          if (row_valid) {
 #pragma unroll
-            for (int c8 = 0; c8 < 4; ++c8) {
-              float f[8];
+          for (int c8 = 0; c8 < 4; ++c8) {
+            float f[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[c8 * 8 + i]) * inv;
-              uint4 v;
-              v.x = pack2<T>(f[0], f[1]);
-              v.y = pack2<T>(f[2], f[3]);
-              v.z = pack2<T>(f[4], f[5]);
-              v.w = pack2<T>(f[6], f[7]);
-              *reinterpret_cast<uint4*>(orow + c2 * 32 + c8 * 8) = v;
-            }
+            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[c8 * 8 + i]) * inv;
+            *reinterpret_cast<uint4*>(mine + lane * 64 + ((c8 ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
           }
+          __syncwarp();
+#pragma unroll
+          for (int r8 = 0; r8 < 4; ++r8) {
+            const int rr = r8 * 8 + (lane >> 2), c8 = lane & 3;
+            const uint4 v = *reinterpret_cast<const uint4*>(mine + rr * 64 + ((c8 ^ ((rr >> 1) & 3)) << 4));
+            if ((rows_ok >> rr) & 1) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + roff[r8] + c2 * 32 + c8 * 8) = v;
+          }
+          __syncwarp();
         }
         tc_fence_before();  // O is read before the next item's PV (ordered by p_full)
         fine = !row_valid || fsum < INFINITY;
@@ -939,8 +937,8 @@ cudaError_t launch_tc(const PackedArgs& a, cudaStream_t stream) {
   p.scale_log2 = a.scale * 1.4426950408889634f;
   CUtensorMap qm, km, vm;
   int rc = encode_rows_tensormap(&qm, a.q, a.q_stride, a.n_tokens, a.n_q_heads, D, a.dtype, p.group, p.tokens);
-  if (rc == 0) rc = encode_rows_tensormap(&km, a.k, a.k_stride, a.n_key_rows, a.n_kv_heads, D, a.dtype, 1, kTcN);
-  if (rc == 0) rc = encode_rows_tensormap(&vm, a.v, a.v_stride, a.n_key_rows, a.n_kv_heads, D, a.dtype, 1, kTcN);
+  if (rc == 0) rc = encode_rows_tensormap(&km, a.k, a.k_stride, a.n_key_rows, a.n_kv_heads, D, a.dtype, 1, TcShape<D>::kN);
+  if (rc == 0) rc = encode_rows_tensormap(&vm, a.v, a.v_stride, a.n_key_rows, a.n_kv_heads, D, a.dtype, 1, TcShape<D>::kN);
   if (rc != 0) return cudaErrorNotSupported;
   const int64_t items = (a.n_tokens / (2 * p.tokens) + static_cast<int64_t>(a.n_seqs)) * a.n_kv_heads;
   if (items > 0x7fffffff) return cudaErrorInvalidConfiguration;
