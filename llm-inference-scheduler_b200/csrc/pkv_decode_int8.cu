@@ -34,6 +34,7 @@
 // that several CTAs share in the workspace, joined in CTA order by a second
 // launch.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "pkv_common.cuh"
@@ -63,7 +64,9 @@ struct D8Params {
   int n_q_heads, n_kv_heads, group, chunks;  // chunks of 8 NT query heads per KV head
   int n_groups;                              // n_kv_heads * chunks
   int teams;                                 // per CTA
+  int min_tiles;                             // of a CTA's range
   int per_cta;                               // head groups per CTA
+  int q_vec;  // q rows take 8-byte (fp32: 16-byte) loads of four elements
   float scale_log2;
   float* part_o;   // [2 * grid][n_q_heads][D]
   float* part_ml;  // [2 * grid][n_q_heads][2]
@@ -135,8 +138,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
   __shared__ int wsum[WARPS];
   __shared__ int slot_seq[2 * WARPS];  // sequence of each team's partials (-1: none)
 
-  pdl_trigger();
   pdl_wait();  // the metadata, q and the pools may come from the kernel before this one
+  pdl_trigger();  // (after the wait: the merge reads the lengths before its own)
 
   // ---- tiles of each sequence, and their prefix
   {
@@ -172,7 +175,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
     __syncthreads();
   }
   const int total = prefix[B];
-  const int per = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), p.teams);
+  const int per = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), p.min_tiles);
   const int c0 = min(total, static_cast<int>(blockIdx.x) * per), c1 = min(total, c0 + per);
   const int team = warp / p.per_cta;
   const int hg = blockIdx.y * p.per_cta + (warp - team * p.per_cta);
@@ -183,18 +186,26 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
   const int nh = works ? min(kHeads, (kvh + 1) * p.group - head0) : 0;  // this warp's query heads
 
   if (r0 < r1) {
-    // ---- the ring: tile i of the range (i from 0) sits in stage i % STAGES
+    // ---- the ring: tiles of the range in order, STAGES - 1 ahead
     const int n_tiles = r1 - r0;
     const int64_t pitch = static_cast<int64_t>(p.n_kv_heads) * D;
+    const int64_t tile_bytes = 16 * pitch;
+    constexpr int cpr = D / 16, kCopies = 16 * cpr / 32;  // chunks of a row, copies of a lane for K (and V)
+    // this lane's chunk of a tile: row lane / cpr (+ 32 / cpr a copy), chunk lane % cpr
+    const int64_t lane_src = (lane / cpr) * pitch + (lane % cpr) * 16 + static_cast<int64_t>(kvh) * D;
+    const int8_t* k_src = p.k_pool + lane_src;
+    const int8_t* v_src = p.v_pool + lane_src;
+    const float* sc_src = (lane ? p.v_scale : p.k_scale) + kvh;
     const uint32_t ring_a = smem_u32(ring);
-    int ids = 0, ids_next = 0;  // lane l: first pool row / 16 of tile 32 b + l
+    uint32_t fill = ring_a;     // the stage the next copies go to
+    int ids = 0, ids_next = 0;  // lane l: first pool row / 16 of tile 32 b + l of the range
     auto load_ids = [&](int b) {
       const int i = b * 32 + lane;
       int row16 = 0;
       if (i < n_tiles) {
         const int s = d8_find(prefix, B, r0 + i);
         const int tile = r0 + i - prefix[s];
-        const int jb = tile / p.tiles_per_block;
+        const int jb = p.tiles_per_block == 1 ? tile : tile / p.tiles_per_block;
         int id = p.block_tables[static_cast<int64_t>(s) * p.bt_stride + jb];
         if (id < 0 || id >= p.num_blocks) {
           raise_flag(p.err, PKV_FLAG_BLOCK_OUT_OF_RANGE);
@@ -204,32 +215,35 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
       }
       return row16;
     };
-    auto issue = [&](int i) {
-      if ((i & 31) == 0) {
-        ids = i == 0 ? load_ids(0) : ids_next;
-        ids_next = load_ids((i >> 5) + 1);
-      }
-      const int row16 = __shfl_sync(0xffffffffu, ids, i & 31);
-      if (i < n_tiles) {
-        const uint32_t st = ring_a + (i % STAGES) * kStage;
-        const int64_t src = static_cast<int64_t>(row16) * 16 * pitch + static_cast<int64_t>(kvh) * D;
-        constexpr int cpr = D / 16;
-#pragma unroll
-        for (int c0_ = 0; c0_ < 16 * cpr; c0_ += 32) {
-          const int c = c0_ + lane, r = c / cpr, ch = c % cpr;
-          cp_async16(st + k_chunk<D>(r, ch), p.k_pool + src + r * pitch + ch * 16);
-          cp_async16(st + 16 * D + v_chunk<D>(r, ch), p.v_pool + src + r * pitch + ch * 16);
+    int to_issue = 0;
+    auto issue = [&]() {
+      if (to_issue < n_tiles) {
+        if ((to_issue & 31) == 0) {
+          ids = to_issue == 0 ? load_ids(0) : ids_next;
+          if (to_issue + 32 < n_tiles) ids_next = load_ids((to_issue >> 5) + 1);
         }
-        if (lane < 2)
-          cp_async4(st + 32 * D + lane * 4, (lane ? p.v_scale : p.k_scale) +
-                    static_cast<int64_t>(row16 / p.tiles_per_block) * p.n_kv_heads + kvh);
+        const int row16 = __shfl_sync(0xffffffffu, ids, to_issue & 31);
+        const int64_t src = row16 * tile_bytes;
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) {
+          const int ch = c * 32 + lane;
+          cp_async16(fill + k_chunk<D>(ch / cpr, ch % cpr), k_src + src + c * (32 / cpr) * pitch);
+          cp_async16(fill + 16 * D + v_chunk<D>(ch / cpr, ch % cpr), v_src + src + c * (32 / cpr) * pitch);
+        }
+        if (lane < 2) {
+          const int id = p.tiles_per_block == 1 ? row16 : row16 / p.tiles_per_block;
+          cp_async4(fill + 32 * D + lane * 4, sc_src + static_cast<int64_t>(id) * p.n_kv_heads);
+        }
+        fill = fill + kStage == ring_a + kRing ? ring_a : fill + kStage;
+        ++to_issue;
       }
       cp_commit();
     };
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) issue(i);
+    for (int i = 0; i < STAGES - 1; ++i) issue();
 
-    int s = d8_find(prefix, B, r0), pos = r0, i = 0;
+    int s = d8_find(prefix, B, r0), pos = r0;
+    const uint8_t* st = ring;  // the stage of the tile at pos
     while (pos < r1) {
       const int seg_end = min(prefix[s + 1], r1);
       const int ctx = ctxs[s];
@@ -248,10 +262,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk) {
           const int d0 = (kk >> 2) * 64 + 16 * t + 4 * (kk & 3);
+          if (on && p.q_vec) {
+            load4_f<T>(row + d0, f[kk]);
+          } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            f[kk][e] = on ? Elem<T>::to_f(row[d0 + e]) : 0.f;
-            amax = fmaxf(amax, fabsf(f[kk][e]));
+            for (int e = 0; e < 4; ++e) f[kk][e] = on ? Elem<T>::to_f(row[d0 + e]) : 0.f;
+          }
+          if (!std::is_same<T, __half>::value) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(f[kk][e]));
           }
         }
         float back = 1.f, inv = 1.f;
@@ -283,28 +302,26 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
         c_head[nt][0] = p.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * t);
         c_head[nt][1] = p.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * t + 4);
       }
-      float m[NT][2], mu[NT][2], l[NT][2], o[NT][KS][4];
+      // mu: the reference of the exponentials, at most kD8Slack (log2) below the
+      // running maximum; it moves when some score passes that, which a vote of the
+      // lanes' own scores tells, so most tiles need no maximum across lanes
+      float mu[NT][2], l[NT][2], o[NT][KS][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          m[nt][c] = -INFINITY;
-          mu[nt][c] = l[nt][c] = 0.f;
-        }
+        mu[nt][0] = mu[nt][1] = l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
         for (int j = 0; j < KS; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
       }
       float v_ref = 0.f, v_inv = 0.f;  // 2^E and 2^-E (0: no tile yet)
+      bool fresh = true;               // no tile of the segment yet
 
       int left = ctx - (pos - prefix[s]) * 16;  // tokens from this tile on
-      for (; pos < seg_end; ++pos, ++i, left -= 16) {
+      for (; pos < seg_end; ++pos, left -= 16) {
         cp_wait<STAGES - 2>();
-        __syncwarp();  // every lane's copies of tile i are in, and every lane is done with tile i - 1
-        issue(i + STAGES - 1);
-        const uint8_t* st = ring + (i % STAGES) * kStage;
+        __syncwarp();  // every lane's copies of this tile are in, and every lane is done with the one before
+        issue();
         const float ks = *reinterpret_cast<const float*>(st + 32 * D);
         const float vs = *reinterpret_cast<const float*>(st + 32 * D + 4);
-        const int valid = min(16, left);
         // ---- S^T = K Q^T
         float sc[NT][4];
 #pragma unroll
@@ -324,30 +341,28 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
                 mma16816<__half>(sc[nt], a, qb[nt][lb][half * 4 + k4][0], qb[nt][lb][half * 4 + k4][1]);
           }
         }
-        // ---- online softmax (exp2), P scaled by V's scale over 2^E
-        bool grow = false;
+        // ---- x - mu of the lane's scores (tokens g, g + 8; heads 2t, 2t + 1)
+        float2 x0[NT], x1[NT];
+        float top = -INFINITY;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float f0 = c_head[nt][0] * ks, f1 = c_head[nt][1] * ks;
-          sc[nt][0] = g < valid ? sc[nt][0] * f0 : -INFINITY;
-          sc[nt][1] = g < valid ? sc[nt][1] * f1 : -INFINITY;
-          sc[nt][2] = g + 8 < valid ? sc[nt][2] * f0 : -INFINITY;
-          sc[nt][3] = g + 8 < valid ? sc[nt][3] * f1 : -INFINITY;
+          const float2 f = __fmul2_rn(make_float2(c_head[nt][0], c_head[nt][1]), make_float2(ks, ks));
+          const float2 nm = make_float2(-mu[nt][0], -mu[nt][1]);
+          x0[nt] = __ffma2_rn(make_float2(sc[nt][0], sc[nt][1]), f, nm);
+          x1[nt] = __ffma2_rn(make_float2(sc[nt][2], sc[nt][3]), f, nm);
         }
-        float mx[NT][2];
+        if (left < 16) {  // a sequence's last tile
+          const float2 none = make_float2(-INFINITY, -INFINITY);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mx[nt][0] = fmaxf(sc[nt][0], sc[nt][2]);
-          mx[nt][1] = fmaxf(sc[nt][1], sc[nt][3]);
-#pragma unroll
-          for (int off = 4; off < 32; off <<= 1) {
-            mx[nt][0] = fmaxf(mx[nt][0], __shfl_xor_sync(0xffffffffu, mx[nt][0], off));
-            mx[nt][1] = fmaxf(mx[nt][1], __shfl_xor_sync(0xffffffffu, mx[nt][1], off));
+          for (int nt = 0; nt < NT; ++nt) {
+            if (g >= left) x0[nt] = none;
+            if (g + 8 >= left) x1[nt] = none;
           }
-          grow = grow || mx[nt][0] > m[nt][0] + kD8Slack || mx[nt][1] > m[nt][1] + kD8Slack;
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) top = fmax3(top, fmaxf(x0[nt].x, x0[nt].y), fmaxf(x1[nt].x, x1[nt].y));
         const bool wider = vs > v_ref;  // warp-uniform
-        if (wider || __any_sync(0xffffffffu, grow)) {
+        if (__any_sync(0xffffffffu, top > kD8Slack) || wider || fresh) {
           const float vf = wider ? v_ref * (1.f / vs) : 1.f;  // exact
           if (wider) {
             v_ref = vs;
@@ -355,37 +370,45 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float cf[2];
+            float mx[2] = {fmaxf(x0[nt].x, x1[nt].x), fmaxf(x0[nt].y, x1[nt].y)}, cf[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              const float mn = fmaxf(m[nt][c], mx[nt][c]);
-              const float mun = mn == -INFINITY ? 0.f : mn;
-              cf[c] = ex2_approx(m[nt][c] - mun);
-              m[nt][c] = mn;
-              mu[nt][c] = mun;
+#pragma unroll
+              for (int off = 4; off < 32; off <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], off));
+              // the reference moves up by mx (the segment's first tile: to its maximum, unless that is not finite)
+              float up = fresh ? mx[c] : fmaxf(mx[c], 0.f);
+              if (!(fabsf(up) < INFINITY)) up = 0.f;
+              cf[c] = ex2_approx(-up);
+              mu[nt][c] += up;
               l[nt][c] *= cf[c];
+              mx[c] = up;
               cf[c] *= vf;
             }
+            const float2 nu = make_float2(-mx[0], -mx[1]);
+            x0[nt] = __fadd2_rn(x0[nt], nu);
+            x1[nt] = __fadd2_rn(x1[nt], nu);
+            if (!fresh) {
 #pragma unroll
-            for (int j = 0; j < KS; ++j) {
-              o[nt][j][0] *= cf[0];
-              o[nt][j][1] *= cf[1];
-              o[nt][j][2] *= cf[0];
-              o[nt][j][3] *= cf[1];
+              for (int j = 0; j < KS; ++j) {
+                o[nt][j][0] *= cf[0];
+                o[nt][j][1] *= cf[1];
+                o[nt][j][2] *= cf[0];
+                o[nt][j][3] *= cf[1];
+              }
             }
           }
+          fresh = false;
         }
-        const float vfac = vs * v_inv;
+        const float2 vfac = make_float2(vs * v_inv, vs * v_inv);
         uint32_t pb[NT][LIMBS][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float e[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) e[c] = ex2_approx(sc[nt][c] - mu[nt][c & 1]);
-          l[nt][0] += e[0] + e[2];
-          l[nt][1] += e[1] + e[3];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) e[c] *= vfac;
+          const float2 p0 = make_float2(ex2_approx(x0[nt].x), ex2_approx(x0[nt].y));
+          const float2 p1 = make_float2(ex2_approx(x1[nt].x), ex2_approx(x1[nt].y));
+          l[nt][0] += p0.x + p1.x;
+          l[nt][1] += p0.y + p1.y;
+          const float2 e0 = __fmul2_rn(p0, vfac), e1 = __fmul2_rn(p1, vfac);
+          float e[4] = {e0.x, e0.y, e1.x, e1.y};
           pb[nt][0][0] = movmatrix_t(pack2<__half>(e[0], e[1]));
           pb[nt][0][1] = movmatrix_t(pack2<__half>(e[2], e[3]));
           if constexpr (LIMBS == 2) {
@@ -421,6 +444,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
                 mma16816<__half>(o[nt][half * 4 + mt], a, pb[nt][lb][0], pb[nt][lb][1]);
           }
         }
+        st = st + kStage == ring + kRing ? ring : st + kStage;
       }
 
       // ---- segment end
@@ -469,7 +493,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
               slot[hh * D + d + 1] = o[nt][j][c + 2] * f;
             }
             if (g == 0) {
-              slot[kHeads * D + 2 * hh] = m[nt][c];
+              slot[kHeads * D + 2 * hh] = mu[nt][c];
               slot[kHeads * D + 2 * hh + 1] = l[nt][c];
             }
           }
@@ -483,68 +507,74 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
   __syncthreads();
 
   // ---- join the teams' partials: runs of slots of one sequence, in order
-  const int n_slots = 2 * p.teams;
-  for (int a = 0; a < n_slots;) {
-    const int s = slot_seq[a];
-    if (s < 0) {
-      ++a;
-      continue;
-    }
-    int b = a + 1;
-    while (b < n_slots && (slot_seq[b] == s || slot_seq[b] < 0)) ++b;
-    const bool complete = prefix[s] >= c0 && prefix[s + 1] <= c1;
-    const int64_t part = prefix[s] > c0 ? 2 * blockIdx.x + 1 : 2 * blockIdx.x;
-    const int n_out = p.per_cta * kHeads * D;
-    for (int e = tid; e < n_out; e += WARPS * 32) {
-      const int w = e / (kHeads * D), hh = (e - w * kHeads * D) / D, d = e % D;
-      const int hgw = blockIdx.y * p.per_cta + w;
-      if (hgw >= p.n_groups) continue;
-      const int kv = hgw / p.chunks, hd0 = kv * p.group + (hgw - kv * p.chunks) * kHeads;
-      if (hd0 + hh >= (kv + 1) * p.group) continue;
-      auto slot_of = [&](int k) {
-        const int wp = (k >> 1) * p.per_cta + w;
-        return (k & 1) ? reinterpret_cast<const float*>(d8_smem + wp * kRing) : heads_part + wp * kSlot;
-      };
-      float mm = -INFINITY;
-      for (int k = a; k < b; ++k)
-        if (slot_seq[k] >= 0) mm = fmaxf(mm, slot_of(k)[kHeads * D + 2 * hh]);
-      const float base = mm == -INFINITY ? 0.f : mm;
-      float ll = 0.f, oo = 0.f;
-      for (int k = a; k < b; ++k)
-        if (slot_seq[k] >= 0) {
-          const float* sl = slot_of(k);
-          const float f = ex2_approx(sl[kHeads * D + 2 * hh] - base) * sl[kHeads * D + 2 * hh + 1];
-          ll += f;
-          oo += f * sl[hh * D + d];
-        }
-      const int head = hd0 + hh;
-      if (complete) {
-        static_cast<T*>(p.out)[static_cast<int64_t>(s) * p.out_stride + static_cast<int64_t>(head) * D + d] =
-            Elem<T>::from_f(oo / ll);
-      } else {
-        p.part_o[(part * p.n_q_heads + head) * D + d] = oo / ll;
-        if (d == 0) {
-          p.part_ml[(part * p.n_q_heads + head) * 2] = mm;
-          p.part_ml[(part * p.n_q_heads + head) * 2 + 1] = ll;
-        }
+  __shared__ int n_runs, run_lo[2 * WARPS], run_n[2 * WARPS], slots[2 * WARPS];
+  if (tid == 0) {
+    int r = 0, k = 0;
+    for (int a = 0; a < 2 * p.teams; ++a) {
+      if (slot_seq[a] < 0) continue;
+      if (k == 0 || slot_seq[a] != slot_seq[slots[k - 1]]) {
+        run_lo[r] = k;
+        run_n[r++] = 0;
       }
+      slots[k++] = a;
+      ++run_n[r - 1];
     }
-    a = b;
+    n_runs = r;
+  }
+  __syncthreads();
+  constexpr int kVec = D / 4;
+  const int per_run = p.per_cta * kHeads * kVec;  // four dims at a time
+  for (int e = tid; e < n_runs * per_run; e += WARPS * 32) {
+    const int r = e / per_run, w = (e - r * per_run) / (kHeads * kVec), hh = (e / kVec) % kHeads, v = e % kVec;
+    const int hgw = blockIdx.y * p.per_cta + w;
+    if (hgw >= p.n_groups) continue;
+    const int kv = p.chunks == 1 ? hgw : hgw / p.chunks, head = kv * p.group + (hgw - kv * p.chunks) * kHeads + hh;
+    if (head >= (kv + 1) * p.group) continue;
+    float mm = 0.f, ll = 0.f;
+    float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int lo = run_lo[r], n = run_n[r];
+    for (int k = 0; k < n; ++k) {
+      const int a = slots[lo + k], wp = (a >> 1) * p.per_cta + w;
+      const float* sl = (a & 1) ? reinterpret_cast<const float*>(d8_smem + wp * kRing) : heads_part + wp * kSlot;
+      const float2 ml = *reinterpret_cast<const float2*>(sl + kHeads * D + 2 * hh);
+      const float4 x = *reinterpret_cast<const float4*>(sl + hh * D + 4 * v);
+      const float mn = k ? fmaxf(mm, ml.x) : ml.x;
+      const float fa = ex2_approx(mm - mn), fb = ex2_approx(ml.x - mn) * ml.y;
+      mm = mn;
+      ll = ll * fa + fb;
+      oo = make_float4(oo.x * fa + x.x * fb, oo.y * fa + x.y * fb, oo.z * fa + x.z * fb, oo.w * fa + x.w * fb);
+    }
+    const int s = slot_seq[slots[lo]];
+    const float inv = 1.f / ll;
+    oo = make_float4(oo.x * inv, oo.y * inv, oo.z * inv, oo.w * inv);
+    if (prefix[s] >= c0 && prefix[s + 1] <= c1) {  // all of it in this CTA
+      T* op = static_cast<T*>(p.out) + static_cast<int64_t>(s) * p.out_stride + static_cast<int64_t>(head) * D + 4 * v;
+      op[0] = Elem<T>::from_f(oo.x);
+      op[1] = Elem<T>::from_f(oo.y);
+      op[2] = Elem<T>::from_f(oo.z);
+      op[3] = Elem<T>::from_f(oo.w);
+    } else {
+      const int64_t part = prefix[s] > c0 ? 2 * blockIdx.x + 1 : 2 * blockIdx.x;
+      reinterpret_cast<float4*>(p.part_o + (part * p.n_q_heads + head) * D)[v] = oo;
+      if (v == 0) *reinterpret_cast<float2*>(p.part_ml + (part * p.n_q_heads + head) * 2) = make_float2(mm, ll);
+    }
   }
 }
 
 // Joins the CTAs' partials of sequence blockIdx.x (heads blockIdx.y * heads_per ..):
-// O = sum_c w_c O_c / sum_c w_c, w_c = 2^(m_c - M) l_c, over the CTAs that share it, in
-// order.  16 lanes of partials per head element group; empty sequences get zeros.
-constexpr int kM8Threads = 256;
+// O = sum_c w_c O_c / sum_c w_c, w_c = 2^(m_c - M) l_c, over the CTAs that share
+// it, in order.  Four dims of one head to a thread; a sequence that many CTAs
+// share (a long one) is read by all the CTA's threads, kLanes partials of a head
+// side by side.  Empty sequences get zeros.  The lengths are read while the
+// decode kernel runs (it starts this one after its own wait for them).
+constexpr int kM8Threads = 256, kM8Few = 6;
 template <typename T, int D>
 __global__ void __launch_bounds__(kM8Threads) merge_int8_kernel(const D8Params p, int grid, int heads_per) {
-  constexpr int kVec = D / 4, kLanes = kM8Threads / kVec;  // partials read side by side
+  constexpr int kVec = D / 4, kLanes = kM8Threads / kVec;
   __shared__ float4 s_o[kLanes][kVec];
   __shared__ float s_m[kLanes], s_l[kLanes];
   __shared__ int red[2][kM8Threads / 32];
   const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  pdl_wait();
   const int64_t room = static_cast<int64_t>(p.max_blocks) * p.tiles_per_block * 16;
   auto tiles_of = [&](int i) {
     return static_cast<int>((min(static_cast<int64_t>(max(p.context_lens[i], 0)), room) + 15) >> 4);
@@ -563,49 +593,88 @@ __global__ void __launch_bounds__(kM8Threads) merge_int8_kernel(const D8Params p
 #pragma unroll
   for (int w = 0; w < kM8Threads / 32; ++w) { before += red[0][w]; total += red[1][w]; }
   const int mine = tiles_of(s);
-  const int per = max((total + grid - 1) / grid, p.teams);
+  const int per = max((total + grid - 1) / grid, p.min_tiles);
   const int h0 = blockIdx.y * heads_per, h1 = min(p.n_q_heads, h0 + heads_per);
   T* orow = static_cast<T*>(p.out) + static_cast<int64_t>(s) * p.out_stride;
+  const int first = mine ? before / per : 0, last = mine ? (before + mine - 1) / per : 0;
+  pdl_wait();  // the decode grid's partials are in memory
   if (mine == 0) {
     for (int e = h0 * D + tid; e < h1 * D; e += kM8Threads) orow[e] = Elem<T>::from_f(0.f);
     return;
   }
-  const int first = before / per, last = (before + mine - 1) / per;
   if (first == last) return;  // one CTA had it all and wrote it
-  const int v = tid % kVec, k0 = tid / kVec;
-  for (int h = h0; h < h1; ++h) {
-    float m = -INFINITY, l = 0.f;
+  struct Acc {
+    float m = 0.f, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = first + k0; c <= last; c += kLanes) {
-      const int64_t part = before > c * per ? 2 * static_cast<int64_t>(c) + 1 : 2 * static_cast<int64_t>(c);
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (part * p.n_q_heads + h) * 2);
-      const float4 x = reinterpret_cast<const float4*>(p.part_o + (part * p.n_q_heads + h) * D)[v];
-      const float mn = fmaxf(m, ml.x), base = mn == -INFINITY ? 0.f : mn;
-      const float fa = ex2_approx(m - base), fb = ex2_approx(ml.x - base) * ml.y;
+    bool any = false;
+    __device__ void add(float2 ml, float4 x) {
+      const float mn = any ? fmaxf(m, ml.x) : ml.x;
+      const float fa = ex2_approx(m - mn), fb = ex2_approx(ml.x - mn) * ml.y;
       m = mn;
+      any = true;
       l = l * fa + fb;
       o = make_float4(o.x * fa + x.x * fb, o.y * fa + x.y * fb, o.z * fa + x.z * fb, o.w * fa + x.w * fb);
     }
-    s_o[k0][v] = o;
-    if (v == 0) { s_m[k0] = m; s_l[k0] = l; }
+  };
+  auto part_of = [&](int c) { return 2 * static_cast<int64_t>(c) + (before > static_cast<int64_t>(c) * per ? 1 : 0); };
+  auto load_o = [&](int64_t part, int h, int v) {
+    return reinterpret_cast<const float4*>(p.part_o + (part * p.n_q_heads + h) * D)[v];
+  };
+  auto load_ml = [&](int64_t part, int h) {
+    return *reinterpret_cast<const float2*>(p.part_ml + (part * p.n_q_heads + h) * 2);
+  };
+  auto store = [&](int h, int v, const Acc& a) {
+    T* op = orow + static_cast<int64_t>(h) * D + 4 * v;
+    const float inv = 1.f / a.l;
+    op[0] = Elem<T>::from_f(a.o.x * inv);
+    op[1] = Elem<T>::from_f(a.o.y * inv);
+    op[2] = Elem<T>::from_f(a.o.z * inv);
+    op[3] = Elem<T>::from_f(a.o.w * inv);
+  };
+  if (last - first < kM8Few) {
+    for (int e = tid; e < (h1 - h0) * kVec; e += kM8Threads) {
+      const int h = h0 + e / kVec, v = e % kVec;
+      float2 ml[kM8Few];
+      float4 x[kM8Few];
+#pragma unroll
+      for (int k = 0; k < kM8Few; ++k)
+        if (first + k <= last) {
+          ml[k] = load_ml(part_of(first + k), h);
+          x[k] = load_o(part_of(first + k), h, v);
+        }
+      Acc a;
+#pragma unroll
+      for (int k = 0; k < kM8Few; ++k)
+        if (first + k <= last) a.add(ml[k], x[k]);
+      store(h, v, a);
+    }
+    return;
+  }
+  const int v = tid % kVec, k0 = tid / kVec;
+  for (int h = h0; h < h1; ++h) {
+    Acc a;
+#pragma unroll 4
+    for (int c = first + k0; c <= last; c += kLanes) a.add(load_ml(part_of(c), h), load_o(part_of(c), h, v));
+    s_o[k0][v] = a.o;
+    if (v == 0) {
+      s_m[k0] = a.m;
+      s_l[k0] = a.any ? a.l : -1.f;
+    }
     __syncthreads();
     if (k0 == 0) {
-      float mm = -INFINITY;
-      for (int k = 0; k < kLanes; ++k) mm = fmaxf(mm, s_m[k]);
-      const float base = mm == -INFINITY ? 0.f : mm;
-      float ll = 0.f;
-      o = make_float4(0.f, 0.f, 0.f, 0.f);
+      Acc all;
       for (int k = 0; k < kLanes; ++k) {
-        const float f = ex2_approx(s_m[k] - base);
+        if (s_l[k] == -1.f) continue;  // no partial (sums are not negative)
+        // a.o is already weighted: as a partial of weight 1 and sum l
+        const float mn = all.any ? fmaxf(all.m, s_m[k]) : s_m[k];
+        const float fa = ex2_approx(all.m - mn), fb = ex2_approx(s_m[k] - mn);
         const float4 x = s_o[k][v];
-        ll += f * s_l[k];
-        o = make_float4(o.x + f * x.x, o.y + f * x.y, o.z + f * x.z, o.w + f * x.w);
+        all.m = mn;
+        all.any = true;
+        all.l = all.l * fa + fb * s_l[k];
+        all.o = make_float4(all.o.x * fa + x.x * fb, all.o.y * fa + x.y * fb, all.o.z * fa + x.z * fb, all.o.w * fa + x.w * fb);
       }
-      T* op = orow + static_cast<int64_t>(h) * D + 4 * v;
-      op[0] = Elem<T>::from_f(o.x / ll);
-      op[1] = Elem<T>::from_f(o.y / ll);
-      op[2] = Elem<T>::from_f(o.z / ll);
-      op[3] = Elem<T>::from_f(o.w / ll);
+      store(h, v, all);
     }
     __syncthreads();
   }
@@ -618,11 +687,17 @@ cudaError_t launch_d8(const AttnArgs& a, void* workspace, cudaStream_t stream) {
   constexpr int kFixed = WARPS * (STAGES * d8_stage<D>() + 8 * NT * (D + 2) * 4);
   constexpr int kMost = kFixed + (2 * kD8MaxSeqs + 1) * 4;
   static_assert(kMost + 1024 <= 232448, "the rings and partials fit the 227 KB of shared memory");
-  int dev = 0, sms = 0;
+  static std::atomic<int> sm_count[64];  // per device, 0: not asked
+  int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
   if (e != cudaSuccess) return e;
+  int sms = dev < 64 ? sm_count[dev].load() : 0;
+  if (sms == 0) {
+    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) sm_count[dev].store(sms);
+  }
   D8Params p{};
   p.k_pool = static_cast<const int8_t*>(a.k_pool);
   p.v_pool = static_cast<const int8_t*>(a.v_pool);
@@ -639,6 +714,7 @@ cudaError_t launch_d8(const AttnArgs& a, void* workspace, cudaStream_t stream) {
   p.n_groups = p.n_kv_heads * p.chunks;
   p.per_cta = std::min(p.n_groups, 8);
   p.teams = WARPS / p.per_cta;
+  p.min_tiles = 2 * p.teams;
   p.scale_log2 = a.scale * kD8Log2e;
   p.out_stride = a.out_stride;
   p.q_stride = a.q_stride;
@@ -655,6 +731,7 @@ cudaError_t launch_d8(const AttnArgs& a, void* workspace, cudaStream_t stream) {
   cfg.numAttrs = 1;
   cfg.stream = stream;
   const int es = sizeof(T);
+  p.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | static_cast<uintptr_t>(a.q_stride * es)) & (4 * es - 1)) == 0;
   for (int s0 = 0; s0 < a.n_seqs; s0 += kD8MaxSeqs) {
     p.n_seqs = std::min(kD8MaxSeqs, a.n_seqs - s0);
     p.out = static_cast<uint8_t*>(a.out) + s0 * a.out_stride * es;
