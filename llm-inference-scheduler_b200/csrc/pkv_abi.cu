@@ -155,20 +155,24 @@ int encode_pool_tensormap(CUtensorMap* map, const void* pool, int num_blocks, in
   if (enc == nullptr) return PKV_ERR_DRIVER;
   // 16-bit pools: 128-byte rows with the 128-byte swizzle (ldmatrix reads them
   // in place); fp8 pools: 64-byte rows, unswizzled (converted by the consumers)
-  const bool fp8 = dtype == kPoolFp8;
-  const cuuint64_t es = fp8 ? 1 : 2;
+  // int8 pools: rows of 64 or 128 bytes swizzled over their own length, 16 at a time
+  const bool fp8 = dtype == kPoolFp8, int8 = dtype == kPoolInt8;
+  const cuuint64_t es = fp8 || int8 ? 1 : 2;
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(n_kv_heads),
                               static_cast<cuuint64_t>(num_blocks) * block_size};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_dim) * es,
                                  static_cast<cuuint64_t>(n_kv_heads) * head_dim * es};
-  const cuuint32_t box[3] = {static_cast<cuuint32_t>(head_dim), 1u, static_cast<cuuint32_t>(block_size)};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(head_dim), 1u,
+                             static_cast<cuuint32_t>(int8 ? 16 : block_size)};
   const cuuint32_t estr[3] = {1u, 1u, 1u};
-  const CUtensorMapDataType dt = fp8                      ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+  const CUtensorMapDataType dt = fp8 || int8              ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                  : dtype == PKV_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const CUresult r = enc(map, dt, 3, const_cast<void*>(pool), dims, strides, box, estr,
                          CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         fp8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                         fp8                      ? CU_TENSOR_MAP_SWIZZLE_NONE
+                         : int8 && head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                  : CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : PKV_ERR_DRIVER;
 }

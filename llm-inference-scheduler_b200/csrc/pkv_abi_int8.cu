@@ -190,7 +190,11 @@ int pkv_paged_decode_attention_int8(void* out, int64_t out_row_stride, const voi
   a.err = err_flags;
   a.k_scale = k_scale;
   a.v_scale = v_scale;
-  return status(launch_decode_int8(a, workspace, static_cast<cudaStream_t>(stream)));
+  CUtensorMap km, vm;
+  rc = pool_tensormap(&km, k_pool, num_blocks, block_size, n_kv_heads, head_dim, kPoolInt8);
+  if (rc == 0) rc = pool_tensormap(&vm, v_pool, num_blocks, block_size, n_kv_heads, head_dim, kPoolInt8);
+  if (rc != 0) return rc;
+  return status(launch_decode_int8(a, &km, &vm, workspace, static_cast<cudaStream_t>(stream)));
 }
 
 // rows per sequence of the laid-out keys: whole key tiles

@@ -8,31 +8,34 @@
 // Mathematics.  With k_j = 2^a_b K_j and v_j = 2^c_b V_j (K, V integers, b the
 // block of token j), x_j = (scale 2^a_b) (q . K_j) and
 //   o = sum_j softmax(x)_j 2^c_b V_j.
-// The integers are exact in fp16, so the products run on the tensor cores
-// (m16n8k16, fp32 sums): S^T = K Q^T with 16 tokens as M and 8 query heads of
-// the GQA group as N, O^T += V^T P^T.  The K scale multiplies the fp32 scores.
-// The V scale goes into P as 2^(c_b - E), E the largest exponent seen so far (a
-// larger one rescales O, exactly), and 2^E into O at the end; the row sum takes
-// the unscaled p.  Running maximum, sums and O are fp32.  q is fp16; bf16 rows
-// are brought into fp16 range by the power of two of their largest value (8 bits
-// fit exactly but for elements 2^-16 below the row's largest, whose error is
-// 2^-25 of it).  fp32 rows, and the P that go with them, are split into two fp16
-// parts (22 bits) and each product is two MMAs.
-//
-// Converting a byte costs no conversion instruction: x ^ 0x80 = x + 128 becomes
-// the low byte of the fp16 1024 + 128 + x (a byte permute), and subtracting 1152
-// is exact.  fp8 bytes need the conversion pipe, which bounds the fp8 kernel at
-// about half of the HBM rate.
+// Scores.  S^T = K Q^T on the integer tensor cores (m16n8k32, 16 tokens as M, the
+// 8 query heads of a GQA group as N), which take K's bytes as they lie.  A q row
+// is brought by a power of two to integers below 2^22 and split into three signed
+// bytes, q = 2^e (65536 A + 256 B + C): exact for fp16 / bf16 elements down to
+// 2^-11 / 2^-14 of the row's largest, off by at most 2^-22 of it below and for fp32.  The
+// three int32 products are exact; they are joined in fp32.
+// Values.  O^T += V^T P^T in fp16 with fp32 sums (m16n8k16).  V's integers are
+// exact in fp16, and no conversion instruction makes them: x ^ 0x80 = x + 128
+// becomes the low byte of the fp16 1024 + 128 + x (a byte permute), and
+// subtracting 1152 is exact.  (fp8 bytes need the conversion pipe, which bounds
+// the fp8 kernel at about half of the HBM rate.)  The V scale goes into P as
+// 2^(c_b - E), E the largest exponent seen so far (a larger one rescales O,
+// exactly), and 2^E into O at the end; the row sum takes the unscaled p.  For
+// fp32 q, P is split into two fp16 parts (22 bits) and each product is two MMAs.
+// Maximum, sums and O are fp32.
 //
 // Work split.  The 16-token tiles of all sequences are cut into one contiguous
 // range per CTA and the range into one sub-range per team of warps (one warp per
 // KV head and chunk of query heads, so the heads of a token are read at about
 // the same time).  Each warp streams its tiles through its own ring of
-// shared-memory stages with 16-byte cp.async (no barrier between warps: a warp
-// waits only for its own copies).  Partial (m, l, O) of a sequence that several
+// shared-memory stages by TMA: it fills a stage once its own lanes are done with
+// it, so no warp waits for another.  Partial (m, l, O) of a sequence that several
 // teams share meet in shared memory at the end of the CTA, those of a sequence
 // that several CTAs share in the workspace, joined in CTA order by a second
 // launch.
+//
+// What bounds it: instructions.  At 256 sequences of about 1,024 tokens (14 / 2
+// heads, 74 MB) the bytes take 11.3 us at the copy rate.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -73,17 +76,18 @@ struct D8Params {
   int* err;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// D = A B + C on int8 (16 x 32 by 32 x 8, int32 sums)
+__device__ __forceinline__ void mma16832_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7},"
+      " {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ uint32_t pack_s8(int a, int b, int c, int d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
 // bytes (biased by 128) -> fp16 pairs; magic = 0x64646464
 __device__ __forceinline__ uint32_t sub1152(uint32_t h) {
   const __half2 c = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
@@ -92,10 +96,6 @@ __device__ __forceinline__ uint32_t sub1152(uint32_t h) {
 }
 __device__ __forceinline__ uint32_t i8_lo(uint32_t biased) { return sub1152(__byte_perm(biased, 0x64646464u, 0x4140)); }
 __device__ __forceinline__ uint32_t i8_hi(uint32_t biased) { return sub1152(__byte_perm(biased, 0x64646464u, 0x4342)); }
-
-__device__ __forceinline__ uint4 flip(uint4 w) {
-  return make_uint4(w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u);
-}
 
 // last s in [0, n) with prefix[s] <= x
 __device__ __forceinline__ int d8_find(const int* prefix, int n, int x) {
@@ -107,27 +107,29 @@ __device__ __forceinline__ int d8_find(const int* prefix, int n, int x) {
   return lo;
 }
 
-// stage: K tile, V tile (16 rows x D bytes each), K scale, V scale
-template <int D> __host__ __device__ constexpr int d8_stage() { return 2 * 16 * D + 16; }
-// Position of the 16-byte chunk c of row r.  K is read 16 bytes a lane (row g,
-// chunk t), V 8 bytes a lane (rows 2t + {0, 1, 8, 9} in an order that depends on
-// t's parity): both orders fill all banks.
-template <int D> __device__ __forceinline__ int k_chunk(int r, int c) {
-  return D == 64 ? r * 64 + c * 16 : r * 128 + ((c ^ ((r & 1) << 2)) << 4);
+// stage: K tile, V tile (16 rows x D bytes each, TMA's 64- or 128-byte swizzle)
+template <int D> __host__ __device__ constexpr int d8_stage() { return 2 * 16 * D; }
+// position of the 16-byte chunk c of row r.  The lanes read K as row g, chunk t
+// (D = 128: 2t, 2t + 1) and V 8 bytes at a time in rows 2t + {0, 1, 8, 9}, in an
+// order that depends on t's parity: all of them fill all banks.
+template <int D> __device__ __forceinline__ int d8_chunk(int r, int c) {
+  return D == 64 ? r * 64 + ((c ^ ((r >> 1) & 3)) << 4) : r * 128 + ((c ^ (r & 7)) << 4);
 }
-template <int D> __device__ __forceinline__ int v_chunk(int r, int c) {
-  return D == 64 ? r * 64 + ((c ^ (((r >> 2) & 1) << 1)) << 4) : r * 128 + ((c ^ (r & 6)) << 4);
-}
+// a sum that starts at this int32 is, read as fp32, 1.5 * 2^23 + the sum (up to 2^22)
+constexpr int kIntBase = 0x4b400000;
+constexpr float kFloatBase = 12582912.f;
 
 template <typename T, int D, int NT, int LIMBS, int WARPS, int STAGES>
-__global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Params p) {
+__global__ void __launch_bounds__(WARPS * 32, 1)
+    decode_int8_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const D8Params p) {
   constexpr int KS = D / 16;          // k-steps of the scores, and m-tiles of O
   constexpr int kHeads = 8 * NT;      // query heads of a warp
   constexpr int kSlot = kHeads * (D + 2);  // floats of a partial: O, then (m, l)
   constexpr int kStage = d8_stage<D>();
   constexpr int kRing = STAGES * kStage;
   static_assert(kRing >= kSlot * 4, "a warp's ring holds its last partial");
-  extern __shared__ __align__(128) uint8_t d8_smem[];
+  extern __shared__ uint8_t d8_raw[];
+  uint8_t* d8_smem = d8_raw + ((1024u - (smem_u32(d8_raw) & 1023u)) & 1023u);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   const int B = p.n_seqs;
@@ -135,9 +137,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
   float* heads_part = reinterpret_cast<float*>(d8_smem + WARPS * kRing);  // [WARPS][kSlot]
   int* prefix = reinterpret_cast<int*>(heads_part + WARPS * kSlot);       // [B + 1] tiles before each sequence
   int* ctxs = prefix + B + 1;                                             // [B]
+  __shared__ __align__(8) uint64_t full[WARPS][STAGES];  // a stage's copies are in
   __shared__ int wsum[WARPS];
   __shared__ int slot_seq[2 * WARPS];  // sequence of each team's partials (-1: none)
 
+  if (lane == 0) {  // the warp's own barriers
+    for (int i = 0; i < STAGES; ++i) mbar_init(&full[warp][i], 1);
+    fence_barrier_init();
+    if (warp == 0) {
+      prefetch_tensormap(&kmap);
+      prefetch_tensormap(&vmap);
+    }
+  }
   pdl_wait();  // the metadata, q and the pools may come from the kernel before this one
   pdl_trigger();  // (after the wait: the merge reads the lengths before its own)
 
@@ -188,20 +199,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
   if (r0 < r1) {
     // ---- the ring: tiles of the range in order, STAGES - 1 ahead
     const int n_tiles = r1 - r0;
-    const int64_t pitch = static_cast<int64_t>(p.n_kv_heads) * D;
-    const int64_t tile_bytes = 16 * pitch;
-    constexpr int cpr = D / 16, kCopies = 16 * cpr / 32;  // chunks of a row, copies of a lane for K (and V)
-    // this lane's chunk of a tile: row lane / cpr (+ 32 / cpr a copy), chunk lane % cpr
-    const int64_t lane_src = (lane / cpr) * pitch + (lane % cpr) * 16 + static_cast<int64_t>(kvh) * D;
-    const int8_t* k_src = p.k_pool + lane_src;
-    const int8_t* v_src = p.v_pool + lane_src;
-    const float* sc_src = (lane ? p.v_scale : p.k_scale) + kvh;
-    const uint32_t ring_a = smem_u32(ring);
-    uint32_t fill = ring_a;     // the stage the next copies go to
-    int ids = 0, ids_next = 0;  // lane l: first pool row / 16 of tile 32 b + l of the range
-    auto load_ids = [&](int b) {
+    int fill = 0;  // the stage the next copies go to
+    // lane l: pool row / 16 and scales of tile 32 b + l of the range
+    int ids = 0, ids_next = 0;
+    float ks_ids = 0.f, vs_ids = 0.f, ks_next = 0.f, vs_next = 0.f;
+    int batch = 0;                                 // of ids
+    const uint64_t policy = l2_evict_first_policy();  // every byte is read once
+    auto load_ids = [&](int b, int& row16, float& ks, float& vs) {
       const int i = b * 32 + lane;
-      int row16 = 0;
       if (i < n_tiles) {
         const int s = d8_find(prefix, B, r0 + i);
         const int tile = r0 + i - prefix[s];
@@ -212,92 +217,87 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
           id = 0;
         }
         row16 = id * p.tiles_per_block + (tile - jb * p.tiles_per_block);
+        ks = p.k_scale[static_cast<int64_t>(id) * p.n_kv_heads + kvh];
+        vs = p.v_scale[static_cast<int64_t>(id) * p.n_kv_heads + kvh];
       }
-      return row16;
     };
-    int to_issue = 0;
-    auto issue = [&]() {
-      if (to_issue < n_tiles) {
-        if ((to_issue & 31) == 0) {
-          ids = to_issue == 0 ? load_ids(0) : ids_next;
-          if (to_issue + 32 < n_tiles) ids_next = load_ids((to_issue >> 5) + 1);
+    load_ids(0, ids, ks_ids, vs_ids);
+    if (n_tiles > 32) load_ids(1, ids_next, ks_next, vs_next);
+    auto issue = [&](int i) {
+      if (i < n_tiles) {
+        // the copies run at most 31 tiles ahead, so i is in this batch or the next
+        const int row16 = __shfl_sync(0xffffffffu, (i >> 5) == batch ? ids : ids_next, i & 31);
+        if (elect_one()) {
+          uint8_t* st = ring + fill * kStage;
+          mbar_arrive_expect_tx(&full[warp][fill], kStage);
+          tma_load_3d_hint(st, &kmap, &full[warp][fill], 0, kvh, row16 * 16, policy);
+          tma_load_3d_hint(st + 16 * D, &vmap, &full[warp][fill], 0, kvh, row16 * 16, policy);
         }
-        const int row16 = __shfl_sync(0xffffffffu, ids, to_issue & 31);
-        const int64_t src = row16 * tile_bytes;
-#pragma unroll
-        for (int c = 0; c < kCopies; ++c) {
-          const int ch = c * 32 + lane;
-          cp_async16(fill + k_chunk<D>(ch / cpr, ch % cpr), k_src + src + c * (32 / cpr) * pitch);
-          cp_async16(fill + 16 * D + v_chunk<D>(ch / cpr, ch % cpr), v_src + src + c * (32 / cpr) * pitch);
-        }
-        if (lane < 2) {
-          const int id = p.tiles_per_block == 1 ? row16 : row16 / p.tiles_per_block;
-          cp_async4(fill + 32 * D + lane * 4, sc_src + static_cast<int64_t>(id) * p.n_kv_heads);
-        }
-        fill = fill + kStage == ring_a + kRing ? ring_a : fill + kStage;
-        ++to_issue;
+        __syncwarp();
+        fill = fill + 1 == STAGES ? 0 : fill + 1;
       }
-      cp_commit();
     };
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) issue();
+    for (int i = 0; i < STAGES - 1; ++i) issue(i);
 
     int s = d8_find(prefix, B, r0), pos = r0;
-    const uint8_t* st = ring;  // the stage of the tile at pos
+    int use = 0, i = 0;  // the stage of the tile at pos, its number in the range
+    uint32_t use_ph = 0;
+    bool dead = false;
     while (pos < r1) {
       const int seg_end = min(prefix[s + 1], r1);
       const int ctx = ctxs[s];
       const bool first = pos == r0;  // the range's first segment
-      // ---- Q^T fragments: column n = g is head head0 + 8 nt + g; k-step kk's
-      // indices 2t, 2t + 1, 2t + 8, 2t + 9 are dims d0 .. d0 + 3
-      uint32_t qb[NT][LIMBS][KS][2];
+      // ---- Q^T fragments: column n = g is head head0 + 8 nt + g; this lane's
+      // dims are those of its K chunks: 16 from 16t (D = 128: 32 from 32t), in
+      // words of four, of which k-step kk takes words 2 kk and 2 kk + 1
+      uint32_t qb[NT][3][D / 32][2];
       float c_head[NT][2];  // score factor of heads 2t, 2t + 1
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const bool on = 8 * nt + g < nh;
         const T* row = static_cast<const T*>(p.q) + static_cast<int64_t>(s) * p.q_stride +
-                       static_cast<int64_t>(head0 + 8 * nt + g) * D;
-        float f[KS][4];
+                       static_cast<int64_t>(head0 + 8 * nt + g) * D + t * (D / 4);
+        float f[D / 16][4];
         float amax = 0.f;
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) {
-          const int d0 = (kk >> 2) * 64 + 16 * t + 4 * (kk & 3);
+        for (int w = 0; w < D / 16; ++w) {
           if (on && p.q_vec) {
-            load4_f<T>(row + d0, f[kk]);
+            load4_f<T>(row + 4 * w, f[w]);
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f[kk][e] = on ? Elem<T>::to_f(row[d0 + e]) : 0.f;
+            for (int e = 0; e < 4; ++e) f[w][e] = on ? Elem<T>::to_f(row[4 * w + e]) : 0.f;
           }
-          if (!std::is_same<T, __half>::value) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(f[kk][e]));
-          }
+          for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(f[w][e]));
         }
-        float back = 1.f, inv = 1.f;
-        if (!std::is_same<T, __half>::value) {
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-          // 2^E with 2^E <= amax < 2^(E+1) (1 for zero, subnormal or not finite rows)
-          const uint32_t ex = __float_as_uint(amax) >> 23;
-          if (ex >= 2 && ex <= 252) {
-            back = __uint_as_float(ex << 23);
-            inv = __uint_as_float((254u - ex) << 23);
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        // the power of two that brings amax to [2^21, 2^22): sums of the top bytes
+        // then stay below 2^22 at any head_dim here.  Rows of zeros and tiny rows
+        // go by 2^-100; a row that is not finite gives NaN
+        const uint32_t ex = max(__float_as_uint(amax) >> 23, 27u);
+        const float inv = __uint_as_float((275u - min(ex, 254u)) << 23);
+        float back = __uint_as_float((min(ex, 254u) - 21u) << 23);
+        bool fine = amax < INFINITY;
+#pragma unroll
+        for (int w = 0; w < D / 16; ++w) {
+          int A[4], Bv[4], C[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            fine = fine && f[w][e] == f[w][e];
+            const int q = __float2int_rn(f[w][e] * inv);
+            A[e] = (q + 32768 + 128) >> 16;
+            const int rest = q - (A[e] << 16);
+            Bv[e] = (rest + 128) >> 8;
+            C[e] = rest - (Bv[e] << 8);
           }
+          qb[nt][0][w / 2][w & 1] = pack_s8(A[0], A[1], A[2], A[3]);
+          qb[nt][1][w / 2][w & 1] = pack_s8(Bv[0], Bv[1], Bv[2], Bv[3]);
+          qb[nt][2][w / 2][w & 1] = pack_s8(C[0], C[1], C[2], C[3]);
         }
-#pragma unroll
-        for (int kk = 0; kk < KS; ++kk) {
-          float v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = f[kk][e] * inv;
-          qb[nt][0][kk][0] = pack2<__half>(v[0], v[1]);
-          qb[nt][0][kk][1] = pack2<__half>(v[2], v[3]);
-          if constexpr (LIMBS == 2) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] -= __half2float(__float2half_rn(v[e]));
-            qb[nt][LIMBS - 1][kk][0] = pack2<__half>(v[0], v[1]);
-            qb[nt][LIMBS - 1][kk][1] = pack2<__half>(v[2], v[3]);
-          }
-        }
+        const unsigned bad = __ballot_sync(0xffffffffu, !fine);
+        if ((bad >> (4 * g)) & 15u) back = NAN;
         // lanes 4n .. hold head n's factor
         c_head[nt][0] = p.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * t);
         c_head[nt][1] = p.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * t + 4);
@@ -316,31 +316,52 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
       bool fresh = true;               // no tile of the segment yet
 
       int left = ctx - (pos - prefix[s]) * 16;  // tokens from this tile on
-      for (; pos < seg_end; ++pos, left -= 16) {
-        cp_wait<STAGES - 2>();
-        __syncwarp();  // every lane's copies of this tile are in, and every lane is done with the one before
-        issue();
-        const float ks = *reinterpret_cast<const float*>(st + 32 * D);
-        const float vs = *reinterpret_cast<const float*>(st + 32 * D + 4);
-        // ---- S^T = K Q^T
-        float sc[NT][4];
+      for (; pos < seg_end; ++pos, ++i, left -= 16) {
+        if (!dead && !mbar_wait(&full[warp][use], use_ph)) dead = true;
+        __syncwarp();  // every lane is done with the tile before, whose stage is filled again
+        issue(i + STAGES - 1);
+        if ((i >> 5) != batch) {  // (uniform) the next 32 tiles
+          batch = i >> 5;
+          ids = ids_next;
+          ks_ids = ks_next;
+          vs_ids = vs_next;
+          if ((batch + 1) * 32 < n_tiles) load_ids(batch + 1, ids_next, ks_next, vs_next);
+        }
+        const float ks = __shfl_sync(0xffffffffu, ks_ids, i & 31), vs = __shfl_sync(0xffffffffu, vs_ids, i & 31);
+        const uint8_t* st = ring + use * kStage;
+        // ---- S^T = K Q^T, one product for each byte of q
+        int si[NT][3][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int lb = 0; lb < 3; ++lb) si[nt][lb][0] = si[nt][lb][1] = si[nt][lb][2] = si[nt][lb][3] = kIntBase;
 #pragma unroll
         for (int half = 0; half < D / 64; ++half) {
-          const uint4 k0 = flip(*reinterpret_cast<const uint4*>(st + k_chunk<D>(g, half * 4 + t)));
-          const uint4 k1 = flip(*reinterpret_cast<const uint4*>(st + k_chunk<D>(g + 8, half * 4 + t)));
-          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+          const int c = D == 64 ? t : 2 * t + half;
+          const uint4 k0 = *reinterpret_cast<const uint4*>(st + d8_chunk<D>(g, c));
+          const uint4 k1 = *reinterpret_cast<const uint4*>(st + d8_chunk<D>(g + 8, c));
 #pragma unroll
-          for (int k4 = 0; k4 < 4; ++k4) {
-            const uint32_t a[4] = {i8_lo(w0[k4]), i8_lo(w1[k4]), i8_hi(w0[k4]), i8_hi(w1[k4])};
+          for (int k2 = 0; k2 < 2; ++k2) {
+            const uint32_t a[4] = {k2 ? k0.z : k0.x, k2 ? k1.z : k1.x, k2 ? k0.w : k0.y, k2 ? k1.w : k1.y};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int lb = 0; lb < LIMBS; ++lb)
-                mma16816<__half>(sc[nt], a, qb[nt][lb][half * 4 + k4][0], qb[nt][lb][half * 4 + k4][1]);
+              for (int lb = 0; lb < 3; ++lb)
+                mma16832_s8(si[nt][lb], a, qb[nt][lb][half * 2 + k2][0], qb[nt][lb][half * 2 + k2][1]);
           }
         }
+        float2 sc[NT][2];  // tokens g, g + 8
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float2 v[3];
+#pragma unroll
+            for (int lb = 0; lb < 3; ++lb)
+              v[lb] = __fadd2_rn(make_float2(__int_as_float(si[nt][lb][2 * r]), __int_as_float(si[nt][lb][2 * r + 1])),
+                                 make_float2(-kFloatBase, -kFloatBase));
+            sc[nt][r] = __ffma2_rn(v[0], make_float2(65536.f, 65536.f), __ffma2_rn(v[1], make_float2(256.f, 256.f), v[2]));
+          }
         // ---- x - mu of the lane's scores (tokens g, g + 8; heads 2t, 2t + 1)
         float2 x0[NT], x1[NT];
         float top = -INFINITY;
@@ -348,8 +369,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
         for (int nt = 0; nt < NT; ++nt) {
           const float2 f = __fmul2_rn(make_float2(c_head[nt][0], c_head[nt][1]), make_float2(ks, ks));
           const float2 nm = make_float2(-mu[nt][0], -mu[nt][1]);
-          x0[nt] = __ffma2_rn(make_float2(sc[nt][0], sc[nt][1]), f, nm);
-          x1[nt] = __ffma2_rn(make_float2(sc[nt][2], sc[nt][3]), f, nm);
+          x0[nt] = __ffma2_rn(sc[nt][0], f, nm);
+          x1[nt] = __ffma2_rn(sc[nt][1], f, nm);
         }
         if (left < 16) {  // a sequence's last tile
           const float2 none = make_float2(-INFINITY, -INFINITY);
@@ -427,7 +448,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int row = 2 * t + (k >> 1) * 8 + ((k & 1) ^ sw);
-            r[k] = *reinterpret_cast<const uint2*>(st + 16 * D + v_chunk<D>(row, half * 4 + (g >> 1)) + (g & 1) * 8);
+            r[k] = *reinterpret_cast<const uint2*>(st + 16 * D + d8_chunk<D>(row, half * 4 + (g >> 1)) + (g & 1) * 8);
             r[k].x ^= 0x80808080u;
             r[k].y ^= 0x80808080u;
           }
@@ -444,7 +465,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
                 mma16816<__half>(o[nt][half * 4 + mt], a, pb[nt][lb][0], pb[nt][lb][1]);
           }
         }
-        st = st + kStage == ring + kRing ? ring : st + kStage;
+        if (++use == STAGES) {
+          use = 0;
+          use_ph ^= 1;
+        }
       }
 
       // ---- segment end
@@ -476,10 +500,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
         // the range's first partial goes to its own slot, a later (last) one
         // into the ring, which no copy in flight uses any more
         float* slot = first ? heads_part + warp * kSlot : reinterpret_cast<float*>(ring);
-        if (!first) {
-          cp_wait<0>();
-          __syncwarp();
-        }
+        if (!first) __syncwarp();  // every lane is done with the last tile
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -502,7 +523,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_int8_kernel(const D8Para
       ++s;
       while (s < B && prefix[s + 1] == prefix[s]) ++s;  // empty sequences
     }
-    cp_wait<0>();
+    if (dead && lane == 0) raise_flag(p.err, PKV_FLAG_PIPELINE_TIMEOUT);
   }
   __syncthreads();
 
@@ -681,10 +702,10 @@ __global__ void __launch_bounds__(kM8Threads) merge_int8_kernel(const D8Params p
 }
 
 template <typename T, int D, int NT, int WARPS, int STAGES>
-cudaError_t launch_d8(const AttnArgs& a, void* workspace, cudaStream_t stream) {
+cudaError_t launch_d8(const AttnArgs& a, const CUtensorMap* kmap, const CUtensorMap* vmap, void* workspace, cudaStream_t stream) {
   constexpr int LIMBS = std::is_same<T, float>::value ? 2 : 1;
   auto kern = decode_int8_kernel<T, D, NT, LIMBS, WARPS, STAGES>;
-  constexpr int kFixed = WARPS * (STAGES * d8_stage<D>() + 8 * NT * (D + 2) * 4);
+  constexpr int kFixed = 1024 + WARPS * (STAGES * d8_stage<D>() + 8 * NT * (D + 2) * 4);
   constexpr int kMost = kFixed + (2 * kD8MaxSeqs + 1) * 4;
   static_assert(kMost + 1024 <= 232448, "the rings and partials fit the 227 KB of shared memory");
   static std::atomic<int> sm_count[64];  // per device, 0: not asked
@@ -741,7 +762,7 @@ cudaError_t launch_d8(const AttnArgs& a, void* workspace, cudaStream_t stream) {
     cfg.gridDim = dim3(gx, gy);
     cfg.blockDim = dim3(WARPS * 32);
     cfg.dynamicSmemBytes = kFixed + (2 * p.n_seqs + 1) * 4;
-    e = cudaLaunchKernelEx(&cfg, kern, p);
+    e = cudaLaunchKernelEx(&cfg, kern, *kmap, *vmap, p);
     if (e != cudaSuccess) return e;
     const int splits = std::max(1, std::min(p.n_q_heads, 296 / p.n_seqs));
     const int heads_per = (p.n_q_heads + splits - 1) / splits;
@@ -755,33 +776,30 @@ cudaError_t launch_d8(const AttnArgs& a, void* workspace, cudaStream_t stream) {
 }
 
 template <typename T>
-cudaError_t launch_d8_t(const AttnArgs& a, void* ws, cudaStream_t stream) {
-  // query heads per warp: 8, or 16 where the group has more (the K and V
-  // fragments are then converted once for both halves)
+cudaError_t launch_d8_t(const AttnArgs& a, const CUtensorMap* km, const CUtensorMap* vm, void* ws, cudaStream_t stream) {
+  // query heads per warp: 8, or 16 where the group has more (V's fragments are
+  // then converted once for both halves)
   const bool two = a.n_q_heads / a.n_kv_heads > 8;
   constexpr bool f32 = std::is_same<T, float>::value;
   if (a.head_dim == 64)
-    return two ? launch_d8<T, 64, 2, f32 ? 8 : 16, f32 ? 6 : 3>(a, ws, stream)
-               : launch_d8<T, 64, 1, 16, 5>(a, ws, stream);
-  return two ? launch_d8<T, 128, 2, 8, 4>(a, ws, stream)
-             : launch_d8<T, 128, 1, f32 ? 8 : 16, f32 ? 4 : 2>(a, ws, stream);
+    return two ? launch_d8<T, 64, 2, 8, 6>(a, km, vm, ws, stream)
+               : launch_d8<T, 64, 1, 16, 5>(a, km, vm, ws, stream);
+  return two ? launch_d8<T, 128, 2, 8, 4>(a, km, vm, ws, stream)
+             : launch_d8<T, 128, 1, f32 ? 8 : 16, f32 ? 4 : 2>(a, km, vm, ws, stream);
 }
 
 }  // namespace
-
-bool decode_int8_supported(const AttnArgs& a) {
-  return (a.head_dim == 64 || a.head_dim == 128) && a.block_size % 16 == 0;
-}
 
 size_t decode_int8_workspace_bytes(int n_q_heads, int head_dim) {
   return static_cast<size_t>(2) * kD8MaxCtas * n_q_heads * (head_dim + 2) * 4;
 }
 
-cudaError_t launch_decode_int8(const AttnArgs& a, void* workspace, cudaStream_t stream) {
+cudaError_t launch_decode_int8(const AttnArgs& a, const CUtensorMap* kmap, const CUtensorMap* vmap,
+                               void* workspace, cudaStream_t stream) {
   if (a.n_seqs == 0) return cudaSuccess;
-  if (a.dtype == PKV_DTYPE_F16) return launch_d8_t<__half>(a, workspace, stream);
-  if (a.dtype == PKV_DTYPE_BF16) return launch_d8_t<__nv_bfloat16>(a, workspace, stream);
-  return launch_d8_t<float>(a, workspace, stream);
+  if (a.dtype == PKV_DTYPE_F16) return launch_d8_t<__half>(a, kmap, vmap, workspace, stream);
+  if (a.dtype == PKV_DTYPE_BF16) return launch_d8_t<__nv_bfloat16>(a, kmap, vmap, workspace, stream);
+  return launch_d8_t<float>(a, kmap, vmap, workspace, stream);
 }
 
 }  // namespace pkv

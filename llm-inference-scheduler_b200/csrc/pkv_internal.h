@@ -12,6 +12,8 @@ namespace pkv {
 // pool format code (internal; not an ABI dtype) of fp8 e4m3 pools, for
 // encode_pool_tensormap / pool_tensormap
 constexpr int kPoolFp8 = 100;
+// ... and of int8 pools (16-row boxes whatever the block size)
+constexpr int kPoolInt8 = 101;
 
 struct RopeArgs {
   void* q_out;
@@ -227,9 +229,9 @@ struct Int8LayArgs {
 };
 cudaError_t launch_lay_out_int8(const Int8LayArgs& a, int dtype, cudaStream_t stream);
 // AttnArgs with k_scale / v_scale per (block, KV head); decode form
-bool decode_int8_supported(const AttnArgs& a);
 size_t decode_int8_workspace_bytes(int n_q_heads, int head_dim);
-cudaError_t launch_decode_int8(const AttnArgs& a, void* workspace, cudaStream_t stream);
+cudaError_t launch_decode_int8(const AttnArgs& a, const CUtensorMap* kmap, const CUtensorMap* vmap,
+                               void* workspace, cudaStream_t stream);
 
 // ---- causal attention over consecutive rows (pkv_packed.cu)
 struct PackedArgs {
