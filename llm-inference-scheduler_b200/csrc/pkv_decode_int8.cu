@@ -528,19 +528,21 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   __syncthreads();
 
   // ---- join the teams' partials: runs of slots of one sequence, in order
-  __shared__ int n_runs, run_lo[2 * WARPS], run_n[2 * WARPS], slots[2 * WARPS];
-  if (tid == 0) {
-    int r = 0, k = 0;
-    for (int a = 0; a < 2 * p.teams; ++a) {
-      if (slot_seq[a] < 0) continue;
-      if (k == 0 || slot_seq[a] != slot_seq[slots[k - 1]]) {
-        run_lo[r] = k;
-        run_n[r++] = 0;
-      }
-      slots[k++] = a;
-      ++run_n[r - 1];
+  static_assert(2 * WARPS <= 32, "a lane for each slot");
+  __shared__ int n_runs;
+  __shared__ unsigned run_mask[2 * WARPS];  // the slots of each run
+  if (warp == 0) {
+    const int v = lane < 2 * p.teams ? slot_seq[lane] : -1;
+    const unsigned used = __ballot_sync(0xffffffffu, v >= 0);
+    const unsigned below = used & ((1u << lane) - 1u);
+    const int before = __shfl_sync(0xffffffffu, v, below ? 31 - __clz(below) : 0);
+    const unsigned starts = __ballot_sync(0xffffffffu, v >= 0 && (below == 0 || before != v));
+    if ((starts >> lane) & 1) {
+      const unsigned later = starts & ~((2u << lane) - 1u);  // starts of later runs (lane 31: 2 << 31 is 0)
+      const unsigned upto = later ? (1u << (__ffs(later) - 1)) - 1u : 0xffffffffu;
+      run_mask[__popc(starts & ((1u << lane) - 1u))] = used & upto & ~((1u << lane) - 1u);
     }
-    n_runs = r;
+    if (lane == 0) n_runs = __popc(starts);
   }
   __syncthreads();
   constexpr int kVec = D / 4;
@@ -553,19 +555,19 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     if (head >= (kv + 1) * p.group) continue;
     float mm = 0.f, ll = 0.f;
     float4 oo = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int lo = run_lo[r], n = run_n[r];
-    for (int k = 0; k < n; ++k) {
-      const int a = slots[lo + k], wp = (a >> 1) * p.per_cta + w;
+    unsigned todo = run_mask[r];
+    const int s = slot_seq[__ffs(todo) - 1];
+    for (bool one = true; todo; todo &= todo - 1, one = false) {
+      const int a = __ffs(todo) - 1, wp = (a >> 1) * p.per_cta + w;
       const float* sl = (a & 1) ? reinterpret_cast<const float*>(d8_smem + wp * kRing) : heads_part + wp * kSlot;
       const float2 ml = *reinterpret_cast<const float2*>(sl + kHeads * D + 2 * hh);
       const float4 x = *reinterpret_cast<const float4*>(sl + hh * D + 4 * v);
-      const float mn = k ? fmaxf(mm, ml.x) : ml.x;
+      const float mn = one ? ml.x : fmaxf(mm, ml.x);
       const float fa = ex2_approx(mm - mn), fb = ex2_approx(ml.x - mn) * ml.y;
       mm = mn;
       ll = ll * fa + fb;
       oo = make_float4(oo.x * fa + x.x * fb, oo.y * fa + x.y * fb, oo.z * fa + x.z * fb, oo.w * fa + x.w * fb);
     }
-    const int s = slot_seq[slots[lo]];
     const float inv = 1.f / ll;
     oo = make_float4(oo.x * inv, oo.y * inv, oo.z * inv, oo.w * inv);
     if (prefix[s] >= c0 && prefix[s + 1] <= c1) {  // all of it in this CTA
