@@ -240,7 +240,13 @@ __global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedAr
 template <typename T, int D>
 cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
   constexpr int smem = (3 * 64 * (D + 4) + 64 * 68) * 4;
-  cudaError_t e = cudaFuncSetAttribute(packed_cores_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<bool> ready[64];  // per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !ready[dev].load())) {
+    e = cudaFuncSetAttribute(packed_cores_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && dev < 64) ready[dev].store(true);
+  }
   if (e != cudaSuccess) return e;
   const int64_t tiles = a.n_tokens / kPkM + static_cast<int64_t>(a.n_seqs);
   cudaLaunchConfig_t cfg = {};

@@ -25,6 +25,8 @@
 // What bounds it: the launch and three dependent round trips (lengths, the free
 // list or table entry, the store) for decode steps; the 16 bytes a token of
 // slots and positions for prompts.
+#include <atomic>
+
 #include "pkv_common.cuh"
 #include "pkv_internal.h"
 
@@ -204,16 +206,20 @@ __global__ void __launch_bounds__(kStThreads) step_tables_kernel(const StepTable
 }  // namespace
 
 cudaError_t launch_step_tables(StepTablesArgs a, cudaStream_t stream) {
-  int dev = 0, sms = 0;
+  static std::atomic<int> sm_count[64];  // per device, 0: not asked
+  int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return e;
-  const size_t smem = 2 * (static_cast<size_t>(a.n_seqs) + 1) * sizeof(unsigned);
-  if (smem > 48 * 1024) {
-    e = cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(2 * (kStepTablesMaxSeqs + 1) * sizeof(unsigned)));
+  int sms = dev < 64 ? sm_count[dev].load() : 0;
+  if (sms == 0) {
+    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(2 * (kStepTablesMaxSeqs + 1) * sizeof(unsigned)));
     if (e != cudaSuccess) return e;
+    if (dev < 64) sm_count[dev].store(sms);
   }
+  const size_t smem = 2 * (static_cast<size_t>(a.n_seqs) + 1) * sizeof(unsigned);
   a.vec_ok = ((reinterpret_cast<uintptr_t>(a.slot_mapping) | reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0;
   const int64_t want = (static_cast<int64_t>(a.n_tokens) + kStThreads * kStTok - 1) / (kStThreads * kStTok);
   const int grid = static_cast<int>(want < 1 ? 1 : want > sms ? sms : want);

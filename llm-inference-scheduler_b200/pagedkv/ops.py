@@ -47,9 +47,10 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 def _row_stride(t: torch.Tensor, name: str) -> int:
     """Token-row stride of a [T, H, D] tensor whose inner [H, D] is dense."""
-    if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
+    st, sh = t.stride(), t.shape
+    if len(sh) != 3 or st[2] != 1 or st[1] != sh[2]:
         raise ValueError(f"pagedkv: `{name}` must be [tokens, heads, head_dim] with dense heads")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return st[0] if sh[0] > 1 else sh[1] * sh[2]
 
 
 def new_error_flags(device) -> torch.Tensor:
@@ -1002,24 +1003,33 @@ def bind_paged_decode_attention_fp8(q, k_pool, v_pool, k_scale, v_scale, block_t
 
 # ---------------------------------------------------------------- step tables on the GPU
 
-def _call(name: str, t: torch.Tensor, *args) -> None:
-    """One C call on t's device and its current stream (the last argument)."""
-    fn = getattr(_lib.load(), name)
-    dev = t.get_device()
-    if dev == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(t))
+_fns: dict = {}  # C functions by name
+
+
+def _call(name: str, dev: int, *args) -> None:
+    """One C call on device dev and its current stream (the last argument)."""
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(_lib.load(), name)
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, _raw_stream(t))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         _lib.check(rc, name)
 
 
-def _same_device(t: torch.Tensor, **others) -> None:
-    """Every tensor on t's CUDA device (None entries are skipped)."""
-    for name, o in others.items():
-        if o is not None and _cuda(o, name).device != t.device:
-            raise ValueError(f"pagedkv: `{name}` is on {o.device}, expected {t.device}")
+def _one_device(names: str, *tensors) -> int:
+    """The CUDA device index that all tensors are on (None entries aside);
+    `names` says what they are, in order, for the error."""
+    dev = tensors[0].get_device() if isinstance(tensors[0], torch.Tensor) else -1
+    for t in tensors:
+        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != dev or dev < 0):
+            for n, o in zip(names.split(), tensors):
+                if o is not None and _cuda(o, n).get_device() != dev:
+                    raise ValueError(f"pagedkv: `{n}` is on {o.device}, expected cuda:{dev}")
+    return dev
 
 
 def _check_err(err: torch.Tensor | None) -> None:
@@ -1073,9 +1083,9 @@ def build_step_tables(block_tables: torch.Tensor, free_blocks: torch.Tensor, n_f
     A request the free list is too short for sets PKV_FLAG_OUT_OF_BLOCKS in
     err; it and those after it get slots -1 and context length 0 and take no
     block.  Reference: scheduler.py:79-156 and block_manager.py:121-131 (host)."""
+    dev = _one_device("block_tables free_blocks n_free num_prior num_new err", block_tables, free_blocks,
+                      n_free, num_prior, num_new, err)
     _check_tables(block_tables)
-    _same_device(block_tables, free_blocks=free_blocks, n_free=n_free, num_prior=num_prior,
-                 num_new=num_new, err=err)
     _check_err(err)
     B = num_prior.shape[0]
     _int_row(num_prior, "num_prior", B), _int_row(num_new, "num_new", B)
@@ -1085,7 +1095,8 @@ def build_step_tables(block_tables: torch.Tensor, free_blocks: torch.Tensor, n_f
     if out is None:
         out = new_step_tables(B, n_tokens, block_tables.device)
     else:
-        _same_device(block_tables, **out._asdict())
+        _one_device("block_tables context_lens query_start_loc slot_mapping positions out.n_free", block_tables,
+                    *out)
         _int_row(out.context_lens, "context_lens", B)
         _int_row(out.query_start_loc, "query_start_loc", B + 1)
         _int_row(out.slot_mapping, "slot_mapping", n_tokens, torch.int64)
@@ -1093,7 +1104,7 @@ def build_step_tables(block_tables: torch.Tensor, free_blocks: torch.Tensor, n_f
         _int_row(out.n_free, "out.n_free", 1)
         if out.n_free.data_ptr() == n_free.data_ptr():
             raise ValueError("pagedkv: the new free count needs a tensor of its own")
-    _call("pkv_build_step_tables", block_tables, block_tables.data_ptr(), block_tables.stride(0),
+    _call("pkv_build_step_tables", dev, block_tables.data_ptr(), block_tables.stride(0),
           block_tables.shape[1], free_blocks.data_ptr(), free_blocks.shape[0], n_free.data_ptr(),
           out.n_free.data_ptr(), num_prior.data_ptr(), num_new.data_ptr(), B, int(block_size),
           out.context_lens.data_ptr(), out.query_start_loc.data_ptr(), out.slot_mapping.data_ptr(),
@@ -1103,21 +1114,21 @@ def build_step_tables(block_tables: torch.Tensor, free_blocks: torch.Tensor, n_f
 
 # ---------------------------------------------------------------- int8 pools, a scale per (block, KV head)
 
-def _check_int8_pools(k_pool, v_pool, k_scale, v_scale, **others):
-    """Shapes, types and devices of int8 pools and their scales; returns
-    (num_blocks, block_size, n_kv_heads, head_dim)."""
-    _cuda(k_pool, "k_pool")
-    _same_device(k_pool, v_pool=v_pool, k_scale=k_scale, v_scale=v_scale, **others)
+def _check_int8_pools(k_pool, v_pool, k_scale, v_scale):
+    """Shapes and types of int8 pools and their scales; returns (num_blocks,
+    block_size, n_kv_heads, head_dim)."""
     if k_pool.dtype != torch.int8 or v_pool.dtype != torch.int8:
         raise TypeError("pagedkv: int8 pools are int8 tensors")
     if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
         raise TypeError("pagedkv: int8 pool scales are float32")
-    if not all(t.is_contiguous() for t in (k_pool, v_pool, k_scale, v_scale)):
+    if not (k_pool.is_contiguous() and v_pool.is_contiguous() and k_scale.is_contiguous() and
+            v_scale.is_contiguous()):
         raise ValueError("pagedkv: pools and scales must be contiguous")
-    if k_pool.dim() != 4 or k_pool.shape != v_pool.shape:
+    shape = k_pool.shape
+    if len(shape) != 4 or shape != v_pool.shape:
         raise ValueError("pagedkv: pools must be [num_blocks, block_size, n_kv_heads, head_dim]")
-    nb, bs, hkv, d = k_pool.shape
-    if tuple(k_scale.shape) != (nb, hkv) or tuple(v_scale.shape) != (nb, hkv):
+    nb, bs, hkv, d = shape
+    if k_scale.shape != (nb, hkv) or v_scale.shape != (nb, hkv):
         raise ValueError("pagedkv: int8 pool scales must be [num_blocks, n_kv_heads]")
     return nb, bs, hkv, d
 
@@ -1147,20 +1158,20 @@ def reshape_and_cache_int8(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tenso
     block's rows of the head, byte = round(x / scale).  A block that goes on
     keeps its rows, requantised when the new ones need a larger scale.
     Reference: block_manager.py:121-131 (unquantised)."""
-    nb, bs, hkv, d = _check_int8_pools(k_pool, v_pool, k_scale, v_scale, k=k, v=v, err=err,
-                                       block_tables=block_tables, context_lens=context_lens,
-                                       query_start_loc=query_start_loc)
+    dev = _one_device("k v k_pool v_pool k_scale v_scale block_tables context_lens query_start_loc err", k, v,
+                      k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, query_start_loc, err)
+    nb, bs, hkv, d = _check_int8_pools(k_pool, v_pool, k_scale, v_scale)
     _check_err(err)
     n_seqs = _check_rows_of(block_tables, context_lens, query_start_loc, "query_start_loc")
     if k.dtype != v.dtype:
         raise TypeError("pagedkv: k and v must share one dtype")
     T = k.shape[0]
-    if tuple(k.shape[1:]) != (hkv, d) or k.shape != v.shape:
+    if k.shape != (T, hkv, d) or k.shape != v.shape:
         raise ValueError("pagedkv: k / v must be [tokens, n_kv_heads, head_dim] as the pools")
     code = dtype_code(k.dtype)
     if T == 0 or n_seqs == 0:
         return
-    _call("pkv_reshape_and_cache_int8", k, k.data_ptr(), v.data_ptr(), _row_stride(k, "k"),
+    _call("pkv_reshape_and_cache_int8", dev, k.data_ptr(), v.data_ptr(), _row_stride(k, "k"),
           _row_stride(v, "v"), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
           v_scale.data_ptr(), nb, block_tables.data_ptr(), block_tables.stride(0),
           block_tables.shape[1], context_lens.data_ptr(), query_start_loc.data_ptr(), n_seqs, T, hkv,
@@ -1175,9 +1186,9 @@ def fetch_int8(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor
     values of `dtype`: (K, V), each [n_rows, Hkv, D], one sequence behind the
     other (rows past row_start_loc[-1] are left as allocated).  Reference: the
     gather of append_and_fetch, block_manager.py:136-141."""
-    nb, bs, hkv, d = _check_int8_pools(k_pool, v_pool, k_scale, v_scale, err=err,
-                                       block_tables=block_tables, context_lens=context_lens,
-                                       row_start_loc=row_start_loc)
+    dev = _one_device("k_pool v_pool k_scale v_scale block_tables context_lens row_start_loc err", k_pool, v_pool,
+                      k_scale, v_scale, block_tables, context_lens, row_start_loc, err)
+    nb, bs, hkv, d = _check_int8_pools(k_pool, v_pool, k_scale, v_scale)
     _check_err(err)
     n_seqs = _check_rows_of(block_tables, context_lens, row_start_loc, "row_start_loc")
     code = dtype_code(dtype)
@@ -1185,7 +1196,7 @@ def fetch_int8(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor
     v = torch.empty((n_rows, hkv, d), dtype=dtype, device=k_pool.device)
     if n_rows == 0 or n_seqs == 0:
         return k, v
-    _call("pkv_fetch_int8", k, k.data_ptr(), v.data_ptr(), hkv * d, hkv * d, k_pool.data_ptr(),
+    _call("pkv_fetch_int8", dev, k.data_ptr(), v.data_ptr(), hkv * d, hkv * d, k_pool.data_ptr(),
           v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), nb, block_tables.data_ptr(),
           block_tables.stride(0), block_tables.shape[1], context_lens.data_ptr(),
           row_start_loc.data_ptr(), n_seqs, int(n_rows), hkv, d, bs, code, _ptr(err))
@@ -1222,9 +1233,9 @@ def paged_decode_attention_int8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: t
     context of length 0 gives a zero row.  workspace: a byte buffer of
     decode_int8_workspace_bytes (any contents; allocated here when None).
     Reference: block_manager.py:136-141 + qwen2.py:98-128 (num_new == 1)."""
-    nb, bs, hkv, d = _check_int8_pools(k_pool, v_pool, k_scale, v_scale, q=q, err=err, out=out,
-                                       block_tables=block_tables, context_lens=context_lens,
-                                       workspace=workspace)
+    dev = _one_device("q k_pool v_pool k_scale v_scale block_tables context_lens workspace out err", q, k_pool,
+                      v_pool, k_scale, v_scale, block_tables, context_lens, workspace, out, err)
+    nb, bs, hkv, d = _check_int8_pools(k_pool, v_pool, k_scale, v_scale)
     _check_tables(block_tables), _check_err(err)
     B, hq, dq = q.shape
     _int_row(context_lens, "context_lens", B)
@@ -1236,7 +1247,7 @@ def paged_decode_attention_int8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: t
         return out
     if workspace is None:
         workspace = torch.empty(decode_int8_workspace_bytes(hq, d), dtype=torch.uint8, device=q.device)
-    _call("pkv_paged_decode_attention_int8", q, out.data_ptr(), _row_stride(out, "out"), q.data_ptr(),
+    _call("pkv_paged_decode_attention_int8", dev, out.data_ptr(), _row_stride(out, "out"), q.data_ptr(),
           _row_stride(q, "q"), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
           v_scale.data_ptr(), nb, block_tables.data_ptr(), block_tables.stride(0),
           block_tables.shape[1], context_lens.data_ptr(), B, hq, hkv, d, bs, float(scale), code,
@@ -1262,9 +1273,10 @@ def paged_prefill_attention_int8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: 
     (prefill_int8_scratch_bytes; allocated here when None), which the packed
     attention kernel then reads.  max_query_len is taken as the other prefill
     calls take it; this path does not need it."""
-    nb, bs, hkv, d = _check_int8_pools(k_pool, v_pool, k_scale, v_scale, q=q, err=err, out=out,
-                                       block_tables=block_tables, query_start_loc=query_start_loc,
-                                       num_prior=num_prior, scratch=scratch)
+    dev = _one_device("q k_pool v_pool k_scale v_scale block_tables query_start_loc num_prior scratch out err", q,
+                      k_pool, v_pool, k_scale, v_scale, block_tables, query_start_loc, num_prior, scratch, out,
+                      err)
+    nb, bs, hkv, d = _check_int8_pools(k_pool, v_pool, k_scale, v_scale)
     _check_err(err)
     n_seqs = _check_rows_of(block_tables, num_prior, query_start_loc, "query_start_loc")
     T, hq, dq = q.shape
@@ -1276,7 +1288,7 @@ def paged_prefill_attention_int8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: 
     if scratch is None:
         scratch = torch.empty(prefill_int8_scratch_bytes(n_seqs, block_tables.shape[1], hkv, d, bs, q.dtype),
                               dtype=torch.uint8, device=q.device)
-    _call("pkv_paged_prefill_attention_int8", q, out.data_ptr(), _row_stride(out, "out"), q.data_ptr(),
+    _call("pkv_paged_prefill_attention_int8", dev, out.data_ptr(), _row_stride(out, "out"), q.data_ptr(),
           _row_stride(q, "q"), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
           v_scale.data_ptr(), nb, block_tables.data_ptr(), block_tables.stride(0),
           block_tables.shape[1], query_start_loc.data_ptr(), num_prior.data_ptr(), n_seqs, T, hq, hkv,
@@ -1297,8 +1309,7 @@ def packed_prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     sequence.  q [T, Hq, D], k, v [T, Hkv, D] (views of a fused projection will
     do), D 64 or 128; query_start_loc int32 [n_seqs + 1].  Rows past the last
     sequence are left as they are.  Reference: qwen2.py:98-128."""
-    _cuda(q, "q")
-    _same_device(q, k=k, v=v, query_start_loc=query_start_loc, out=out, err=err)
+    dev = _one_device("q k v query_start_loc out err", q, k, v, query_start_loc, out, err)
     _check_err(err)
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError("pagedkv: q, k and v must share one dtype")
@@ -1312,7 +1323,7 @@ def packed_prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     out = _like_q(out, q)
     if T == 0 or n_seqs == 0:
         return out
-    _call("pkv_packed_prompt_attention", q, out.data_ptr(), _row_stride(out, "out"), q.data_ptr(),
+    _call("pkv_packed_prompt_attention", dev, out.data_ptr(), _row_stride(out, "out"), q.data_ptr(),
           _row_stride(q, "q"), k.data_ptr(), _row_stride(k, "k"), v.data_ptr(), _row_stride(v, "v"),
           query_start_loc.data_ptr(), n_seqs, T, hq, hkv, d, float(scale), code, _ptr(err))
     return out
