@@ -91,14 +91,22 @@ __device__ __forceinline__ bool find_tile(const PackedArgs& a, int64_t u, int m_
   return tile >= 0 && static_cast<int64_t>(tile) * m_rows < n;
 }
 
+__device__ __forceinline__ void pk_copy16(void* dst, const void* src, bool on) {  // zeros where not on
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+
+// A thread takes 4 rows x 4 keys of S (keys tx + 16 c) and 4 rows x 4 (or 2 x 4)
+// dims of O, two products an instruction (the paired fp32 FMA): 8 16-byte reads
+// of shared memory for 32 of them, in both.  fp32 rows on 16-byte boundaries come
+// by cp.async, a key tile ahead; other rows element by element.
 template <typename T, int D>
-__global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedArgs a) {
-  extern __shared__ float pk_smem[];
+__global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedArgs a, int wide) {
+  extern __shared__ __align__(16) float pk_smem[];
   constexpr int kLd = D + 4;                // row pitch of the Q, K and V tiles (16-byte rows, spread banks)
+  constexpr int kTile = 64 * kLd;
   float* qs = pk_smem;                      // [64][kLd]
-  float* ks = qs + kPkM * kLd;              // [64][kLd]
-  float* vs = ks + kPkN * kLd;              // [64][kLd]
-  float* ps = vs + kPkN * kLd;              // [64][68] probabilities
+  float* kvs = qs + kTile;                  // [2 buffers][K, V][64][kLd]
+  float* ps = kvs + 4 * kTile;              // [64][68] probabilities
   constexpr int kLp = kPkN + 4;
   pdl_trigger();
   pdl_wait();
@@ -115,6 +123,12 @@ __global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedAr
   auto load_tile = [&](float* dst, const T* src, int64_t stride, int n) {
     for (int c = tid; c < 64 * (D / 4); c += kPkThreads) {
       const int r = c / (D / 4), d = (c - r * (D / 4)) * 4;
+      if constexpr (sizeof(T) == 4) {
+        if (wide) {
+          pk_copy16(dst + r * kLd + d, src + (r < n ? r * stride + d : 0), r < n);
+          continue;
+        }
+      }
       float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < n) {
         const T* p = src + r * stride + d;
@@ -123,32 +137,41 @@ __global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedAr
       *reinterpret_cast<float4*>(dst + r * kLd + d) = f;
     }
   };
+  auto load_kv = [&](int k0) {
+    float* buf = kvs + ((k0 / kPkN) & 1) * 2 * kTile;
+    const int n = min(kPkN, last - k0);
+    if (n > 0) {
+      load_tile(buf, static_cast<const T*>(a.k) + (span.row0 + k0) * a.k_stride + static_cast<int64_t>(g) * D, a.k_stride, n);
+      load_tile(buf + kTile, static_cast<const T*>(a.v) + (span.row0 + k0) * a.v_stride + static_cast<int64_t>(g) * D, a.v_stride, n);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
   load_tile(qs, static_cast<const T*>(a.q) + static_cast<int64_t>(q_begin + q0) * a.q_stride +
                     static_cast<int64_t>(h) * D, a.q_stride, rows);
-  // this thread: rows 4 ty .. 4 ty + 3; keys tx + 16 c; dims tx + 16 c
-  constexpr int kDim = D / 16;
-  float o[4][kDim], m[4], l[4];
+  load_kv(0);
+  constexpr int kDim = D / 16;  // dims of O per thread and row: 4 tx .. + 3 (D = 128: and 64 on)
+  float2 o[4][kDim / 2];
+  float m[4], l[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     m[r] = -INFINITY;
     l[r] = 0.f;
 #pragma unroll
-    for (int c = 0; c < kDim; ++c) o[r][c] = 0.f;
+    for (int c = 0; c < kDim / 2; ++c) o[r][c] = make_float2(0.f, 0.f);
   }
   const float sl2 = a.scale * 1.4426950408889634f;
   for (int k0 = 0; k0 < last; k0 += kPkN) {
+    load_kv(k0 + kPkN);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncthreads();
+    const float* ks = kvs + ((k0 / kPkN) & 1) * 2 * kTile;
+    const float* vs = ks + kTile;
     const int n = min(kPkN, last - k0);
-    load_tile(ks, static_cast<const T*>(a.k) + (span.row0 + k0) * a.k_stride + static_cast<int64_t>(g) * D,
-              a.k_stride, n);
-    load_tile(vs, static_cast<const T*>(a.v) + (span.row0 + k0) * a.v_stride + static_cast<int64_t>(g) * D,
-              a.v_stride, n);
-    __syncthreads();
-    float x[4][4];
+    float2 x2[4][4];
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) x[r][c] = 0.f;
+      for (int c = 0; c < 4; ++c) x2[r][c] = make_float2(0.f, 0.f);
 #pragma unroll 4
     for (int d = 0; d < D; d += 4) {
       float4 qa[4], kb[4];
@@ -160,20 +183,18 @@ __global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedAr
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          x[r][c] = fmaf(qa[r].x, kb[c].x, x[r][c]);
-          x[r][c] = fmaf(qa[r].y, kb[c].y, x[r][c]);
-          x[r][c] = fmaf(qa[r].z, kb[c].z, x[r][c]);
-          x[r][c] = fmaf(qa[r].w, kb[c].w, x[r][c]);
+          x2[r][c] = __ffma2_rn(make_float2(qa[r].x, qa[r].y), make_float2(kb[c].x, kb[c].y), x2[r][c]);
+          x2[r][c] = __ffma2_rn(make_float2(qa[r].z, qa[r].w), make_float2(kb[c].z, kb[c].w), x2[r][c]);
         }
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int lim = span.prior + q0 + 4 * ty + r + 1 - k0;  // keys of this tile the row sees
-      float mx = -INFINITY;
+      float mx = -INFINITY, x[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        x[r][c] = tx + 16 * c < min(lim, n) ? x[r][c] * sl2 : -INFINITY;
-        mx = fmaxf(mx, x[r][c]);
+        x[c] = tx + 16 * c < min(lim, n) ? (x2[r][c].x + x2[r][c].y) * sl2 : -INFINITY;
+        mx = fmaxf(mx, x[c]);
       }
 #pragma unroll
       for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
@@ -183,43 +204,54 @@ __global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedAr
       float sum = 0.f;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const float p = exp2f(x[r][c] - base);
+        const float p = exp2f(x[c] - base);
         sum += p;
         ps[(4 * ty + r) * kLp + tx + 16 * c] = p;
       }
-#pragma unroll
-      for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
       m[r] = mn;
-      l[r] = l[r] * f + sum;
+      l[r] = l[r] * f + sum;  // this thread's keys; joined at the end
 #pragma unroll
-      for (int c = 0; c < kDim; ++c) o[r][c] *= f;
+      for (int c = 0; c < kDim / 2; ++c) o[r][c] = __fmul2_rn(o[r][c], make_float2(f, f));
     }
     __syncwarp();  // a warp's two row groups write and read only their own rows of ps
-#pragma unroll 4
-    for (int j = 0; j < kPkN; ++j) {
-      float pv[4];
+#pragma unroll 2
+    for (int j = 0; j < kPkN; j += 4) {
+      float4 pv[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) pv[r] = ps[(4 * ty + r) * kLp + j];
+      for (int r = 0; r < 4; ++r) pv[r] = *reinterpret_cast<const float4*>(ps + (4 * ty + r) * kLp + j);
 #pragma unroll
-      for (int c = 0; c < kDim; ++c) {
-        const float v = vs[j * kLd + tx + 16 * c];
+      for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r][c] = fmaf(pv[r], v, o[r][c]);
-      }
+        for (int c = 0; c < kDim / 4; ++c) {
+          const float4 v = *reinterpret_cast<const float4*>(vs + (j + jj) * kLd + 64 * c + 4 * tx);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float p = jj == 0 ? pv[r].x : jj == 1 ? pv[r].y : jj == 2 ? pv[r].z : pv[r].w;
+            o[r][2 * c] = __ffma2_rn(make_float2(p, p), make_float2(v.x, v.y), o[r][2 * c]);
+            o[r][2 * c + 1] = __ffma2_rn(make_float2(p, p), make_float2(v.z, v.w), o[r][2 * c + 1]);
+          }
+        }
     }
+    __syncthreads();  // the buffer is filled again next
   }
   bool fine[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int row = 4 * ty + r;
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
     const float inv = 1.f / l[r];
     bool ok = true;
     T* out = static_cast<T*>(a.out) + static_cast<int64_t>(q_begin + q0 + row) * a.out_stride +
              static_cast<int64_t>(h) * D;
 #pragma unroll
-    for (int c = 0; c < kDim; ++c) {
-      ok = ok && fabsf(o[r][c] * inv) < INFINITY;
-      if (row < rows) out[tx + 16 * c] = Elem<T>::from_f(o[r][c] * inv);
+    for (int c = 0; c < kDim / 4; ++c) {
+      const float v[4] = {o[r][2 * c].x * inv, o[r][2 * c].y * inv, o[r][2 * c + 1].x * inv, o[r][2 * c + 1].y * inv};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ok = ok && fabsf(v[i]) < INFINITY;
+        if (row < rows) out[64 * c + 4 * tx + i] = Elem<T>::from_f(v[i]);
+      }
     }
     fine[r] = ok || row >= rows;
   }
@@ -239,7 +271,7 @@ __global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedAr
 
 template <typename T, int D>
 cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
-  constexpr int smem = (3 * 64 * (D + 4) + 64 * 68) * 4;
+  constexpr int smem = (5 * 64 * (D + 4) + 64 * 68) * 4;
   static std::atomic<bool> ready[64];  // per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -259,7 +291,10 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, packed_cores_kernel<T, D>, a);
+  const int es = sizeof(T);
+  const int wide = es == 4 && ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                                static_cast<uintptr_t>((a.q_stride | a.k_stride | a.v_stride) * es)) & 15) == 0;
+  return cudaLaunchKernelEx(&cfg, packed_cores_kernel<T, D>, a, wide);
 }
 
 
