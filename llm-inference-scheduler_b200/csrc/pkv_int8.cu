@@ -21,8 +21,8 @@
 // head, K or V), so one warp owns a scale and the rows under it and nothing is
 // atomic.  The host does not know how many blocks each sequence touches, but
 // floor(n / b) + 2 bounds it, so sequence i's units start at
-// floor(start_i / b) + 2 i and a warp finds its sequence by binary search on
-// the start positions: no prefix pass, no scratch.  Bound by the bytes of the
+// floor(start_i / b) + 2 i and a warp finds its sequence by a search on the
+// start positions: no prefix pass, no scratch.  Bound by the bytes of the
 // rows for prompts, by launch and round trips for decode steps.
 #include <type_traits>
 
@@ -34,6 +34,7 @@ namespace pkv {
 namespace {
 
 constexpr int kI8Warps = 4;
+constexpr int kI8Regs = 8;  // 16-byte loads a lane keeps
 
 // the block scale for rows of largest finite magnitude amax
 __device__ __forceinline__ float int8_block_scale(float amax) {
@@ -79,18 +80,45 @@ __device__ __forceinline__ void bytes_to_f(uint32_t w, float* v) {
   for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
 }
 
+// 16 bytes as floats
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4& w, float* v) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(u[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = __uint_as_float(u[i] << 16), v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      }
+    }
+  }
+}
+
 // the sequence and touched-block number of unit u (see the header comment)
 struct Unit {
   int s, j;        // sequence, number of the touched block
   int row0, n;     // first packed row of the sequence, rows of the sequence
   int ctx;         // tokens of the sequence after the call
 };
+// (whole warp) the last sequence whose units start at or before u: 32 positions a
+// round, so two dependent loads for up to 1,024 sequences where halving takes ten
 __device__ __forceinline__ bool find_unit(const int32_t* start_loc, const int32_t* context_lens,
                                           int n_seqs, int n_rows, int bs, int64_t u, Unit& w) {
-  int lo = 0, hi = n_seqs - 1;
-  while (lo < hi) {
-    const int m = (lo + hi + 1) >> 1;
-    if (start_loc[m] / bs + 2 * static_cast<int64_t>(m) <= u) lo = m; else hi = m - 1;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = n_seqs;  // the answer is in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 31) / 32, m = lo + lane * step;
+    const bool before = lane * step < n && start_loc[m] / bs + 2 * static_cast<int64_t>(m) <= u;
+    const unsigned hits = __ballot_sync(0xffffffffu, before) | 1u;  // (lane 0: a bad first start goes to sequence lo)
+    const int k = 31 - __clz(hits);
+    n = min(step, n - k * step);
+    lo += k * step;
   }
   w.s = lo;
   w.row0 = start_loc[lo];
@@ -152,15 +180,41 @@ __global__ void __launch_bounds__(kI8Warps * 32) append_int8_kernel(const Int8Ro
 
   // units of four consecutive elements: cpr to a row
   const int cpr = D / 4, total = (end - held) * cpr;
+  // new rows that one load of 16 bytes a lane, at most kI8Regs times, can bring:
+  // they stay in registers between absmax and rounding (every block of 16 or 32
+  // rows here but fp32 ones of 128 dims); others are read twice
+  constexpr int kPer = 16 / sizeof(T), kLog = sizeof(T) == 2 ? 3 : 2;
+  const int chunks = total * 4 / kPer, row_log = (D == 64 ? 6 : 7) - kLog;  // 2^row_log chunks to a row
+  const bool once = (isv ? a.v_vec16 : a.k_vec16) && chunks <= 32 * kI8Regs;
+  uint4 raw[kI8Regs];
   float amax = 0.f;
-  for (int c = lane; c < total; c += 32) {
-    const int r = c / cpr, d = (c - r * cpr) * 4;
-    float v[4];
-    load4_any<T>(src + r * stride + d, vec, v);
+  auto take = [&](const float* v, int n) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < n; ++i) {
       const float m = fabsf(v[i]);
       amax = fmaxf(amax, m < INFINITY ? m : 0.f);
+    }
+  };
+  if (once) {
+#pragma unroll
+    for (int i = 0; i < kI8Regs; ++i) {
+      const int c = i * 32 + lane;
+      raw[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (c < chunks)
+        raw[i] = *reinterpret_cast<const uint4*>(src + (c >> row_log) * stride + ((c & ((1 << row_log) - 1)) << kLog));
+    }
+#pragma unroll
+    for (int i = 0; i < kI8Regs; ++i) {
+      float v[kPer];
+      unpack16<T>(raw[i], v);
+      take(v, kPer);
+    }
+  } else {
+    for (int c = lane; c < total; c += 32) {
+      const int r = c / cpr, d = (c - r * cpr) * 4;
+      float v[4];
+      load4_any<T>(src + r * stride + d, vec, v);
+      take(v, 4);
     }
   }
 #pragma unroll
@@ -182,12 +236,30 @@ __global__ void __launch_bounds__(kI8Warps * 32) append_int8_kernel(const Int8Ro
     }
   }
   const float inv = 1.f / sc;  // exact: a power of two
-  for (int c = lane; c < total; c += 32) {
-    const int r = c / cpr, d = (c - r * cpr) * 4;
-    float v[4];
-    load4_any<T>(src + r * stride + d, vec, v);
-    *reinterpret_cast<uint32_t*>(dst + (held + r) * pitch + d) =
-        pack_bytes(int8_round(v[0], inv), int8_round(v[1], inv), int8_round(v[2], inv), int8_round(v[3], inv));
+  auto four = [&](const float* v) {
+    return pack_bytes(int8_round(v[0], inv), int8_round(v[1], inv), int8_round(v[2], inv), int8_round(v[3], inv));
+  };
+  if (once) {
+#pragma unroll
+    for (int i = 0; i < kI8Regs; ++i) {
+      const int c = i * 32 + lane;
+      if (c >= chunks) continue;
+      float v[kPer];
+      unpack16<T>(raw[i], v);
+      int8_t* to = dst + (held + (c >> row_log)) * pitch + ((c & ((1 << row_log) - 1)) << kLog);
+      if constexpr (kPer == 8) {
+        *reinterpret_cast<uint2*>(to) = make_uint2(four(v), four(v + 4));
+      } else {
+        *reinterpret_cast<uint32_t*>(to) = four(v);
+      }
+    }
+  } else {
+    for (int c = lane; c < total; c += 32) {
+      const int r = c / cpr, d = (c - r * cpr) * 4;
+      float v[4];
+      load4_any<T>(src + r * stride + d, vec, v);
+      *reinterpret_cast<uint32_t*>(dst + (held + r) * pitch + d) = four(v);
+    }
   }
   __syncwarp();
   if (lane == 0) *scale = sc;
@@ -240,6 +312,30 @@ __global__ void __launch_bounds__(kI8Warps * 32) fetch_int8_kernel(const Int8Row
   const int8_t* src = static_cast<const int8_t*>(isv ? a.v_pool : a.k_pool) +
                       (static_cast<int64_t>(id) * bs * a.n_kv_heads + h) * D + r0 * pitch;
   const float sc = (isv ? a.v_scale : a.k_scale)[static_cast<int64_t>(id) * a.n_kv_heads + h];
+  if (isv ? a.v_vec16 : a.k_vec16) {  // 16 elements a lane
+    const int row_log = D == 64 ? 2 : 3, total = (r1 - r0) << row_log;
+#pragma unroll 4
+    for (int c = lane; c < total; c += 32) {
+      const int r = c >> row_log, d = (c & ((1 << row_log) - 1)) * 16;
+      const uint4 w = *reinterpret_cast<const uint4*>(src + r * pitch + d);
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+      T* to = dst + r * stride + d;
+#pragma unroll
+      for (int k = 0; k < 4; k += 16 / (4 * static_cast<int>(sizeof(T)))) {
+        float v[8];
+        bytes_to_f(u[k], v);
+        if constexpr (sizeof(T) == 2) bytes_to_f(u[k + 1], v + 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= sc;
+        if constexpr (sizeof(T) == 2) {
+          reinterpret_cast<uint4*>(to)[k / 2] = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+        } else {
+          reinterpret_cast<float4*>(to)[k] = make_float4(v[0], v[1], v[2], v[3]);
+        }
+      }
+    }
+    return;
+  }
   const int cpr = D / 4, total = (r1 - r0) * cpr;
   for (int c = lane; c < total; c += 32) {
     const int r = c / cpr, d = (c - r * cpr) * 4;
@@ -333,15 +429,17 @@ cudaError_t launch_rows(K f16, K bf16, K f32, Int8RowsArgs a, cudaStream_t strea
   return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
-// may four consecutive elements of these rows be one access?
-bool rows_vec(const void* p, int64_t stride, int esize) {
-  return ((reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride * esize)) & (4 * esize - 1)) == 0;
+// may `bytes` of these rows, from a multiple of that, be one access?
+bool rows_vec(const void* p, int64_t stride, int esize, int bytes) {
+  return ((reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride * esize)) & (bytes - 1)) == 0;
 }
 
 void fill_rows(Int8RowsArgs& a) {
   const int es = a.dtype == PKV_DTYPE_F32 ? 4 : 2;
-  a.k_vec = rows_vec(a.k, a.k_stride, es);
-  a.v_vec = rows_vec(a.v, a.v_stride, es);
+  a.k_vec = rows_vec(a.k, a.k_stride, es, 4 * es);
+  a.v_vec = rows_vec(a.v, a.v_stride, es, 4 * es);
+  a.k_vec16 = rows_vec(a.k, a.k_stride, es, 16);
+  a.v_vec16 = rows_vec(a.v, a.v_stride, es, 16);
   a.n_units = a.n_rows / a.block_size + 2 * static_cast<int64_t>(a.n_seqs);
 }
 

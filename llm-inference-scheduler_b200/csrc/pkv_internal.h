@@ -206,7 +206,7 @@ struct Int8RowsArgs {
   const int32_t* start_loc;  // [n_seqs + 1]: the last start_loc[i + 1] - start_loc[i] rows of context i
   int n_seqs, n_rows, num_blocks, block_size, n_kv_heads, head_dim, dtype;
   int* err;
-  int k_vec, v_vec;  // set by the launcher
+  int k_vec, v_vec, k_vec16, v_vec16;  // set by the launcher: accesses of 4 elements, of 16 bytes
   int64_t n_units;
 };
 cudaError_t launch_append_int8(Int8RowsArgs a, cudaStream_t stream);

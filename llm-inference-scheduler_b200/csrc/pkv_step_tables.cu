@@ -47,6 +47,7 @@ __global__ void __launch_bounds__(kStThreads) step_tables_kernel(const StepTable
   const int B = a.n_seqs, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned* start = st_smem;         // [B + 1] first token of each request
   unsigned* first = start + B + 1;   // [B + 1] first new block of each request
+  int* prior = reinterpret_cast<int*>(first + B + 1);  // [B] cached tokens, -1: lengths not valid
   __shared__ unsigned wsum[2][kStThreads / 32];
   __shared__ unsigned s_taken;
   const int64_t room = static_cast<int64_t>(a.max_blocks) * a.block_size;
@@ -56,24 +57,22 @@ __global__ void __launch_bounds__(kStThreads) step_tables_kernel(const StepTable
     if (blockIdx.x == 0 && tid == 0) raise_flag(a.err, PKV_FLAG_BLOCK_OUT_OF_RANGE);
     n_free = n_free < 0 ? 0 : a.free_capacity;
   }
-  // the tokens and new blocks of request i (none if its lengths are not valid)
-  auto lengths = [&](int i, int& p, int& n) {
-    p = __ldg(a.num_prior + i);
-    n = __ldg(a.num_new + i);
-    const bool ok = p >= 0 && n >= 0 && static_cast<int64_t>(p) + n <= room;
-    if (!ok) p = n = 0;
-    return ok;
-  };
   auto blocks_of = [&](int n) { return static_cast<unsigned>((static_cast<int64_t>(n) + bs - 1) / bs); };
 
+  // lengths once from memory: the tokens (start) and new blocks (first) of each
+  // request, none if its lengths are not valid, then their prefixes
   const int per = (B + kStThreads - 1) / kStThreads;
   const int lo = min(B, tid * per), hi = min(B, lo + per);
   unsigned tn = 0, tb = 0;
   for (int i = lo; i < hi; ++i) {
-    int p, n;
-    lengths(i, p, n);
-    tn = sat_add(tn, n);
-    tb = sat_add(tb, blocks_of(p + n) - blocks_of(p));
+    const int p = __ldg(a.num_prior + i), n = __ldg(a.num_new + i);
+    const bool ok = p >= 0 && n >= 0 && static_cast<int64_t>(p) + n <= room;
+    const unsigned blocks = ok ? blocks_of(p + n) - blocks_of(p) : 0u;
+    prior[i] = ok ? p : -1;
+    start[i] = ok ? n : 0;
+    first[i] = blocks;
+    tn = sat_add(tn, start[i]);
+    tb = sat_add(tb, blocks);
   }
   unsigned xn = tn, xb = tb;
 #pragma unroll
@@ -92,12 +91,11 @@ __global__ void __launch_bounds__(kStThreads) step_tables_kernel(const StepTable
   const unsigned en = __shfl_up_sync(0xffffffffu, xn, 1), eb = __shfl_up_sync(0xffffffffu, xb, 1);
   unsigned rn = lane ? sat_add(bn, en) : bn, rb = lane ? sat_add(bb, eb) : bb;
   for (int i = lo; i < hi; ++i) {
-    int p, n;
-    lengths(i, p, n);
+    const unsigned n = start[i], blocks = first[i];
     start[i] = rn;
     first[i] = rb;
     rn = sat_add(rn, n);
-    rb = sat_add(rb, blocks_of(p + n) - blocks_of(p));
+    rb = sat_add(rb, blocks);
   }
   if (hi == B && lo < B) { start[B] = rn; first[B] = rb; }
   if (B == 0 && tid == 0) start[0] = first[0] = 0;
@@ -111,10 +109,9 @@ __global__ void __launch_bounds__(kStThreads) step_tables_kernel(const StepTable
 
   // ---- the requests' outputs, dealt over the grid
   for (int i = blockIdx.x * kStThreads + tid; i < B; i += gridDim.x * kStThreads) {
-    int p, n;
-    const bool ok = lengths(i, p, n);
+    const bool ok = prior[i] >= 0;
     const bool srv = ok && served(i);
-    a.context_lens[i] = srv ? p + n : 0;
+    a.context_lens[i] = srv ? prior[i] + static_cast<int>(start[i + 1] - start[i]) : 0;
     a.query_start_loc[i] = static_cast<int>(start[i]);
     if (!ok) {
       const int rp = a.num_prior[i], rn2 = a.num_new[i];
@@ -152,7 +149,7 @@ __global__ void __launch_bounds__(kStThreads) step_tables_kernel(const StepTable
       }
       s = l;
     }
-    int p = 0, n = 0, have = 0, cur = -1, col = -1, blk = 0;
+    int p = 0, have = 0, cur = -1, col = -1, blk = 0;
     bool srv = false;
 #pragma unroll
     for (int k = 0; k < kStTok; ++k) {
@@ -163,7 +160,7 @@ __global__ void __launch_bounds__(kStThreads) step_tables_kernel(const StepTable
       while (start[s + 1] <= static_cast<unsigned>(t)) ++s;  // empty requests are passed over
       if (s != cur) {
         cur = s;
-        lengths(s, p, n);
+        p = prior[s];
         have = static_cast<int>(blocks_of(p));
         srv = served(s);
         col = -1;
@@ -215,11 +212,11 @@ cudaError_t launch_step_tables(StepTablesArgs a, cudaStream_t stream) {
     e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(step_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               static_cast<int>(2 * (kStepTablesMaxSeqs + 1) * sizeof(unsigned)));
+                               static_cast<int>((3 * kStepTablesMaxSeqs + 2) * sizeof(unsigned)));
     if (e != cudaSuccess) return e;
     if (dev < 64) sm_count[dev].store(sms);
   }
-  const size_t smem = 2 * (static_cast<size_t>(a.n_seqs) + 1) * sizeof(unsigned);
+  const size_t smem = (3 * static_cast<size_t>(a.n_seqs) + 2) * sizeof(unsigned);
   a.vec_ok = ((reinterpret_cast<uintptr_t>(a.slot_mapping) | reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0;
   const int64_t want = (static_cast<int64_t>(a.n_tokens) + kStThreads * kStTok - 1) / (kStThreads * kStTok);
   const int grid = static_cast<int>(want < 1 ? 1 : want > sms ? sms : want);

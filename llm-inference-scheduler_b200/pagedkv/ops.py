@@ -1058,11 +1058,10 @@ class StepTables(NamedTuple):
 def new_step_tables(n_seqs: int, n_tokens: int, device) -> StepTables:
     """Buffers of build_step_tables for up to n_seqs requests and n_tokens
     tokens, for a caller that fills the same ones every step (a captured one)."""
-    return StepTables(torch.empty(n_seqs, dtype=torch.int32, device=device),
-                      torch.empty(n_seqs + 1, dtype=torch.int32, device=device),
-                      torch.empty(n_tokens, dtype=torch.int64, device=device),
-                      torch.empty(n_tokens, dtype=torch.int64, device=device),
-                      torch.empty(1, dtype=torch.int32, device=device))
+    ctx, start, n_free = torch.empty(2 * n_seqs + 2, dtype=torch.int32, device=device).split(
+        (n_seqs, n_seqs + 1, 1))
+    return StepTables(ctx, start, torch.empty(n_tokens, dtype=torch.int64, device=device),
+                      torch.empty(n_tokens, dtype=torch.int64, device=device), n_free)
 
 
 def build_step_tables(block_tables: torch.Tensor, free_blocks: torch.Tensor, n_free: torch.Tensor,
