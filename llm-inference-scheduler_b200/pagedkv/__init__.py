@@ -7,5 +7,6 @@ torch-facing wrappers (`ops`) and the reference's operator surface
 """
 
 from .block_manager import BlockManager, OutOfBlocks, PagedKVCache, StepMetadata  # noqa: F401
+from .device_tables import DeviceStepTables  # noqa: F401
 
-__all__ = ["BlockManager", "OutOfBlocks", "PagedKVCache", "StepMetadata"]
+__all__ = ["BlockManager", "DeviceStepTables", "OutOfBlocks", "PagedKVCache", "StepMetadata"]

@@ -55,6 +55,10 @@ class BlockManager:
     reference): k_cache / v_cache hold the bytes (uint8) and k_scale_cache /
     v_scale_cache [L, NB, block_size, n_kv_heads] one fp32 scale per (slot,
     KV head) row; copy_block copies both.
+
+    dtype=torch.int8 keeps int8 pools with one power-of-two scale per (block,
+    KV head): k_scale_cache / v_scale_cache [L, NB, n_kv_heads], head_dim 64 or
+    128 and blocks of a multiple of 16 tokens (ops.reshape_and_cache_int8).
     """
 
     def __init__(self, num_blocks: int, block_size: int, num_layers: int, num_kv_heads: int,
@@ -66,6 +70,9 @@ class BlockManager:
         self.head_dim = head_dim
         self.dtype = dtype
         self.fp8 = dtype == torch.float8_e4m3fn
+        self.int8 = dtype == torch.int8
+        if self.int8 and (head_dim not in (64, 128) or block_size % 16):
+            raise ValueError("pagedkv: int8 pools need head_dim 64 or 128 and blocks of a multiple of 16 tokens")
         self.k_scale_cache = self.v_scale_cache = None
         self.k_scale = self.v_scale = None
         if device is None:
@@ -79,9 +86,9 @@ class BlockManager:
                     "pagedkv.BlockManager keeps its pools in GPU memory; pass a CUDA device "
                     "(or device=None for a bookkeeping-only manager)")
             shape = (num_layers, num_blocks, block_size, num_kv_heads, head_dim)
-            if self.fp8:
-                pool_dt = torch.uint8
-                sshape = shape[:-1]
+            if self.fp8 or self.int8:
+                pool_dt = torch.uint8 if self.fp8 else torch.int8
+                sshape = shape[:-1] if self.fp8 else (num_layers, num_blocks, num_kv_heads)
                 self.k_scale_cache = torch.zeros(sshape, device=self.device, dtype=torch.float32)
                 self.v_scale_cache = torch.zeros(sshape, device=self.device, dtype=torch.float32)
                 self.k_scale = [self.k_scale_cache[layer] for layer in range(num_layers)]
@@ -109,7 +116,7 @@ class BlockManager:
     @property
     def block_bytes(self) -> int:
         """Bytes of one block of one layer's K (or V) pool."""
-        esize = 1 if self.fp8 else torch.tensor([], dtype=self.dtype).element_size()
+        esize = 1 if self.fp8 or self.int8 else torch.tensor([], dtype=self.dtype).element_size()
         return self.block_size * self.num_kv_heads * self.head_dim * esize
 
     def allocate(self) -> int:
@@ -160,7 +167,7 @@ class BlockManager:
         host = torch.tensor(pairs, dtype=torch.int32).pin_memory()
         dev = host.to(self.device, non_blocking=True)
         ops.copy_blocks(self.k_cache, self.v_cache, dev, self.err)
-        if self.fp8:  # the rows' scales travel with their bytes
+        if self.fp8 or self.int8:  # the scales travel with their bytes
             ops.copy_blocks(self.k_scale_cache, self.v_scale_cache, dev, self.err)
         self.copies_launched += 1
 
@@ -278,6 +285,10 @@ class PagedKVCache:
         self._workspace: torch.Tensor | None = None
         self._schedule_buf: torch.Tensor | None = None
         self._fp8_scratch: torch.Tensor | None = None
+        self._int8_workspace: torch.Tensor | None = None
+        self._int8_scratch: torch.Tensor | None = None
+        self._counts: torch.Tensor | None = None  # int32 0, 1, 2, ..
+        self._slots_int8: torch.Tensor | None = None  # int64 0, 1, 2, ..
         self._mirror = _TableMirror()
         self._stage_ring: list = [[None, None] for _ in range(4)]
         self._stage_next = 0
@@ -330,6 +341,8 @@ class PagedKVCache:
         assert total <= len(table) * bs, (
             f"seq {seq_id}: {total} tokens but only {len(table)} blocks allocated")
         mgr.flush_copies()
+        if mgr.int8:
+            return self._append_and_fetch_int8(layer, seq_id, k_new, v_new, num_prior)
         if n_new:
             slots = torch.from_numpy(self._slots(table, num_prior, n_new)).to(mgr.device)
             if mgr.fp8:
@@ -349,6 +362,22 @@ class PagedKVCache:
             vs = mgr.v_scale[layer][idx].reshape(used * bs, -1, 1)[:total]
             k = (k.view(torch.float8_e4m3fn).float() * ks).to(k_new.dtype)
             v = (v.view(torch.float8_e4m3fn).float() * vs).to(v_new.dtype)
+        return k, v, num_prior
+
+    def _append_and_fetch_int8(self, layer, seq_id, k_new, v_new, num_prior):
+        """append_and_fetch over int8 pools: the values in k_new's dtype."""
+        mgr = self.mgr
+        total = num_prior + k_new.shape[0]
+        used = max(1, -(-total // mgr.block_size))
+        meta = torch.tensor((self.block_tables[seq_id][:used] or [0]) + [total, 0, k_new.shape[0], 0, total],
+                            dtype=torch.int32).to(mgr.device)
+        w = meta.shape[0] - 5
+        tab, ctx, new, whole = meta[:w].view(1, w), meta[w:w + 1], meta[w + 1:w + 3], meta[w + 3:]
+        pools = (mgr.k_pool[layer], mgr.v_pool[layer], mgr.k_scale[layer], mgr.v_scale[layer])
+        ops.reshape_and_cache_int8(k_new, v_new, *pools, tab, ctx, new, mgr.err)
+        if layer == mgr.num_layers - 1:
+            self._len[seq_id] = total
+        k, v = ops.fetch_int8(*pools, tab, ctx, whole, total, k_new.dtype, mgr.err)
         return k, v, num_prior
 
     # ---- batched hot path ---------------------------------------------------
@@ -548,6 +577,8 @@ class PagedKVCache:
             out = torch.empty((meta.n_tokens,) + tuple(q.shape[1:]), dtype=q.dtype, device=q.device)
         if mgr.fp8:
             return self._forward_layer_fp8(layer, q, k_new, v_new, meta, scale, out, advance)
+        if mgr.int8:
+            return self._forward_layer_int8(layer, q, k_new, v_new, meta, scale, out, advance)
         nd = meta.n_decode
         plan = meta.decode_plan
         if nd == meta.n_tokens and plan is not None and plan.scale == scale:
@@ -605,10 +636,10 @@ class PagedKVCache:
         if mgr._pending:
             mgr.flush_copies()
         nd = meta.n_decode
-        if defer_first and (meta.layers_plan is None or mgr.fp8):
+        if defer_first and (meta.layers_plan is None or mgr.fp8 or mgr.int8):
             raise ValueError("pagedkv: defer_first needs meta.layers_plan over this run's own "
                              "split-K sets (16-bit pools)")
-        if 0 < nd == meta.n_tokens:
+        if 0 < nd == meta.n_tokens and not mgr.int8:
             plan = meta.layers_plan
             kind = ops.DecodeAppendFp8LayersPlan if mgr.fp8 else ops.DecodeAppendLayersPlan
             if plan is None or plan.scale != scale or not isinstance(plan, kind):
@@ -676,6 +707,51 @@ class PagedKVCache:
             self._advance(meta)
         return out
 
+    def counts(self, n: int) -> torch.Tensor:
+        """int32 0, 1, .., n - 1 on the device (grown on demand)."""
+        if self._counts is None or self._counts.shape[0] < n:
+            self._counts = torch.arange(max(n, 1025), dtype=torch.int32, device=self.mgr.device)
+        return self._counts[:n]
+
+    def int8_buffers(self, n_prefill: int, width: int, n_q_heads: int, dtype: torch.dtype):
+        """The int8 pools' split-K workspace and prefill scratch (None without
+        prefill sequences), grown on demand and reused across layers and
+        steps (stream order keeps each use behind the previous)."""
+        mgr = self.mgr
+        need = ops.decode_int8_workspace_bytes(n_q_heads, mgr.head_dim)
+        if self._int8_workspace is None or self._int8_workspace.numel() < need:
+            self._int8_workspace = torch.empty(need, dtype=torch.uint8, device=mgr.device)
+        if not n_prefill:
+            return self._int8_workspace, None
+        need = ops.prefill_int8_scratch_bytes(n_prefill, width, mgr.num_kv_heads, mgr.head_dim,
+                                              mgr.block_size, dtype)
+        if self._int8_scratch is None or self._int8_scratch.numel() < need:
+            self._int8_scratch = torch.empty(need, dtype=torch.uint8, device=mgr.device)
+        return self._int8_workspace, self._int8_scratch
+
+    def _forward_layer_int8(self, layer, q, k_new, v_new, meta, scale, out, advance):
+        """forward_layer over int8 pools: the decode sequences' append and
+        attention, then the chunks' (each append quantises by block)."""
+        mgr = self.mgr
+        pools = (mgr.k_pool[layer], mgr.v_pool[layer], mgr.k_scale[layer], mgr.v_scale[layer])
+        nd = meta.n_decode
+        tabs, ctx = meta.block_tables, meta.context_lens
+        ws, scratch = self.int8_buffers(meta.n_seqs - nd, tabs.shape[1], q.shape[1], q.dtype)
+        if nd:
+            ops.reshape_and_cache_int8(k_new[:nd], v_new[:nd], *pools, tabs[:nd], ctx[:nd],
+                                       self.counts(nd + 1), mgr.err)
+            ops.paged_decode_attention_int8(q[:nd], *pools, tabs[:nd], ctx[:nd], scale, workspace=ws,
+                                            out=out[:nd], err=mgr.err)
+        if nd < meta.n_seqs:
+            ops.reshape_and_cache_int8(k_new[nd:], v_new[nd:], *pools, tabs[nd:], ctx[nd:],
+                                       meta.query_start_loc, mgr.err)
+            ops.paged_prefill_attention_int8(q[nd:], *pools, tabs[nd:], meta.query_start_loc,
+                                             meta.num_prior_dev[nd:], meta.max_query_len, scale,
+                                             out=out[nd:], err=mgr.err, scratch=scratch)
+        if advance and layer == mgr.num_layers - 1:
+            self._advance(meta)
+        return out
+
     def _attend_fp8(self, layer, q, meta, scale, out, advance):
         """The step's attention launches over fp8 pools whose rows are already
         appended: decode (with the step's schedule) and chunked prefill."""
@@ -710,6 +786,19 @@ class PagedKVCache:
         mgr = self.mgr
         if mgr._pending:
             mgr.flush_copies()
+        if mgr.int8:
+            # q and k rotated, k and v as plain rows (a pool of their own), for
+            # the append that quantises by block
+            T, bs = qkv.shape[0], mgr.block_size
+            rows = torch.empty((2, -(-T // bs), bs, mgr.num_kv_heads, mgr.head_dim), dtype=qkv.dtype,
+                               device=qkv.device)
+            if self._slots_int8 is None or self._slots_int8.shape[0] < T:
+                self._slots_int8 = torch.arange(max(T, 1024), dtype=torch.int64, device=qkv.device)
+            q = ops.rope_reshape_and_cache(qkv, positions, cos, sin, rows[0], rows[1], self._slots_int8[:T],
+                                           err=mgr.err)
+            k, v = rows.view(2, -1, mgr.num_kv_heads, mgr.head_dim)[:, :T]
+            return self._forward_layer_int8(layer, q, k, v, meta, scale,
+                                            torch.empty_like(q) if out is None else out, advance)
         rope = meta.rope_plan
         if rope is None or not rope.uses(positions, cos, sin):
             rope = meta.rope_plan = ops.RopePlan(positions, cos, sin, meta.slot_mapping, mgr.err)

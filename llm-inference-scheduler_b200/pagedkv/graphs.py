@@ -192,6 +192,14 @@ class StepGraphs:
             if kv._fp8_scratch is None or kv._fp8_scratch.numel() < need:
                 kv._fp8_scratch = torch.empty(need, dtype=torch.uint8, device=dev)
             self.scratch = kv._fp8_scratch
+        if mgr.int8:
+            # what the captured layers use of the cache's, held for the same reason
+            tokens = max(self._layout(R, P)["T"] for R, P in keys)
+            kv.counts(Rm + 1)
+            if kv._slots_int8 is None or kv._slots_int8.shape[0] < tokens:
+                kv._slots_int8 = torch.arange(tokens, dtype=torch.int64, device=dev)
+            self.int8_held = (kv.int8_buffers(self.prefill_seqs, self.W, cfg.num_attention_heads, m.dtype),
+                              kv._counts, kv._slots_int8)
         cos, sin = m.rope.tables(self.W * mgr.block_size)
         self.cos, self.sin = cos, sin  # held: an eager step that grows the tables drops them
 
@@ -221,10 +229,11 @@ class StepGraphs:
         meta = self._meta(R, P)
         v = self._views(R, P)
         pos = v["positions"]
-        meta.decode_schedule = ops.build_decode_schedule(
-            self.schedule, meta.block_tables[:R], meta.context_lens[:R], mgr.num_blocks,
-            cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, m.dtype,
-            fp8=mgr.fp8, err=mgr.err)
+        if not mgr.int8:  # (the int8 decode kernel splits the step itself)
+            meta.decode_schedule = ops.build_decode_schedule(
+                self.schedule, meta.block_tables[:R], meta.context_lens[:R], mgr.num_blocks,
+                cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim, m.dtype,
+                fp8=mgr.fp8, err=mgr.err)
         rot = None
         if not m.fused_rope:
             rot = (self.cos[pos].unsqueeze(1), self.sin[pos].unsqueeze(1))
@@ -439,7 +448,7 @@ class DecodeStepGraph:
     def __init__(self, kv_cache: PagedKVCache, host_qkv: torch.Tensor, host_out: torch.Tensor,
                  scale: float, chunks: tuple[int, ...] | None = None, max_blocks_per_seq: int = 64):
         mgr = kv_cache.mgr
-        if mgr.fp8 or mgr.device is None or mgr.device.type != "cuda":
+        if mgr.fp8 or mgr.int8 or mgr.device is None or mgr.device.type != "cuda":
             raise RuntimeError("pagedkv: DecodeStepGraph serves 16-bit pools on a CUDA device")
         L, R, width, D = host_qkv.shape
         hkv = mgr.num_kv_heads

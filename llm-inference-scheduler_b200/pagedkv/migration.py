@@ -66,6 +66,9 @@ class PeerPools:
     def __init__(self, mgr: BlockManager, mode: str = "pull"):
         if mode not in ("push", "pull"):
             raise ValueError("mode is 'push' (the source launches the copy) or 'pull'")
+        if mgr.int8:
+            # a block's scales are fewer bytes than the 16 that one peer access moves
+            raise ValueError("pagedkv: int8 pools do not migrate between ranks")
         if not dist.is_initialized():
             raise RuntimeError("PeerPools needs torch.distributed initialised (one process per GPU)")
         self.mgr = mgr

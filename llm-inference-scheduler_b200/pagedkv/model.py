@@ -27,6 +27,7 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
+from . import ops
 from .block_manager import PagedKVCache
 
 
@@ -228,3 +229,33 @@ class PagedQwen2Model:
             gu = torch.mm(x, lw["wgu"].t())
             h = torch.addmm(residual, F.silu(gu[:, :I]) * gu[:, I:], lw["wdown"].t())
         return h
+
+    @torch.inference_mode()
+    def forward_all_logits(self, input_ids: torch.Tensor, lengths: list[int]) -> torch.Tensor:
+        """Score whole prompts without a cache: input_ids [T] holds prompts of
+        `lengths` tokens one behind the other (on the device), the result is
+        the logits of every token [T, vocab].  The layers are forward()'s with
+        ops.packed_prompt_attention in place of the paged calls.  Reference:
+        Qwen2Model.forward's layer math (qwen2.py:143-176) over _attention
+        (qwen2.py:98-128), prompt by prompt."""
+        cfg = self.cfg
+        hq, hkv, d = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+        H, I, eps = cfg.hidden_size, cfg.intermediate_size, cfg.rms_norm_eps
+        T = int(input_ids.shape[0])
+        if any(n < 0 for n in lengths) or sum(lengths) != T:
+            raise ValueError(f"pagedkv: prompts of {sum(lengths)} tokens in {T} input ids")
+        starts = np.concatenate([[0], np.cumsum(lengths, dtype=np.int64)]).astype(np.int64)
+        pos_np = np.arange(T, dtype=np.int64) - np.repeat(starts[:-1], lengths)
+        both = torch.from_numpy(np.concatenate([starts, pos_np])).pin_memory().to(self.device, non_blocking=True)
+        start_loc, positions = both[: len(starts)].to(torch.int32), both[len(starts):]
+        cos_t, sin_t = self.rope.tables(max(lengths, default=0) + 1)
+        cos, sin = cos_t[positions].unsqueeze(1), sin_t[positions].unsqueeze(1)
+        h = self.embed[input_ids]
+        for lw in self.layers:
+            qkv = F.linear(F.rms_norm(h, (H,), lw["ln1"], eps), lw["wqkv"], lw["bqkv"]).view(T, hq + 2 * hkv, d)
+            qk = Rope.rotate(qkv[:, : hq + hkv], cos, sin)
+            attn = ops.packed_prompt_attention(qk[:, :hq], qk[:, hq:], qkv[:, hq + hkv:], start_loc, self.scale)
+            h = torch.addmm(h, attn.view(T, hq * d), lw["wo"].t())
+            gu = torch.mm(F.rms_norm(h, (H,), lw["ln2"], eps), lw["wgu"].t())
+            h = torch.addmm(h, F.silu(gu[:, :I]) * gu[:, I:], lw["wdown"].t())
+        return F.linear(F.rms_norm(h, (H,), self.final_norm, eps), self.embed)
