@@ -18,7 +18,8 @@
 // Infinities are stored as +-127 and do not enter absmax; NaN is stored as 0.
 //
 // Work split of the append and the fetch: one warp per (sequence, touched block,
-// head, K or V), so one warp owns a scale and the rows under it and nothing is
+// K or V, head or, where there are warps enough for the GPU without, several
+// heads in turn), so one warp owns a scale and the rows under it and nothing is
 // atomic.  The host does not know how many blocks each sequence touches, but
 // floor(n / b) + 2 bounds it, so sequence i's units start at
 // floor(start_i / b) + 2 i and a warp finds its sequence by a search on the
@@ -52,6 +53,15 @@ __device__ __forceinline__ uint32_t pack_bytes(int a, int b, int c, int d) {
   return (a & 255) | ((b & 255) << 8) | ((c & 255) << 16) | (static_cast<uint32_t>(d) << 24);
 }
 
+// four values of at most 127.5 in size as bytes, rounded to nearest even: the low
+// byte of 1.5 * 2^23 + x * inv (x * inv is exact, the sum rounds once)
+__device__ __forceinline__ uint32_t pack_scaled(const float* v, float2 inv) {
+  const float2 big = make_float2(12582912.f, 12582912.f);
+  const float2 a = __ffma2_rn(make_float2(v[0], v[1]), inv, big), b = __ffma2_rn(make_float2(v[2], v[3]), inv, big);
+  return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040),
+                     __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
+}
+
 // four consecutive elements; `vec` says whether they may be loaded as one word
 template <typename T>
 __device__ __forceinline__ void load4_any(const T* p, bool vec, float* v) {
@@ -75,9 +85,12 @@ __device__ __forceinline__ void store4_any(T* p, bool vec, const float* v) {
     for (int i = 0; i < 4; ++i) p[i] = Elem<T>::from_f(v[i]);
   }
 }
+// signed bytes as floats, exactly and without conversion instructions: x + 128 as
+// the low byte of 2^23 + 128 + x
 __device__ __forceinline__ void bytes_to_f(uint32_t w, float* v) {
+  w ^= 0x80808080u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
+  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540 + i)) - 8388736.f;
 }
 
 // 16 bytes as floats
@@ -134,11 +147,11 @@ __global__ void __launch_bounds__(kI8Warps * 32) append_int8_kernel(const Int8Ro
   pdl_wait();  // the metadata and the rows may come from the kernel before this one
   const int lane = threadIdx.x & 31;
   const int64_t wid = static_cast<int64_t>(blockIdx.x) * kI8Warps + (threadIdx.x >> 5);
-  const int per_unit = 2 * a.n_kv_heads;
+  const int per_half = (a.n_kv_heads + a.heads_per_warp - 1) / a.heads_per_warp, per_unit = 2 * per_half;
   const int64_t u = wid / per_unit;
   const int rem = static_cast<int>(wid - u * per_unit);
-  const bool isv = rem >= a.n_kv_heads;
-  const int h = isv ? rem - a.n_kv_heads : rem;
+  const bool isv = rem >= per_half;
+  const int h0 = (isv ? rem - per_half : rem) * a.heads_per_warp, h1 = min(a.n_kv_heads, h0 + a.heads_per_warp);
   const int bs = a.block_size, D = a.head_dim;
   if (u >= a.n_units) return;
   Unit w;
@@ -169,13 +182,13 @@ __global__ void __launch_bounds__(kI8Warps * 32) append_int8_kernel(const Int8Ro
   const int held = max(0, prior - static_cast<int>(blk0));                // rows the block keeps
   const int end = min(bs, static_cast<int>(w.ctx - blk0));                // rows after the call
   const int src0 = w.row0 + static_cast<int>(blk0) + held - prior;        // packed row of row `held`
-  const T* src = static_cast<const T*>(isv ? a.v : a.k) +
-                 static_cast<int64_t>(src0) * (isv ? a.v_stride : a.k_stride) + static_cast<int64_t>(h) * D;
   const int64_t stride = isv ? a.v_stride : a.k_stride;
   const bool vec = isv ? a.v_vec : a.k_vec;
+  const int64_t pitch = static_cast<int64_t>(a.n_kv_heads) * D;
+  for (int h = h0; h < h1; ++h) {
+  const T* src = static_cast<const T*>(isv ? a.v : a.k) + src0 * stride + static_cast<int64_t>(h) * D;
   int8_t* dst = static_cast<int8_t*>(isv ? a.v_pool : a.k_pool) +
                 (static_cast<int64_t>(id) * bs * a.n_kv_heads + h) * D;
-  const int64_t pitch = static_cast<int64_t>(a.n_kv_heads) * D;
   float* scale = (isv ? a.v_scale : a.k_scale) + static_cast<int64_t>(id) * a.n_kv_heads + h;
 
   // units of four consecutive elements: cpr to a row
@@ -185,16 +198,9 @@ __global__ void __launch_bounds__(kI8Warps * 32) append_int8_kernel(const Int8Ro
   // rows here but fp32 ones of 128 dims); others are read twice
   constexpr int kPer = 16 / sizeof(T), kLog = sizeof(T) == 2 ? 3 : 2;
   const int chunks = total * 4 / kPer, row_log = (D == 64 ? 6 : 7) - kLog;  // 2^row_log chunks to a row
-  const bool once = (isv ? a.v_vec16 : a.k_vec16) && chunks <= 32 * kI8Regs;
+  bool once = (isv ? a.v_vec16 : a.k_vec16) && chunks <= 32 * kI8Regs;
   uint4 raw[kI8Regs];
   float amax = 0.f;
-  auto take = [&](const float* v, int n) {
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-      const float m = fabsf(v[i]);
-      amax = fmaxf(amax, m < INFINITY ? m : 0.f);
-    }
-  };
   if (once) {
 #pragma unroll
     for (int i = 0; i < kI8Regs; ++i) {
@@ -203,18 +209,41 @@ __global__ void __launch_bounds__(kI8Warps * 32) append_int8_kernel(const Int8Ro
       if (c < chunks)
         raw[i] = *reinterpret_cast<const uint4*>(src + (c >> row_log) * stride + ((c & ((1 << row_log) - 1)) << kLog));
     }
+    // the largest magnitude as an integer: of the bit patterns without their
+    // signs (two 16-bit ones at a time), which order as the values do, with
+    // infinities and NaN above all
+    uint32_t top = 0u;
 #pragma unroll
     for (int i = 0; i < kI8Regs; ++i) {
-      float v[kPer];
-      unpack16<T>(raw[i], v);
-      take(v, kPer);
+      constexpr uint32_t kMask = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;
+      const uint32_t x = raw[i].x & kMask, y = raw[i].y & kMask, z = raw[i].z & kMask, w4 = raw[i].w & kMask;
+      if constexpr (sizeof(T) == 4) {
+        top = max(max(top, max(x, y)), max(z, w4));
+      } else {
+        top = __vimax3_u16x2(__vimax3_u16x2(top, x, y), z, w4);
+      }
     }
-  } else {
+    if constexpr (sizeof(T) == 4) {
+      amax = __uint_as_float(top);
+    } else {
+      const uint32_t m = max(top & 0xffffu, top >> 16);
+      if constexpr (std::is_same<T, __half>::value) amax = __half2float(__ushort_as_half(static_cast<unsigned short>(m)));
+      else amax = __uint_as_float(m << 16);
+    }
+    // rows with infinities or NaN take the other path
+    once = __all_sync(0xffffffffu, amax < INFINITY);
+  }
+  if (!once) {
+    amax = 0.f;
     for (int c = lane; c < total; c += 32) {
       const int r = c / cpr, d = (c - r * cpr) * 4;
       float v[4];
       load4_any<T>(src + r * stride + d, vec, v);
-      take(v, 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float m = fabsf(v[i]);
+        amax = fmaxf(amax, m < INFINITY ? m : 0.f);
+      }
     }
   }
 #pragma unroll
@@ -236,10 +265,8 @@ __global__ void __launch_bounds__(kI8Warps * 32) append_int8_kernel(const Int8Ro
     }
   }
   const float inv = 1.f / sc;  // exact: a power of two
-  auto four = [&](const float* v) {
-    return pack_bytes(int8_round(v[0], inv), int8_round(v[1], inv), int8_round(v[2], inv), int8_round(v[3], inv));
-  };
   if (once) {
+    const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
     for (int i = 0; i < kI8Regs; ++i) {
       const int c = i * 32 + lane;
@@ -248,9 +275,9 @@ __global__ void __launch_bounds__(kI8Warps * 32) append_int8_kernel(const Int8Ro
       unpack16<T>(raw[i], v);
       int8_t* to = dst + (held + (c >> row_log)) * pitch + ((c & ((1 << row_log) - 1)) << kLog);
       if constexpr (kPer == 8) {
-        *reinterpret_cast<uint2*>(to) = make_uint2(four(v), four(v + 4));
+        *reinterpret_cast<uint2*>(to) = make_uint2(pack_scaled(v, inv2), pack_scaled(v + 4, inv2));
       } else {
-        *reinterpret_cast<uint32_t*>(to) = four(v);
+        *reinterpret_cast<uint32_t*>(to) = pack_scaled(v, inv2);
       }
     }
   } else {
@@ -258,11 +285,13 @@ __global__ void __launch_bounds__(kI8Warps * 32) append_int8_kernel(const Int8Ro
       const int r = c / cpr, d = (c - r * cpr) * 4;
       float v[4];
       load4_any<T>(src + r * stride + d, vec, v);
-      *reinterpret_cast<uint32_t*>(dst + (held + r) * pitch + d) = four(v);
+      *reinterpret_cast<uint32_t*>(dst + (held + r) * pitch + d) =
+          pack_bytes(int8_round(v[0], inv), int8_round(v[1], inv), int8_round(v[2], inv), int8_round(v[3], inv));
     }
   }
   __syncwarp();
   if (lane == 0) *scale = sc;
+  }
 }
 
 template <typename T>
@@ -271,11 +300,11 @@ __global__ void __launch_bounds__(kI8Warps * 32) fetch_int8_kernel(const Int8Row
   pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t wid = static_cast<int64_t>(blockIdx.x) * kI8Warps + (threadIdx.x >> 5);
-  const int per_unit = 2 * a.n_kv_heads;
+  const int per_half = (a.n_kv_heads + a.heads_per_warp - 1) / a.heads_per_warp, per_unit = 2 * per_half;
   const int64_t u = wid / per_unit;
   const int rem = static_cast<int>(wid - u * per_unit);
-  const bool isv = rem >= a.n_kv_heads;
-  const int h = isv ? rem - a.n_kv_heads : rem;
+  const bool isv = rem >= per_half;
+  const int h0 = (isv ? rem - per_half : rem) * a.heads_per_warp, h1 = min(a.n_kv_heads, h0 + a.heads_per_warp);
   const int bs = a.block_size, D = a.head_dim;
   if (u >= a.n_units) return;
   Unit w;
@@ -306,44 +335,56 @@ __global__ void __launch_bounds__(kI8Warps * 32) fetch_int8_kernel(const Int8Row
   const int r1 = min(bs, static_cast<int>(w.ctx - blk0));
   const int64_t out0 = w.row0 + (blk0 + r0 - from);
   const int64_t stride = isv ? a.v_stride : a.k_stride;
-  T* dst = static_cast<T*>(const_cast<void*>(isv ? a.v : a.k)) + out0 * stride + static_cast<int64_t>(h) * D;
   const bool vec = isv ? a.v_vec : a.k_vec;
   const int64_t pitch = static_cast<int64_t>(a.n_kv_heads) * D;
-  const int8_t* src = static_cast<const int8_t*>(isv ? a.v_pool : a.k_pool) +
-                      (static_cast<int64_t>(id) * bs * a.n_kv_heads + h) * D + r0 * pitch;
-  const float sc = (isv ? a.v_scale : a.k_scale)[static_cast<int64_t>(id) * a.n_kv_heads + h];
-  if (isv ? a.v_vec16 : a.k_vec16) {  // 16 elements a lane
-    const int row_log = D == 64 ? 2 : 3, total = (r1 - r0) << row_log;
-#pragma unroll 4
-    for (int c = lane; c < total; c += 32) {
-      const int r = c >> row_log, d = (c & ((1 << row_log) - 1)) * 16;
-      const uint4 w = *reinterpret_cast<const uint4*>(src + r * pitch + d);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-      T* to = dst + r * stride + d;
+  for (int h = h0; h < h1; ++h) {
+    T* dst = static_cast<T*>(const_cast<void*>(isv ? a.v : a.k)) + out0 * stride + static_cast<int64_t>(h) * D;
+    const int8_t* src = static_cast<const int8_t*>(isv ? a.v_pool : a.k_pool) +
+                        (static_cast<int64_t>(id) * bs * a.n_kv_heads + h) * D + r0 * pitch;
+    const float sc = (isv ? a.v_scale : a.k_scale)[static_cast<int64_t>(id) * a.n_kv_heads + h];
+    if (isv ? a.v_vec16 : a.k_vec16) {  // 16 elements a lane, four loads ahead of the stores
+      const int row_log = D == 64 ? 2 : 3, total = (r1 - r0) << row_log;
+      for (int c0 = lane; c0 < total; c0 += 128) {
+        uint4 w[4];
 #pragma unroll
-      for (int k = 0; k < 4; k += 16 / (4 * static_cast<int>(sizeof(T)))) {
-        float v[8];
-        bytes_to_f(u[k], v);
-        if constexpr (sizeof(T) == 2) bytes_to_f(u[k + 1], v + 4);
+        for (int k = 0; k < 4; ++k) {
+          const int c = c0 + 32 * k;
+          if (c < total) w[k] = *reinterpret_cast<const uint4*>(src + (c >> row_log) * pitch + (c & ((1 << row_log) - 1)) * 16);
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= sc;
-        if constexpr (sizeof(T) == 2) {
-          reinterpret_cast<uint4*>(to)[k / 2] = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
-        } else {
-          reinterpret_cast<float4*>(to)[k] = make_float4(v[0], v[1], v[2], v[3]);
+        for (int k = 0; k < 4; ++k) {
+          const int c = c0 + 32 * k;
+          if (c >= total) continue;
+          T* to = dst + (c >> row_log) * stride + (c & ((1 << row_log) - 1)) * 16;
+          const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+          float v[16];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) bytes_to_f(u[i], v + 4 * i);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] *= sc;
+          if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              reinterpret_cast<uint4*>(to)[i] = make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
+                                                           pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              reinterpret_cast<float4*>(to)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          }
         }
       }
+      continue;
     }
-    return;
-  }
-  const int cpr = D / 4, total = (r1 - r0) * cpr;
-  for (int c = lane; c < total; c += 32) {
-    const int r = c / cpr, d = (c - r * cpr) * 4;
-    float v[4];
-    bytes_to_f(*reinterpret_cast<const uint32_t*>(src + r * pitch + d), v);
+    const int cpr = D / 4, total = (r1 - r0) * cpr;
+    for (int c = lane; c < total; c += 32) {
+      const int r = c / cpr, d = (c - r * cpr) * 4;
+      float v[4];
+      bytes_to_f(*reinterpret_cast<const uint32_t*>(src + r * pitch + d), v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= sc;
-    store4_any<T>(dst + r * stride + d, vec, v);
+      for (int i = 0; i < 4; ++i) v[i] *= sc;
+      store4_any<T>(dst + r * stride + d, vec, v);
+    }
   }
 }
 
@@ -412,7 +453,11 @@ __global__ void __launch_bounds__(128) lay_out_int8_kernel(const Int8LayArgs a) 
 
 template <typename K>
 cudaError_t launch_rows(K f16, K bf16, K f32, Int8RowsArgs a, cudaStream_t stream) {
-  const int64_t warps = a.n_units * 2 * a.n_kv_heads;
+  // one head a warp while that leaves the SMs' warp slots short, up to four beyond
+  const int64_t each = a.n_units * 2 * a.n_kv_heads;
+  a.heads_per_warp = each < 32768 ? 1 : each < 65536 ? 2 : 4;
+  if (a.heads_per_warp > a.n_kv_heads) a.heads_per_warp = a.n_kv_heads;
+  const int64_t warps = a.n_units * 2 * ((a.n_kv_heads + a.heads_per_warp - 1) / a.heads_per_warp);
   const int64_t grid = (warps + kI8Warps - 1) / kI8Warps;
   if (grid == 0) return cudaSuccess;
   if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;

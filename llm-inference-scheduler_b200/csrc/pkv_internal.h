@@ -207,6 +207,7 @@ struct Int8RowsArgs {
   int n_seqs, n_rows, num_blocks, block_size, n_kv_heads, head_dim, dtype;
   int* err;
   int k_vec, v_vec, k_vec16, v_vec16;  // set by the launcher: accesses of 4 elements, of 16 bytes
+  int heads_per_warp;                     // likewise
   int64_t n_units;
 };
 cudaError_t launch_append_int8(Int8RowsArgs a, cudaStream_t stream);
