@@ -201,13 +201,16 @@ __global__ void __launch_bounds__(kI8Warps * 32) append_int8_kernel(const Int8Ro
   bool once = (isv ? a.v_vec16 : a.k_vec16) && chunks <= 32 * kI8Regs;
   uint4 raw[kI8Regs];
   float amax = 0.f;
+  // a load of the warp covers 32 >> row_log rows
+  const int lane_row = lane >> row_log, lane_col = (lane & ((1 << row_log) - 1)) << kLog;
   if (once) {
+    const T* from = src + lane_row * stride + lane_col;
+    const int64_t step = (32 >> row_log) * stride;
 #pragma unroll
     for (int i = 0; i < kI8Regs; ++i) {
-      const int c = i * 32 + lane;
       raw[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (c < chunks)
-        raw[i] = *reinterpret_cast<const uint4*>(src + (c >> row_log) * stride + ((c & ((1 << row_log) - 1)) << kLog));
+      if (i * 32 + lane < chunks) raw[i] = *reinterpret_cast<const uint4*>(from);
+      from += step;
     }
     // the largest magnitude as an integer: of the bit patterns without their
     // signs (two 16-bit ones at a time), which order as the values do, with
@@ -267,13 +270,13 @@ __global__ void __launch_bounds__(kI8Warps * 32) append_int8_kernel(const Int8Ro
   const float inv = 1.f / sc;  // exact: a power of two
   if (once) {
     const float2 inv2 = make_float2(inv, inv);
+    int8_t* to = dst + (held + lane_row) * pitch + lane_col;
+    const int64_t step = (32 >> row_log) * pitch;
 #pragma unroll
-    for (int i = 0; i < kI8Regs; ++i) {
-      const int c = i * 32 + lane;
-      if (c >= chunks) continue;
+    for (int i = 0; i < kI8Regs; ++i, to += step) {
+      if (i * 32 + lane >= chunks) continue;
       float v[kPer];
       unpack16<T>(raw[i], v);
-      int8_t* to = dst + (held + (c >> row_log)) * pitch + ((c & ((1 << row_log) - 1)) << kLog);
       if constexpr (kPer == 8) {
         *reinterpret_cast<uint2*>(to) = make_uint2(pack_scaled(v, inv2), pack_scaled(v + 4, inv2));
       } else {
@@ -342,35 +345,36 @@ __global__ void __launch_bounds__(kI8Warps * 32) fetch_int8_kernel(const Int8Row
     const int8_t* src = static_cast<const int8_t*>(isv ? a.v_pool : a.k_pool) +
                         (static_cast<int64_t>(id) * bs * a.n_kv_heads + h) * D + r0 * pitch;
     const float sc = (isv ? a.v_scale : a.k_scale)[static_cast<int64_t>(id) * a.n_kv_heads + h];
-    if (isv ? a.v_vec16 : a.k_vec16) {  // 16 elements a lane, four loads ahead of the stores
-      const int row_log = D == 64 ? 2 : 3, total = (r1 - r0) << row_log;
-      for (int c0 = lane; c0 < total; c0 += 128) {
-        uint4 w[4];
+    if (isv ? a.v_vec16 : a.k_vec16) {
+      // a 16-byte store a lane, so that a store of the warp fills whole sectors
+      // (two a lane, 32 bytes apart, wrote every sector twice); eight loads ahead
+      constexpr int kPer = 16 / sizeof(T);
+      const int row_log = (D == 64 ? 6 : 7) - (sizeof(T) == 2 ? 3 : 2), total = (r1 - r0) << row_log;
+      const int row = lane >> row_log, col = (lane & ((1 << row_log) - 1)) * kPer;
+      const int8_t* from = src + row * pitch + col;
+      T* to = dst + row * stride + col;
+      const int64_t from_step = (32 >> row_log) * pitch, to_step = (32 >> row_log) * stride;
+      for (int c0 = lane; c0 < total; c0 += 256) {
+        uint2 w[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int c = c0 + 32 * k;
-          if (c < total) w[k] = *reinterpret_cast<const uint4*>(src + (c >> row_log) * pitch + (c & ((1 << row_log) - 1)) * 16);
-        }
+        for (int k = 0; k < 8; ++k, from += from_step)
+          if (c0 + 32 * k < total) {
+            if constexpr (sizeof(T) == 2) w[k] = *reinterpret_cast<const uint2*>(from);
+            else w[k].x = *reinterpret_cast<const uint32_t*>(from);
+          }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int c = c0 + 32 * k;
-          if (c >= total) continue;
-          T* to = dst + (c >> row_log) * stride + (c & ((1 << row_log) - 1)) * 16;
-          const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-          float v[16];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) bytes_to_f(u[i], v + 4 * i);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] *= sc;
+        for (int k = 0; k < 8; ++k, to += to_step) {
+          if (c0 + 32 * k >= total) continue;
+          float v[8];
+          bytes_to_f(w[k].x, v);
           if constexpr (sizeof(T) == 2) {
+            bytes_to_f(w[k].y, v + 4);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              reinterpret_cast<uint4*>(to)[i] = make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
-                                                           pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
+            for (int i = 0; i < 8; ++i) v[i] *= sc;
+            *reinterpret_cast<uint4*>(to) =
+                make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
           } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              reinterpret_cast<float4*>(to)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            *reinterpret_cast<float4*>(to) = make_float4(v[0] * sc, v[1] * sc, v[2] * sc, v[3] * sc);
           }
         }
       }
@@ -417,36 +421,36 @@ __global__ void __launch_bounds__(128) lay_out_int8_kernel(const Int8LayArgs a) 
   }
   const int valid = id < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(16), keys - row0));
   const int pitch = a.n_kv_heads * a.head_dim;       // elements of a row
-  const int chunks = pitch / 16;                     // 16 elements at a time
+  constexpr int kPer = 16 / sizeof(T);               // elements of a 16-byte store
+  const int chunks = pitch / kPer;
   const int64_t src0 = (static_cast<int64_t>(id < 0 ? 0 : id) * bs + row0 % bs) * pitch;
   const int64_t dst0 = (static_cast<int64_t>(s) * a.cap + row0) * pitch;
+  // 16 rows x pitch are consecutive on both sides
   for (int c = threadIdx.x; c < 2 * 16 * chunks; c += blockDim.x) {
     const bool isv = c >= 16 * chunks;
     const int cc = isv ? c - 16 * chunks : c;
-    const int r = cc / chunks, e = (cc - r * chunks) * 16;
-    T* dst = static_cast<T*>(isv ? a.v_out : a.k_out) + dst0 + static_cast<int64_t>(r) * pitch + e;
-    float v[16];
+    const int r = cc / chunks, e = (cc - r * chunks) * kPer;
+    T* dst = static_cast<T*>(isv ? a.v_out : a.k_out) + dst0 + static_cast<int64_t>(cc) * kPer;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
     if (r < valid) {
-      const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const int8_t*>(isv ? a.v_pool : a.k_pool) +
-                                                      src0 + static_cast<int64_t>(r) * pitch + e);
+      const int8_t* src = static_cast<const int8_t*>(isv ? a.v_pool : a.k_pool) + src0 + static_cast<int64_t>(cc) * kPer;
       const float sc = (isv ? a.v_scale : a.k_scale)[static_cast<int64_t>(id) * a.n_kv_heads + e / a.head_dim];
-      bytes_to_f(w.x, v), bytes_to_f(w.y, v + 4), bytes_to_f(w.z, v + 8), bytes_to_f(w.w, v + 12);
+      if constexpr (sizeof(T) == 2) {
+        const uint2 w = *reinterpret_cast<const uint2*>(src);
+        bytes_to_f(w.x, v), bytes_to_f(w.y, v + 4);
+      } else {
+        bytes_to_f(*reinterpret_cast<const uint32_t*>(src), v);
+      }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] *= sc;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = 0.f;
+      for (int i = 0; i < 8; ++i) v[i] *= sc;
     }
     if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
     } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        reinterpret_cast<uint4*>(dst)[i] =
-            make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
-                       pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
+      *reinterpret_cast<uint4*>(dst) =
+          make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
     }
   }
 }
