@@ -649,9 +649,11 @@ int pkv_paged_decode_attention_int8(void* out, int64_t out_row_stride, const voi
                                     int block_size, float scale, int dtype, void* workspace,
                                     size_t workspace_bytes, int* err_flags, pkv_stream_t stream);
 
-/* Scratch of the chunked prefill below: the visible rows of every sequence as values. */
-size_t pkv_prefill_int8_scratch_bytes(int n_seqs, int max_blocks_per_seq, int n_kv_heads,
-                                      int head_dim, int block_size, int dtype);
+/* Scratch of the chunked prefill below (any initial contents): the visible rows of
+ * every sequence as values and, for calls of few rows, the partial results of work
+ * split over the keys. */
+size_t pkv_prefill_int8_scratch_bytes(int n_seqs, int n_tokens, int max_blocks_per_seq, int n_q_heads,
+                                      int n_kv_heads, int head_dim, int block_size, int dtype);
 
 /* pkv_paged_prefill_attention over such pools (the chunk already appended): query
  * i of sequence s sees keys 0 .. num_prior[s] + i.  One pass lays the visible

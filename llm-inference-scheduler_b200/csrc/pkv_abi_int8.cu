@@ -202,13 +202,31 @@ static int64_t lay_cap(int max_blocks, int block_size) {
   return (static_cast<int64_t>(max_blocks) * block_size + 127) / 128 * 128;
 }
 
-size_t pkv_prefill_int8_scratch_bytes(int n_seqs, int max_blocks_per_seq, int n_kv_heads,
-                                      int head_dim, int block_size, int dtype) {
-  if (n_seqs <= 0 || max_blocks_per_seq <= 0 || n_kv_heads <= 0 || head_dim <= 0 || block_size <= 0 ||
-      !known_dtype(dtype))
+// the scratch: K and V rows, then counters, O and (m, l) of the segments
+namespace {
+struct PrefillScratch {
+  size_t kv, counts, o, ml, total;  // bytes of K (and of V), offsets, size
+  int parts;
+};
+PrefillScratch prefill_scratch(int n_seqs, int n_tokens, int max_blocks, int hq, int hkv, int d, int bs, int dtype) {
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  PrefillScratch s;
+  s.kv = static_cast<size_t>(n_seqs) * lay_cap(max_blocks, bs) * hkv * d * size_of(dtype);
+  s.parts = packed_split_parts(n_seqs, n_tokens, hq, hkv, static_cast<int64_t>(max_blocks) * bs, dtype);
+  s.counts = up(2 * s.kv);
+  s.o = s.counts + up(static_cast<size_t>(s.parts) * 32);
+  s.ml = s.o + static_cast<size_t>(s.parts) * 2 * 128 * d * 4;
+  s.total = s.ml + static_cast<size_t>(s.parts) * 2 * 128 * 8;
+  return s;
+}
+}  // namespace
+
+size_t pkv_prefill_int8_scratch_bytes(int n_seqs, int n_tokens, int max_blocks_per_seq, int n_q_heads,
+                                      int n_kv_heads, int head_dim, int block_size, int dtype) {
+  if (n_seqs <= 0 || n_tokens < 0 || max_blocks_per_seq <= 0 || n_kv_heads <= 0 || n_q_heads < n_kv_heads ||
+      head_dim <= 0 || block_size <= 0 || !known_dtype(dtype) || n_q_heads / n_kv_heads > 65535)
     return 0;
-  return static_cast<size_t>(2) * n_seqs * lay_cap(max_blocks_per_seq, block_size) * n_kv_heads *
-         head_dim * size_of(dtype);
+  return prefill_scratch(n_seqs, n_tokens, max_blocks_per_seq, n_q_heads, n_kv_heads, head_dim, block_size, dtype).total;
 }
 
 int pkv_paged_prefill_attention_int8(void* out, int64_t out_row_stride, const void* q,
@@ -231,9 +249,9 @@ int pkv_paged_prefill_attention_int8(void* out, int64_t out_row_stride, const vo
   if (q_row_stride < row || out_row_stride < row) return PKV_ERR_BAD_SHAPE;
   const int64_t cap = lay_cap(max_blocks_per_seq, block_size);
   if (n_seqs > 65535 || cap * n_seqs > 0x7fffffff) return PKV_ERR_BAD_SHAPE;
-  if (scratch_bytes < pkv_prefill_int8_scratch_bytes(n_seqs, max_blocks_per_seq, n_kv_heads, head_dim,
-                                                     block_size, dtype))
-    return PKV_ERR_WORKSPACE_TOO_SMALL;
+  const PrefillScratch sc = prefill_scratch(n_seqs, n_tokens, max_blocks_per_seq, n_q_heads, n_kv_heads,
+                                            head_dim, block_size, dtype);
+  if (scratch_bytes < sc.total) return PKV_ERR_WORKSPACE_TOO_SMALL;
   if (!aligned(scratch, 256) || !aligned(q, size_of(dtype)) || !aligned(out, size_of(dtype)))
     return PKV_ERR_MISALIGNED;
   Int8LayArgs y{};
@@ -252,8 +270,10 @@ int pkv_paged_prefill_attention_int8(void* out, int64_t out_row_stride, const vo
   y.n_kv_heads = n_kv_heads;
   y.head_dim = head_dim;
   y.k_out = scratch;
-  y.v_out = static_cast<uint8_t*>(scratch) +
-            static_cast<size_t>(n_seqs) * cap * n_kv_heads * head_dim * size_of(dtype);
+  uint8_t* room = static_cast<uint8_t*>(scratch);
+  y.v_out = room + sc.kv;
+  y.zero = reinterpret_cast<int*>(room + sc.counts);
+  y.n_zero = 8 * sc.parts;
   y.cap = static_cast<int>(cap);
   y.err = err_flags;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -271,6 +291,10 @@ int pkv_paged_prefill_attention_int8(void* out, int64_t out_row_stride, const vo
   a.num_prior = num_prior;
   a.key_cap = static_cast<int>(cap);
   a.n_key_rows = static_cast<int>(cap * n_seqs);
+  a.n_parts = sc.parts;
+  a.part_count = sc.parts ? y.zero : nullptr;
+  a.part_o = reinterpret_cast<float*>(room + sc.o);
+  a.part_ml = reinterpret_cast<float2*>(room + sc.ml);
   a.key_limit = max_blocks_per_seq * block_size;
   a.n_seqs = n_seqs;
   a.n_tokens = n_tokens;

@@ -392,65 +392,82 @@ __global__ void __launch_bounds__(kI8Warps * 32) fetch_int8_kernel(const Int8Row
   }
 }
 
-// Rows 16 j .. 16 j + 15 of sequence s (CTA (j, s)) as values, all heads, K and
-// V, into row s * cap + 16 j of k_out / v_out [n_seqs * cap][n_kv_heads][D], so
-// that a sequence's visible keys are consecutive rows.  Rows past its last key
-// are zeros up to the next multiple of 128 (the attention kernel's key tile):
-// a tile holds no stale bytes.
+// The visible rows of sequence blockIdx.y as values, all heads, K and V, row j
+// into row s * cap + j of k_out / v_out [n_seqs * cap][n_kv_heads][D], so that a
+// sequence's keys are consecutive rows.  Rows past its last key are zeros up to
+// the next multiple of 128 (the attention kernel's key tile): a tile holds no
+// stale bytes.  A warp takes up to kLayLoads stores a lane of a 16-row group's K or V at
+// a time, all its loads ahead of them.
+// Also clears the counters of the attention behind it.
+constexpr int kLayThreads = 256, kLayLoads = 8;
 template <typename T>
-__global__ void __launch_bounds__(128) lay_out_int8_kernel(const Int8LayArgs a) {
+__global__ void __launch_bounds__(kLayThreads) lay_out_int8_kernel(const Int8LayArgs a) {
   pdl_trigger();
   pdl_wait();  // the append before it writes the pools; an earlier layer may still read the scratch
-  const int j = blockIdx.x, s = blockIdx.y, bs = a.block_size;
+  const int s = blockIdx.y, bs = a.block_size, lane = threadIdx.x & 31;
+  for (int64_t i = (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * kLayThreads + threadIdx.x; i < a.n_zero;
+       i += static_cast<int64_t>(gridDim.x) * gridDim.y * kLayThreads)
+    a.zero[i] = 0;
   const int new_rows = a.query_start_loc[s + 1] - a.query_start_loc[s];
   int64_t keys = static_cast<int64_t>(max(a.num_prior[s], 0)) + max(new_rows, 0);
   if (keys > static_cast<int64_t>(a.max_blocks) * bs) {
-    if (j == 0 && threadIdx.x == 0) raise_flag(a.err, PKV_FLAG_CONTEXT_EXCEEDS_TABLE);
+    if (blockIdx.x == 0 && threadIdx.x == 0) raise_flag(a.err, PKV_FLAG_CONTEXT_EXCEEDS_TABLE);
     keys = static_cast<int64_t>(a.max_blocks) * bs;
   }
-  const int64_t row0 = static_cast<int64_t>(j) * 16;
-  if (row0 >= (keys + 127) / 128 * 128) return;
-  const int jb = static_cast<int>(row0 / bs);
-  int id = -1;
-  if (row0 < keys) {
-    id = a.block_tables[static_cast<int64_t>(s) * a.bt_stride + jb];
-    if (id < 0 || id >= a.num_blocks) {
-      if (threadIdx.x == 0) raise_flag(a.err, PKV_FLAG_BLOCK_OUT_OF_RANGE);
-      id = -1;
-    }
-  }
-  const int valid = id < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(16), keys - row0));
-  const int pitch = a.n_kv_heads * a.head_dim;       // elements of a row
   constexpr int kPer = 16 / sizeof(T);               // elements of a 16-byte store
-  const int chunks = pitch / kPer;
-  const int64_t src0 = (static_cast<int64_t>(id < 0 ? 0 : id) * bs + row0 % bs) * pitch;
-  const int64_t dst0 = (static_cast<int64_t>(s) * a.cap + row0) * pitch;
-  // 16 rows x pitch are consecutive on both sides
-  for (int c = threadIdx.x; c < 2 * 16 * chunks; c += blockDim.x) {
-    const bool isv = c >= 16 * chunks;
-    const int cc = isv ? c - 16 * chunks : c;
-    const int r = cc / chunks, e = (cc - r * chunks) * kPer;
-    T* dst = static_cast<T*>(isv ? a.v_out : a.k_out) + dst0 + static_cast<int64_t>(cc) * kPer;
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    if (r < valid) {
-      const int8_t* src = static_cast<const int8_t*>(isv ? a.v_pool : a.k_pool) + src0 + static_cast<int64_t>(cc) * kPer;
-      const float sc = (isv ? a.v_scale : a.k_scale)[static_cast<int64_t>(id) * a.n_kv_heads + e / a.head_dim];
-      if constexpr (sizeof(T) == 2) {
-        const uint2 w = *reinterpret_cast<const uint2*>(src);
-        bytes_to_f(w.x, v), bytes_to_f(w.y, v + 4);
-      } else {
-        bytes_to_f(*reinterpret_cast<const uint32_t*>(src), v);
+  const int pitch = a.n_kv_heads * a.head_dim;       // elements of a row
+  const int chunks = 16 * pitch / kPer;              // stores of a group, K or V
+  const int parts = (chunks + 32 * kLayLoads - 1) / (32 * kLayLoads);  // warps of a group, K or V
+  const int64_t n_work = (keys + 127) / 128 * 8 * 2 * parts;           // 16-row groups x K, V x parts
+  for (int64_t w = static_cast<int64_t>(blockIdx.x) * (kLayThreads / 32) + (threadIdx.x >> 5); w < n_work;
+       w += static_cast<int64_t>(gridDim.x) * (kLayThreads / 32)) {
+    const int part = static_cast<int>(w % parts);
+    const bool isv = (w / parts) & 1;
+    const int64_t row0 = w / (2 * parts) * 16;
+    int id = -1;
+    if (row0 < keys) {
+      id = a.block_tables[static_cast<int64_t>(s) * a.bt_stride + row0 / bs];
+      if (id < 0 || id >= a.num_blocks) {
+        if (lane == 0) raise_flag(a.err, PKV_FLAG_BLOCK_OUT_OF_RANGE);
+        id = -1;
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= sc;
     }
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-      *reinterpret_cast<uint4*>(dst) =
-          make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+    const int64_t left = id < 0 ? 0 : min(static_cast<int64_t>(16), keys - row0);
+    const int valid = static_cast<int>(left) * pitch / kPer;  // stores of rows that are keys
+    // 16 rows x pitch are consecutive on both sides
+    const int8_t* src = static_cast<const int8_t*>(isv ? a.v_pool : a.k_pool) +
+                        (static_cast<int64_t>(id < 0 ? 0 : id) * bs + row0 % bs) * pitch;
+    T* dst = static_cast<T*>(isv ? a.v_out : a.k_out) + (static_cast<int64_t>(s) * a.cap + row0) * pitch;
+    const float* scale = (isv ? a.v_scale : a.k_scale) + static_cast<int64_t>(id < 0 ? 0 : id) * a.n_kv_heads;
+    uint2 u[kLayLoads];
+    float sc[kLayLoads];
+#pragma unroll
+    for (int k = 0; k < kLayLoads; ++k) {
+      const int c = (part * kLayLoads + k) * 32 + lane;
+      u[k] = make_uint2(0u, 0u);
+      sc[k] = 0.f;
+      if (c < valid) {
+        if constexpr (sizeof(T) == 2) u[k] = *reinterpret_cast<const uint2*>(src + static_cast<int64_t>(c) * kPer);
+        else u[k].x = *reinterpret_cast<const uint32_t*>(src + static_cast<int64_t>(c) * kPer);
+        sc[k] = scale[c * kPer % pitch / a.head_dim];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kLayLoads; ++k) {
+      const int c = (part * kLayLoads + k) * 32 + lane;
+      if (c >= chunks) continue;
+      float v[8];
+      bytes_to_f(u[k].x, v);
+      T* to = dst + static_cast<int64_t>(c) * kPer;
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(to) = make_float4(v[0] * sc[k], v[1] * sc[k], v[2] * sc[k], v[3] * sc[k]);
+      } else {
+        bytes_to_f(u[k].y, v + 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= sc[k];
+        *reinterpret_cast<uint4*>(to) =
+            make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+      }
     }
   }
 }
@@ -508,8 +525,14 @@ cudaError_t launch_fetch_int8(Int8RowsArgs a, cudaStream_t stream) {
 
 cudaError_t launch_lay_out_int8(const Int8LayArgs& a, int dtype, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.cap / 16, a.n_seqs);
-  cfg.blockDim = dim3(128);
+  // a warp for every unit of work of the longest possible sequence, up to what
+  // fills the GPU; the kernel's loop takes the rest
+  const int kv_bytes = 16 * a.n_kv_heads * a.head_dim * (dtype == PKV_DTYPE_F32 ? 4 : 2);
+  const int64_t parts = (kv_bytes + 512 * kLayLoads - 1) / (512 * kLayLoads);
+  const int64_t want = (static_cast<int64_t>(a.cap) / 16 * 2 * parts + kLayThreads / 32 - 1) / (kLayThreads / 32);
+  const int64_t most = (2048 + a.n_seqs - 1) / a.n_seqs;
+  cfg.gridDim = dim3(static_cast<unsigned>(want < most ? want : most), a.n_seqs);
+  cfg.blockDim = dim3(kLayThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

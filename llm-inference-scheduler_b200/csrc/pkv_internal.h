@@ -226,6 +226,8 @@ struct Int8LayArgs {
   void* k_out;
   void* v_out;
   int cap;  // rows per sequence in k_out / v_out, a multiple of 128
+  int* zero;  // words to clear for the attention behind this pass
+  int n_zero;
   int* err;
 };
 cudaError_t launch_lay_out_int8(const Int8LayArgs& a, int dtype, cudaStream_t stream);
@@ -249,12 +251,20 @@ struct PackedArgs {
   int key_cap;
   int key_limit;   // keys a sequence's table can hold
   int n_key_rows;  // rows of k / v
+  // splitting of long items over their keys (NULL: not split): zeroed counters
+  // (8 a segment) and partials for n_parts segments (packed_split_parts)
+  int* part_count = nullptr;
+  float* part_o = nullptr;   // 16-byte aligned
+  float2* part_ml = nullptr;
+  int n_parts = 0;
   int n_seqs, n_tokens, n_q_heads, n_kv_heads, head_dim;
   float scale;
   int dtype;
   int* err;
 };
 cudaError_t launch_packed_attention(const PackedArgs& a, cudaStream_t stream);
+// segments that a chunk call of these sizes may be split into (0: it is not)
+int packed_split_parts(int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads, int64_t key_limit, int dtype);
 
 // TMA descriptor for rows [n_rows][n_heads][head_dim] of 16-bit values (row stride
 // in elements) with a box of 64 dims x box_heads x box_rows, 128-byte swizzle.

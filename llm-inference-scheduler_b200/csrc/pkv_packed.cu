@@ -327,6 +327,16 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
 // softmax warps about 700 cycles, in which one issuer for both would leave the
 // tensor pipe idle (1,780 cycles a step at D = 64).
 //
+// A chunk of few rows behind many cached keys would leave most SMs idle, or one of
+// them busy long after the others.  Where the caller brings room for partials,
+// items much longer than an SM's share of all key tiles are cut over their keys
+// into segments of that length, items of their own; each leaves its normalised O with its maximum and
+// sum, and the one that finishes last joins them in segment order.  16 rows
+// behind 32,768 keys (14 heads / 2 x 64): 226 us unsplit, 42 split; 512 behind
+// 8,192: 95, 65; 16 chunks of about 500 of which two lie behind some 3,400 keys:
+// 79.7, 68.4.  Segments of half the share, of 1,024 keys at least or up to 32 an
+// item were no faster.
+//
 // Items are handed out while the kernel runs: a CTA starts with its own block
 // index and then takes the indices of blocks that have not started
 // (clusterlaunchcontrol.try_cancel), one item ahead, so tensor memory, barriers
@@ -337,7 +347,10 @@ constexpr int kTcProducerWarp = 8, kTcQkWarp = 9, kTcSchedWarp = 10;  // warp 11
 constexpr int kTcRegsSoftmax = 224, kTcRegsOther = 56;
 constexpr int kTcRegSplit = 256 * kTcRegsSoftmax + 128 * kTcRegsOther;
 constexpr int kTcMaxSorted = 384;   // sequences ordered by their keys (more: taken as they come)
-constexpr int kTcItemInts = 8;
+constexpr int kTcItemInts = 12;
+constexpr int kTcMaxSegs = 16;      // segments of an item
+constexpr int kTcSegKeys = 1536;    // least keys of a segment
+constexpr int kTcSplitPerSm = 4;    // split calls of up to this many items an SM
 constexpr uint32_t kTcTmemCols = 512;
 
 template <int D> struct TcShape {
@@ -357,8 +370,8 @@ template <int D> struct TcShape {
   static constexpr int kOffClc = (kOffBar + kBars * 8 + 15) / 16 * 16;
   static constexpr int kOffItem = kOffClc + 16;
   static constexpr int kOffTmem = kOffItem + 2 * kTcItemInts * 4;
-  static constexpr int kOffOrder = kOffTmem + 16;        // sorted sequences, then item prefix
-  static constexpr int kOffOut = (kOffOrder + (2 * kTcMaxSorted + 1) * 4 + 15) / 16 * 16;  // 2 KB per softmax warp
+  static constexpr int kOffOrder = kOffTmem + 16;        // sorted sequences, item prefix, items and key tiles of each
+  static constexpr int kOffOut = (kOffOrder + (4 * kTcMaxSorted + 1) * 4 + 15) / 16 * 16;  // 2 KB per softmax warp
   static constexpr int kBytes = 1024 + kOffOut + 8 * 2048;
   static constexpr uint32_t kColO = kBufs * kN;          // O_A, O_B behind the S buffers
 };
@@ -368,6 +381,7 @@ struct TcParams {
   PackedArgs a;
   int group, tokens;   // query heads per KV head, tokens per tile
   int sorted;
+  int n_sms;
   float scale_log2;
 };
 
@@ -416,10 +430,13 @@ __device__ __forceinline__ int clc_index(const void* result) {
   return ok ? static_cast<int>(x) : -1;
 }
 
-// an item: two tiles of one (sequence, KV head)
+// an item: two tiles of one (sequence, KV head), or a segment of their keys
 struct TcItem {
   int s, g, tok0, q_begin, n_new, prior, keys;
-  int row0;  // first key row
+  int row0;      // first key row
+  int j0, j1;    // key tiles
+  int seg, segs; // which of how many segments
+  int idx;       // index of this one (segment q of the same item: idx + (seg - q) n_kv_heads)
 };
 
 template <typename T, int D>
@@ -451,6 +468,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + Sh::kOffTmem);
   int* order = reinterpret_cast<int*>(base + Sh::kOffOrder);
   int* first_item = order + kTcMaxSorted;
+  int* n_items = first_item + kTcMaxSorted + 1;
+  int* last_tiles = n_items + kTcMaxSorted;
   const PackedArgs& a = p.a;
   const int G = p.group, TT = p.tokens, B = a.n_seqs;
 
@@ -487,6 +506,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (tid == 0) pdl_trigger();
   pdl_wait();  // the starts, q, k and v may come from the kernel before this one
   const int per_item = 2 * TT;
+  __shared__ int seg_len;   // key tiles of a segment, if items are split
+  // segments of the items of a sequence of so many key tiles
+  auto segs_of = [&](int tiles, int len) { return tiles <= max(len + len / 4, 3 * kTcSegKeys / 2 / kN) ? 1 : min(kTcMaxSegs, (tiles + len - 1) / len); };
   if (blockIdx.x == 0)
     for (int t = tid; t < B; t += kTcThreads) {
       const int b = a.query_start_loc[t], n = a.query_start_loc[t + 1] - b;
@@ -505,17 +527,49 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (tid < B)
       for (int u = 0; u < B; ++u) rank += keys[u] > mine || (keys[u] == mine && u < tid);
     __syncthreads();
-    if (tid < B) order[rank] = tid;
+    if (tid < B) {
+      const int len = max(a.query_start_loc[tid + 1] - a.query_start_loc[tid], 0);
+      order[rank] = tid;
+      n_items[rank] = (min(len, a.n_tokens) + per_item - 1) / per_item;
+      if (a.part_count != nullptr) last_tiles[rank] = (key_span(a, tid, 0, len).keys + kN - 1) / kN;
+    }
     __syncthreads();
     if (warp == 0) {
+      if (a.part_count != nullptr) {
+        // an SM's share of the key tiles of all items (a sequence's taken as
+        // between those of its first and last) is a segment's length: there are
+        // at most two SMs' worth more segments than items
+        float work = 0.f, n = 0.f;
+        int most = 0;
+        for (int i = lane; i < B; i += 32) {
+          n += static_cast<float>(n_items[i]);
+          work += n_items[i] * (last_tiles[i] - 0.5f * n_items[i] * per_item / kN);
+          most = max(most, last_tiles[i]);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          work += __shfl_xor_sync(0xffffffffu, work, o);
+          n += __shfl_xor_sync(0xffffffffu, n, o);
+          most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        }
+        int len = max(kTcSegKeys / kN, static_cast<int>(fminf(work * a.n_kv_heads / p.n_sms + 1.f, 1e9f)));
+        float split = 0.f;
+        for (int i = lane; i < B; i += 32) split += static_cast<float>(n_items[i]) * segs_of(last_tiles[i], len);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) split += __shfl_xor_sync(0xffffffffu, split, o);
+        // none if they pass the room all the same (lengths that are flagged); and
+        // items that find an SM each anyway are split only where that shortens the
+        // longest (2,048 rows behind 16,384 keys: 114 items, 192 us; in halves, 210)
+        if (split * a.n_kv_heads > static_cast<float>(gridDim.x) ||
+            (n * a.n_kv_heads <= p.n_sms && ceilf(split * a.n_kv_heads / p.n_sms) >= 0.9f * segs_of(most, len)))
+          len = INT_MAX / 2;
+        if (lane == 0) seg_len = len;
+        __syncwarp();
+      }
       int run = 0;
       for (int b0 = 0; b0 < B; b0 += 32) {
         const int i = b0 + lane;
-        int n = 0;
-        if (i < B) {
-          const int len = a.query_start_loc[order[i] + 1] - a.query_start_loc[order[i]];
-          n = (min(max(len, 0), a.n_tokens) + per_item - 1) / per_item;
-        }
+        const int n = i < B ? n_items[i] * (a.part_count != nullptr ? segs_of(last_tiles[i], seg_len) : 1) : 0;
         int x = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -537,7 +591,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   auto find_item = [&](int idx, TcItem& it) -> bool {
     const int u = idx / a.n_kv_heads;
     it.g = idx - u * a.n_kv_heads;
-    int tile;
+    it.idx = idx;
+    it.seg = 0;
+    it.segs = 1;
+    it.j0 = 0;
+    it.j1 = INT_MAX;
+    int tile, segs = 1, last = 0;
     if (p.sorted) {
       int lo = 0, hi = B - 1;
       if (u >= first_item[B]) return false;
@@ -547,6 +606,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       it.s = order[lo];
       tile = first_item[lo + 1] - 1 - u;  // last tokens first
+      if (a.part_count != nullptr) {
+        last = last_tiles[lo];
+        segs = segs_of(last, seg_len);
+        it.seg = tile % segs;
+        tile /= segs;
+      }
       it.q_begin = a.query_start_loc[it.s];
       it.n_new = a.query_start_loc[it.s + 1] - it.q_begin;
     } else {
@@ -568,6 +633,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     it.prior = k.prior;
     it.keys = k.keys;
     it.row0 = static_cast<int>(k.row0);
+    if (segs > 1) {
+      // the sequence's segments are equally long; an item uses those that its keys reach
+      const int len = (last + segs - 1) / segs;
+      const int tiles = (min(it.prior + min(it.tok0 + per_item, it.n_new), it.keys) + kN - 1) / kN;
+      it.j0 = it.seg * len;
+      it.j1 = it.j0 + len;
+      it.segs = (tiles + len - 1) / len;
+      if (it.seg >= it.segs) return false;
+    }
     return true;
   };
   // item `k` (counted per CTA) as the scheduler published it; tok0 < 0: no more
@@ -576,7 +650,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     bool ok = mbar_wait(&item_full[sl], (k >> 1) & 1);
     ok = __all_sync(0xffffffffu, ok);
     const int* w = items + sl * kTcItemInts;
-    it.s = w[0], it.g = w[1], it.tok0 = w[2], it.q_begin = w[3], it.n_new = w[4], it.prior = w[5], it.keys = w[6], it.row0 = w[7];
+    it.s = w[0], it.g = w[1], it.tok0 = w[2], it.q_begin = w[3], it.n_new = w[4], it.prior = w[5], it.keys = w[6], it.row0 = w[7], it.j0 = w[8], it.j1 = w[9];
+    it.seg = w[10] & 255, it.segs = w[10] >> 8, it.idx = w[11];
     __syncwarp();
     if (lane == 0) mbar_arrive(&item_empty[sl]);
     if (!ok && lane == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
@@ -588,6 +663,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int n = min(max(it.n_new - t0, 0), TT);
     return n > 0 ? min(it.prior + t0 + n, it.keys) : 0;
   };
+  // key tiles of tile x in this item (segment)
+  auto item_tiles = [&](const TcItem& it, int x) { return max(0, min((tile_keys(it, x) + kN - 1) / kN, it.j1) - it.j0); };
 
   if (warp >= 8) {
     setmaxnreg_dec<kTcRegsOther>();
@@ -624,7 +701,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           int* w = items + sl * kTcItemInts;
           w[0] = it.s, w[1] = it.g, w[2] = have ? it.tok0 : -1, w[3] = it.q_begin, w[4] = it.n_new, w[5] = it.prior, w[6] = it.keys,
-          w[7] = it.row0;
+          w[7] = it.row0, w[8] = it.j0, w[9] = it.j1, w[10] = it.seg | (it.segs << 8), w[11] = it.idx;
           mbar_arrive(&item_full[sl]);
           if (!have) break;
         }
@@ -635,7 +712,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       int c = 0;  // K / V tiles loaded so far
       TcItem it;
       for (int k = 0; take_item(k, it); ++k) {
-        const int n_tiles = (max(tile_keys(it, 0), tile_keys(it, 1)) + kN - 1) / kN;
+        const int n_tiles = max(item_tiles(it, 0), item_tiles(it, 1));
         if (k >= 1 && !__all_sync(0xffffffffu, mbar_wait(q_empty, (k - 1) & 1))) {
           if (lane == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
           break;
@@ -667,7 +744,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
               for (int h = 0; h < kHalves; ++h)
                 tma_load_3d(base + (kv ? Sh::kOffV : Sh::kOffK) + st * Sh::kKTile + h * Sh::kKHalf, kv ? &vmap : &kmap, full, h * 64, it.g,
-                            it.row0 + j * kN);
+                            it.row0 + (it.j0 + j) * kN);
             }
             __syncwarp();
           }
@@ -691,8 +768,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       auto open_item = [&](int k) {
         TcItem it;
         const bool ok = __all_sync(0xffffffffu, take_item(k, it));
-        nt0 = __shfl_sync(0xffffffffu, (tile_keys(it, 0) + kN - 1) / kN, 0);
-        nt1 = __shfl_sync(0xffffffffu, (tile_keys(it, 1) + kN - 1) / kN, 0);
+        nt0 = __shfl_sync(0xffffffffu, item_tiles(it, 0), 0);
+        nt1 = __shfl_sync(0xffffffffu, item_tiles(it, 1), 0);
         return ok;
       };
       // past a step of tile x
@@ -788,8 +865,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     bool dead = false;
     TcItem it;
     for (int k = 0; take_item(k, it); ++k) {
-      const int kvx = tile_keys(it, x), ntx = (kvx + kN - 1) / kN;
-      const int nto = (tile_keys(it, 1 - x) + kN - 1) / kN;
+      const int kvx = tile_keys(it, x), ntx = item_tiles(it, x), nto = item_tiles(it, 1 - x);
       // PV number i of this item and tile has completed.  PVs signal a ring of
       // barriers: a wait tells a phase from the one before it only, and the S
       // that the caller has seen vouches for the PV a ring's length back.
@@ -817,7 +893,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_wait_ld_regs(sr[0]);
 #pragma unroll
         for (int c4 = 1; c4 < kN / 32; ++c4) reg_after_wait(sr[c4]);
-        const int kbase = j * kN;
+        const int kbase = (it.j0 + j) * kN;
         if (kbase + kN > lim) {
 #pragma unroll
           for (int c = 0; c < kN; ++c)
@@ -880,47 +956,123 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       bool fine = true;
       const int64_t row = static_cast<int64_t>(it.q_begin) + tok;
       const int head = it.g * G + rhead;
+      // 32 columns at a time through the warp's 2 KB: a store then covers 64
+      // bytes of each of 8 rows (each thread storing its own row, 16 bytes
+      // here and there, took 3,300 cycles an item at D = 64, 5,500 at 128)
+      const int64_t off = row * a.out_stride + static_cast<int64_t>(head) * D;
+      const unsigned rows_ok = __ballot_sync(0xffffffffu, row_valid);
+      uint8_t* mine = base + Sh::kOffOut + warp * 2048;
+      int64_t roff[4];
+#pragma unroll
+      for (int r8 = 0; r8 < 4; ++r8) roff[r8] = __shfl_sync(0xffffffffu, off, r8 * 8 + (lane >> 2));
+      auto store32 = [&](int c2, const float* f) {
+#pragma unroll
+        for (int c8 = 0; c8 < 4; ++c8)
+          *reinterpret_cast<uint4*>(mine + lane * 64 + ((c8 ^ ((lane >> 1) & 3)) << 4)) =
+              make_uint4(pack2<T>(f[8 * c8], f[8 * c8 + 1]), pack2<T>(f[8 * c8 + 2], f[8 * c8 + 3]),
+                         pack2<T>(f[8 * c8 + 4], f[8 * c8 + 5]), pack2<T>(f[8 * c8 + 6], f[8 * c8 + 7]));
+        __syncwarp();
+#pragma unroll
+        for (int r8 = 0; r8 < 4; ++r8) {
+          const int rr = r8 * 8 + (lane >> 2), c8 = lane & 3;
+          const uint4 v = *reinterpret_cast<const uint4*>(mine + rr * 64 + ((c8 ^ ((rr >> 1) & 3)) << 4));
+          if ((rows_ok >> rr) & 1) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + roff[r8] + c2 * 32 + c8 * 8) = v;
+        }
+        __syncwarp();
+      };
+      // partials of segment q: four columns of a tile's 128 rows side by side
+      auto part_slot = [&](int q) { return static_cast<int64_t>(it.idx + (it.seg - q) * a.n_kv_heads) * 2 + x; };
+      const bool whole = it.segs == 1;
       if (ntx > 0) {
         wait_pv(ntx - 1);
         __syncwarp();
         tc_fence_after();
         const float inv = l > 0.f ? 1.f / l : l;  // NaN stays
         float fsum = l;
-        // 32 columns at a time through the warp's 2 KB: a store then covers 64
-        // bytes of each of 8 rows (each thread storing its own row, 16 bytes
-        // here and there, took 3,300 cycles an item at D = 64, 5,500 at 128)
-        const int64_t off = row * a.out_stride + static_cast<int64_t>(head) * D;
-        const unsigned rows_ok = __ballot_sync(0xffffffffu, row_valid);
-        uint8_t* mine = base + Sh::kOffOut + warp * 2048;
-        int64_t roff[4];
-#pragma unroll
-        for (int r8 = 0; r8 < 4; ++r8) roff[r8] = __shfl_sync(0xffffffffu, off, r8 * 8 + (lane >> 2));
 #pragma unroll
         for (int c2 = 0; c2 < D / 32; ++c2) {
           uint32_t o[32];
           tmem_ld32(t_o + c2 * 32, o);
           tmem_wait_ld_regs(o);
+          float f[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) fsum += fabsf(__uint_as_float(o[i]));
-#pragma unroll
-          for (int c8 = 0; c8 < 4; ++c8) {
-            float f[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[c8 * 8 + i]) * inv;
-            *reinterpret_cast<uint4*>(mine + lane * 64 + ((c8 ^ ((lane >> 1) & 3)) << 4)) =
-                make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+          for (int i = 0; i < 32; ++i) {
+            fsum += fabsf(__uint_as_float(o[i]));
+            f[i] = __uint_as_float(o[i]) * inv;
           }
-          __syncwarp();
+          if (whole) {
+            store32(c2, f);
+          } else {
+            float4* to = reinterpret_cast<float4*>(a.part_o) + (part_slot(it.seg) * (D / 4) + c2 * 8) * 128 + r;
 #pragma unroll
-          for (int r8 = 0; r8 < 4; ++r8) {
-            const int rr = r8 * 8 + (lane >> 2), c8 = lane & 3;
-            const uint4 v = *reinterpret_cast<const uint4*>(mine + rr * 64 + ((c8 ^ ((rr >> 1) & 3)) << 4));
-            if ((rows_ok >> rr) & 1) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + roff[r8] + c2 * 32 + c8 * 8) = v;
+            for (int i = 0; i < 8; ++i) to[i * 128] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
           }
-          __syncwarp();
         }
         tc_fence_before();  // O is read before the next item's PV (ordered by p_full)
-        fine = !row_valid || fsum < INFINITY;
+        if (whole) fine = !row_valid || fsum < INFINITY;
+      }
+      if (!whole) {
+        // each warp on its own: its rows of all segments are in memory once their
+        // warps have counted
+        a.part_ml[part_slot(it.seg) * 128 + r] = make_float2(m_used, ntx > 0 ? l : 0.f);
+        __threadfence();
+        __syncwarp();
+        int seen = 0;
+        if (lane == 0) seen = atomicAdd(a.part_count + (it.idx + it.seg * a.n_kv_heads) * 8 + warp, 1);
+        if (__shfl_sync(0xffffffffu, seen, 0) == it.segs - 1) {
+          __threadfence();
+          // several segments' loads at a time: each is a trip to L2
+          float top = -INFINITY, sum = 0.f, w[kTcMaxSegs];
+          float2 ml[kTcMaxSegs];
+#pragma unroll 4
+          for (int q = 0; q < kTcMaxSegs; ++q) {
+            if (q < it.segs) ml[q] = __ldcg(a.part_ml + part_slot(q) * 128 + r);
+          }
+          for (int q = 0; q < it.segs; ++q)
+            if (ml[q].y != 0.f) top = fmaxf(top, ml[q].x);  // (0: the row saw nothing there)
+          for (int q = 0; q < it.segs; ++q) {
+            w[q] = ml[q].y != 0.f ? ex2_approx(ml[q].x - top) * ml[q].y : 0.f;
+            sum += w[q];
+          }
+          const float inv = sum > 0.f ? 1.f / sum : sum;  // NaN stays
+          float fsum = sum;
+          for (int c2 = 0; c2 < D / 32; ++c2) {
+            float f[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = 0.f;
+            for (int q = 0; q < it.segs; q += 2) {
+              const float w0 = w[q] * inv, w1 = q + 1 < it.segs ? w[q + 1] * inv : 0.f;
+              const float4* from0 = reinterpret_cast<const float4*>(a.part_o) + (part_slot(q) * (D / 4) + c2 * 8) * 128 + r;
+              const float4* from1 = from0 - (q + 1 < it.segs ? a.n_kv_heads * 2 * (D / 4) * 128 : 0);
+              float4 v0[8], v1[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v0[i] = __ldcg(from0 + i * 128);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v1[i] = __ldcg(from1 + i * 128);
+              // (without a weight its O may not have been written)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                if (w0 != 0.f) {
+                  f[4 * i] = fmaf(w0, v0[i].x, f[4 * i]);
+                  f[4 * i + 1] = fmaf(w0, v0[i].y, f[4 * i + 1]);
+                  f[4 * i + 2] = fmaf(w0, v0[i].z, f[4 * i + 2]);
+                  f[4 * i + 3] = fmaf(w0, v0[i].w, f[4 * i + 3]);
+                }
+                if (w1 != 0.f) {
+                  f[4 * i] = fmaf(w1, v1[i].x, f[4 * i]);
+                  f[4 * i + 1] = fmaf(w1, v1[i].y, f[4 * i + 1]);
+                  f[4 * i + 2] = fmaf(w1, v1[i].z, f[4 * i + 2]);
+                  f[4 * i + 3] = fmaf(w1, v1[i].w, f[4 * i + 3]);
+                }
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) fsum += fabsf(f[i]);
+            __syncwarp();
+            store32(c2, f);
+          }
+          fine = !row_valid || fsum < INFINITY;
+        }
       }
       cx += ntx;
       n0 += ntx + nto;
@@ -950,10 +1102,15 @@ bool tc_supported(const PackedArgs& a) {
          al(a.v, a.v_stride) && al(a.out, a.out_stride);
 }
 
+int64_t tc_items(int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads) {
+  const int tokens = kTcM / (n_q_heads / n_kv_heads);
+  return (n_tokens / (2 * tokens) + static_cast<int64_t>(n_seqs)) * n_kv_heads;
+}
+
 template <typename T, int D>
 cudaError_t launch_tc(const PackedArgs& a, cudaStream_t stream) {
   auto kern = packed_tc_kernel<T, D>;
-  static std::atomic<int> ready[64];  // per device: 0 not asked, 1 ready, -1 the register split does not fit
+  static std::atomic<int> ready[64];  // per device: 0 not asked, SMs: ready, -1 the register split does not fit
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -962,27 +1119,31 @@ cudaError_t launch_tc(const PackedArgs& a, cudaStream_t stream) {
     cudaFuncAttributes fa;
     e = cudaFuncGetAttributes(&fa, kern);
     if (e != cudaSuccess) return e;
-    state = fa.numRegs * kTcThreads >= kTcRegSplit ? 1 : -1;
-    if (state == 1) {
+    state = -1;
+    if (fa.numRegs * kTcThreads >= kTcRegSplit) {
       e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<D>::kBytes);
+      if (e == cudaSuccess) e = cudaDeviceGetAttribute(&state, cudaDevAttrMultiProcessorCount, dev);
       if (e != cudaSuccess) return e;
     }
     if (dev < 64) ready[dev].store(state);
   }
-  if (state != 1) return launch_cores<T, D>(a, stream);
+  if (state < 0) return launch_cores<T, D>(a, stream);
   TcParams p{};
   p.a = a;
   p.group = a.n_q_heads / a.n_kv_heads;
   p.tokens = kTcM / p.group;
   p.sorted = a.n_seqs <= kTcMaxSorted;
+  p.n_sms = state;
+  if (a.n_parts == 0) p.a.part_count = nullptr;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   CUtensorMap qm, km, vm;
   int rc = encode_rows_tensormap(&qm, a.q, a.q_stride, a.n_tokens, a.n_q_heads, D, a.dtype, p.group, p.tokens);
   if (rc == 0) rc = encode_rows_tensormap(&km, a.k, a.k_stride, a.n_key_rows, a.n_kv_heads, D, a.dtype, 1, TcShape<D>::kN);
   if (rc == 0) rc = encode_rows_tensormap(&vm, a.v, a.v_stride, a.n_key_rows, a.n_kv_heads, D, a.dtype, 1, TcShape<D>::kN);
   if (rc != 0) return cudaErrorNotSupported;
-  const int64_t items = (a.n_tokens / (2 * p.tokens) + static_cast<int64_t>(a.n_seqs)) * a.n_kv_heads;
+  int64_t items = tc_items(a.n_seqs, a.n_tokens, a.n_q_heads, a.n_kv_heads);
   if (items > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  if (p.a.part_count != nullptr) items = a.n_parts;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(items));
   cfg.blockDim = dim3(kTcThreads);
@@ -998,6 +1159,16 @@ cudaError_t launch_tc(const PackedArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
+// The room for partials: a slot for every item and two for each of 148 SMs
+// besides; none if no item can be long enough.  Calls with more than
+// kTcSplitPerSm items an SM are not split (they fill the GPU, and their partials
+// would fill memory).
+int packed_split_parts(int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads, int64_t key_limit, int dtype) {
+  if (dtype == PKV_DTYPE_F32 || n_seqs > kTcMaxSorted || n_q_heads / n_kv_heads > 64) return 0;
+  if (key_limit <= 3 * kTcSegKeys / 2) return 0;
+  const int64_t items = tc_items(n_seqs, n_tokens, n_q_heads, n_kv_heads);
+  return items > 148 * kTcSplitPerSm ? 0 : static_cast<int>(items + 2 * 148);
+}
 cudaError_t launch_packed_attention(const PackedArgs& a, cudaStream_t stream) {
   if (a.n_tokens == 0 || a.n_seqs == 0) return cudaSuccess;
   auto go = [&](auto tag) {

@@ -713,9 +713,9 @@ class PagedKVCache:
             self._counts = torch.arange(max(n, 1025), dtype=torch.int32, device=self.mgr.device)
         return self._counts[:n]
 
-    def int8_buffers(self, n_prefill: int, width: int, n_q_heads: int, dtype: torch.dtype):
+    def int8_buffers(self, n_prefill: int, n_tokens: int, width: int, n_q_heads: int, dtype: torch.dtype):
         """The int8 pools' split-K workspace and prefill scratch (None without
-        prefill sequences), grown on demand and reused across layers and
+        prefill sequences; n_tokens: their rows), grown on demand and reused across layers and
         steps (stream order keeps each use behind the previous)."""
         mgr = self.mgr
         need = ops.decode_int8_workspace_bytes(n_q_heads, mgr.head_dim)
@@ -723,8 +723,8 @@ class PagedKVCache:
             self._int8_workspace = torch.empty(need, dtype=torch.uint8, device=mgr.device)
         if not n_prefill:
             return self._int8_workspace, None
-        need = ops.prefill_int8_scratch_bytes(n_prefill, width, mgr.num_kv_heads, mgr.head_dim,
-                                              mgr.block_size, dtype)
+        need = ops.prefill_int8_scratch_bytes(n_prefill, n_tokens, width, n_q_heads, mgr.num_kv_heads,
+                                              mgr.head_dim, mgr.block_size, dtype)
         if self._int8_scratch is None or self._int8_scratch.numel() < need:
             self._int8_scratch = torch.empty(need, dtype=torch.uint8, device=mgr.device)
         return self._int8_workspace, self._int8_scratch
@@ -736,7 +736,7 @@ class PagedKVCache:
         pools = (mgr.k_pool[layer], mgr.v_pool[layer], mgr.k_scale[layer], mgr.v_scale[layer])
         nd = meta.n_decode
         tabs, ctx = meta.block_tables, meta.context_lens
-        ws, scratch = self.int8_buffers(meta.n_seqs - nd, tabs.shape[1], q.shape[1], q.dtype)
+        ws, scratch = self.int8_buffers(meta.n_seqs - nd, q.shape[0] - nd, tabs.shape[1], q.shape[1], q.dtype)
         if nd:
             ops.reshape_and_cache_int8(k_new[:nd], v_new[:nd], *pools, tabs[:nd], ctx[:nd],
                                        self.counts(nd + 1), mgr.err)

@@ -198,8 +198,9 @@ class StepGraphs:
             kv.counts(Rm + 1)
             if kv._slots_int8 is None or kv._slots_int8.shape[0] < tokens:
                 kv._slots_int8 = torch.arange(tokens, dtype=torch.int64, device=dev)
-            self.int8_held = (kv.int8_buffers(self.prefill_seqs, self.W, cfg.num_attention_heads, m.dtype),
-                              kv._counts, kv._slots_int8)
+            for P in {P for _, P in keys}:  # (a larger one may need less: it is not split)
+                kv.int8_buffers(self.prefill_seqs if P else 0, P, self.W, cfg.num_attention_heads, m.dtype)
+            self.int8_held = (kv._int8_workspace, kv._int8_scratch, kv._counts, kv._slots_int8)
         cos, sin = m.rope.tables(self.W * mgr.block_size)
         self.cos, self.sin = cos, sin  # held: an eager step that grows the tables drops them
 

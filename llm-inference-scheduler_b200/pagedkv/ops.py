@@ -1254,10 +1254,12 @@ def paged_decode_attention_int8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: t
     return out
 
 
-def prefill_int8_scratch_bytes(n_seqs: int, max_blocks_per_seq: int, n_kv_heads: int, head_dim: int,
-                               block_size: int, dtype: torch.dtype) -> int:
-    return int(_lib.load().pkv_prefill_int8_scratch_bytes(n_seqs, max_blocks_per_seq, n_kv_heads,
-                                                          head_dim, block_size, dtype_code(dtype)))
+def prefill_int8_scratch_bytes(n_seqs: int, n_tokens: int, max_blocks_per_seq: int, n_q_heads: int,
+                               n_kv_heads: int, head_dim: int, block_size: int,
+                               dtype: torch.dtype) -> int:
+    return int(_lib.load().pkv_prefill_int8_scratch_bytes(
+        n_seqs, n_tokens, max_blocks_per_seq, n_q_heads, n_kv_heads, head_dim, block_size,
+        dtype_code(dtype)))
 
 
 def paged_prefill_attention_int8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -1285,8 +1287,9 @@ def paged_prefill_attention_int8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: 
     if T == 0 or n_seqs == 0:
         return out
     if scratch is None:
-        scratch = torch.empty(prefill_int8_scratch_bytes(n_seqs, block_tables.shape[1], hkv, d, bs, q.dtype),
-                              dtype=torch.uint8, device=q.device)
+        scratch = torch.empty(
+            prefill_int8_scratch_bytes(n_seqs, T, block_tables.shape[1], hq, hkv, d, bs, q.dtype),
+            dtype=torch.uint8, device=q.device)
     _call("pkv_paged_prefill_attention_int8", dev, out.data_ptr(), _row_stride(out, "out"), q.data_ptr(),
           _row_stride(q, "q"), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
           v_scale.data_ptr(), nb, block_tables.data_ptr(), block_tables.stride(0),

@@ -330,6 +330,8 @@ CHUNKS = {
     "small": ([0, 7, 70, 33], [5, 1, 45, 0]),
     "tiles": ([128, 0, 1, 255], [128, 129, 300, 17]),
     "behind": ([1500, 3], [200, 257]),
+    "far behind": ([6000, 0, 2500], [3, 40, 90]),  # few rows behind many keys: split over the keys
+    "far alone": ([9001], [2]),
 }
 
 
@@ -473,8 +475,13 @@ def test_c_refusals():
     assert call(wsb=L.pkv_decode_int8_workspace_bytes(14, 64) - 1) == _lib.ERR_WORKSPACE_TOO_SMALL
     assert call(ws=ctypes.c_void_p(0x1004)) == _lib.ERR_MISALIGNED
     assert call(d=32, qs=896) == call(bs=24) == _lib.ERR_UNSUPPORTED
-    assert L.pkv_decode_int8_workspace_bytes(0, 64) == 0 and L.pkv_prefill_int8_scratch_bytes(1, 0, 2, 64, 16, 1) == 0
-    assert L.pkv_prefill_int8_scratch_bytes(2, 9, 2, 64, 16, 1) == 2 * 2 * 256 * 2 * 64 * 2
+    assert L.pkv_decode_int8_workspace_bytes(0, 64) == 0 and L.pkv_prefill_int8_scratch_bytes(1, 5, 0, 14, 2, 64, 16, 1) == 0
+    # K and V rows of two sequences, 9 blocks of 16 rounded up to 256 rows; no splitting of fp32 rows
+    assert L.pkv_prefill_int8_scratch_bytes(2, 9, 9, 14, 2, 64, 16, 0) == 2 * 2 * 256 * 2 * 64 * 4
+    assert L.pkv_prefill_int8_scratch_bytes(2, 9, 9, 14, 2, 64, 16, 1) == 2 * 2 * 256 * 2 * 64 * 2
+    # long ones in 16-bit types also get room for the parts of a split
+    assert L.pkv_prefill_int8_scratch_bytes(2, 9, 512, 14, 2, 64, 16, 0) == 2 * 2 * 8192 * 2 * 64 * 4
+    assert L.pkv_prefill_int8_scratch_bytes(2, 9, 512, 14, 2, 64, 16, 1) > 2 * 2 * 8192 * 2 * 64 * 2
     pre = dict(out=FAKE, os=896, q=FAKE, qs=896, kp=FAKE, vp=FAKE, ksc=FAKE, vsc=FAKE, nb=64, tables=FAKE, bts=8, width=8, qsl=FAKE,
                prior=FAKE, n=2, T=5, hq=14, hkv=2, d=64, bs=16, scale=0.125, dt=1, sc=FAKE, scb=1 << 30, err=None, stream=None)
 
