@@ -598,7 +598,8 @@ int pkv_build_step_tables(int32_t* block_tables, int64_t block_table_stride, int
  * power of two s = 2^e, e >= -120, with absmax <= 127 s over the block's rows of
  * that head; byte = x / s rounded to nearest even; value = byte * s (exact in
  * fp16 range, bf16 and fp32).  Infinities are stored as +-127 and NaN as 0, and
- * neither enters absmax.  q, out and new rows are in `dtype` (fp32, fp16 or
+ * neither enters absmax.  In fp16, rows of more than 65,024 in magnitude may come
+ * back as infinities (64 * 1,024 is past 65,504).  q, out and new rows are in `dtype` (fp32, fp16 or
  * bf16).  head_dim 64 or 128, block_size a multiple of 16, pools 16-byte aligned
  * (else PKV_ERR_UNSUPPORTED / PKV_ERR_MISALIGNED).
  */
@@ -658,7 +659,7 @@ size_t pkv_prefill_int8_scratch_bytes(int n_seqs, int n_tokens, int max_blocks_p
 /* pkv_paged_prefill_attention over such pools (the chunk already appended): query
  * i of sequence s sees keys 0 .. num_prior[s] + i.  One pass lays the visible
  * rows out in the scratch (256-byte aligned), then the packed attention runs over
- * it.  scale > 0. */
+ * it.  scale > 0; out must not overlap q. */
 int pkv_paged_prefill_attention_int8(void* out, int64_t out_row_stride, const void* q,
                                      int64_t q_row_stride, const void* k_pool, const void* v_pool,
                                      const float* k_scale, const float* v_scale, int num_blocks,
@@ -676,9 +677,10 @@ int pkv_paged_prefill_attention_int8(void* out, int64_t out_row_stride, const vo
  * Qwen2Model._attention (mini_engine/model/qwen2.py:98-128) for callers that
  * score prompts.  q, out [n_tokens][n_q_heads][head_dim], k, v
  * [n_tokens][n_kv_heads][head_dim] with row strides in elements (views of one
- * fused projection will do); out must not overlap k or v.  head_dim 64 or 128,
- * scale > 0.  Rows past query_start_loc[n_seqs] are neither read nor written.  A
- * key that a row must not see never enters it, whatever it holds.
+ * fused projection will do); out must not overlap q, k or v.  head_dim 64 or 128,
+ * scale > 0.  Rows before query_start_loc[0] and past query_start_loc[n_seqs] are
+ * not written and enter no result.  A key that a row must not see never enters
+ * it, whatever it holds.
  */
 int pkv_packed_prompt_attention(void* out, int64_t out_row_stride, const void* q,
                                 int64_t q_row_stride, const void* k, int64_t k_row_stride,

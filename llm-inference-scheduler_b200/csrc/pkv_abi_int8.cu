@@ -254,6 +254,7 @@ int pkv_paged_prefill_attention_int8(void* out, int64_t out_row_stride, const vo
   if (scratch_bytes < sc.total) return PKV_ERR_WORKSPACE_TOO_SMALL;
   if (!aligned(scratch, 256) || !aligned(q, size_of(dtype)) || !aligned(out, size_of(dtype)))
     return PKV_ERR_MISALIGNED;
+  if (out == q) return PKV_ERR_UNSUPPORTED;  // a row may be read again after its first store
   Int8LayArgs y{};
   y.k_pool = k_pool;
   y.v_pool = v_pool;
@@ -326,6 +327,7 @@ int pkv_packed_prompt_attention(void* out, int64_t out_row_stride, const void* q
   if (head_dim != 64 && head_dim != 128) return PKV_ERR_UNSUPPORTED;
   const int es = size_of(dtype);
   if (!aligned(out, es) || !aligned(q, es) || !aligned(k, es) || !aligned(v, es)) return PKV_ERR_MISALIGNED;
+  if (out == q || out == k || out == v) return PKV_ERR_UNSUPPORTED;  // rows are read again after a first store
   PackedArgs a{};
   a.out = out;
   a.q = q;

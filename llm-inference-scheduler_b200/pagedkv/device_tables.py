@@ -73,7 +73,9 @@ class DeviceStepTables:
         prior = self.lens_dev
         st = ops.build_step_tables(self.tables, self.free_blocks, self.n_free, prior, new_dev, bs, T, err=self.mgr.err)
         meta = StepMetadata(
-            seq_ids=list(range(self.n_seqs)), num_new=list(num_new), num_prior=self.lens, n_tokens=T,
+            # no sequence of a cache has such an id: its lengths stay as they are even
+            # if a layer is told to advance them
+            seq_ids=[-1 - i for i in range(self.n_seqs)], num_new=list(num_new), num_prior=self.lens, n_tokens=T,
             n_decode=nd, max_query_len=max(num_new[nd:], default=0), slot_mapping=st.slot_mapping,
             block_tables=self.tables, context_lens=st.context_lens,
             # relative to the rows behind the decode sequences' one each
