@@ -417,13 +417,16 @@ __global__ void __launch_bounds__(kLayThreads) lay_out_int8_kernel(const Int8Lay
   constexpr int kPer = 16 / sizeof(T);               // elements of a 16-byte store
   const int pitch = a.n_kv_heads * a.head_dim;       // elements of a row
   const int chunks = 16 * pitch / kPer;              // stores of a group, K or V
-  const int parts = (chunks + 32 * kLayLoads - 1) / (32 * kLayLoads);  // warps of a group, K or V
-  const int64_t n_work = (keys + 127) / 128 * 8 * 2 * parts;           // 16-row groups x K, V x parts
-  for (int64_t w = static_cast<int64_t>(blockIdx.x) * (kLayThreads / 32) + (threadIdx.x >> 5); w < n_work;
-       w += static_cast<int64_t>(gridDim.x) * (kLayThreads / 32)) {
-    const int part = static_cast<int>(w % parts);
-    const bool isv = (w / parts) & 1;
-    const int64_t row0 = w / (2 * parts) * 16;
+  const unsigned parts = (chunks + 32 * kLayLoads - 1) / (32 * kLayLoads);  // warps of a group, K or V
+  // 16-row groups x K, V x parts, of 4 KB each: 2^31 of them would be 8 TB
+  const unsigned n_work = static_cast<unsigned>((keys + 127) / 128) * 16 * parts;
+  const int per_head = (a.head_dim == 64 ? 64 : 128) / kPer;               // stores of a row of a head
+  const int head_step = 32 / per_head % a.n_kv_heads;                      // heads that 32 stores go on by
+  for (unsigned w = blockIdx.x * (kLayThreads / 32) + (threadIdx.x >> 5); w < n_work; w += gridDim.x * (kLayThreads / 32)) {
+    const unsigned wp = parts == 1 ? w : w / parts;
+    const int part = static_cast<int>(w - wp * parts);
+    const bool isv = wp & 1;
+    const int row0 = static_cast<int>(wp >> 1) * 16;
     int id = -1;
     if (row0 < keys) {
       id = a.block_tables[static_cast<int64_t>(s) * a.bt_stride + row0 / bs];
@@ -432,13 +435,14 @@ __global__ void __launch_bounds__(kLayThreads) lay_out_int8_kernel(const Int8Lay
         id = -1;
       }
     }
-    const int64_t left = id < 0 ? 0 : min(static_cast<int64_t>(16), keys - row0);
-    const int valid = static_cast<int>(left) * pitch / kPer;  // stores of rows that are keys
+    const int left = id < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(16), keys - row0));
+    const int valid = left * (pitch / kPer);  // stores of rows that are keys
     // 16 rows x pitch are consecutive on both sides
     const int8_t* src = static_cast<const int8_t*>(isv ? a.v_pool : a.k_pool) +
                         (static_cast<int64_t>(id < 0 ? 0 : id) * bs + row0 % bs) * pitch;
     T* dst = static_cast<T*>(isv ? a.v_out : a.k_out) + (static_cast<int64_t>(s) * a.cap + row0) * pitch;
     const float* scale = (isv ? a.v_scale : a.k_scale) + static_cast<int64_t>(id < 0 ? 0 : id) * a.n_kv_heads;
+    int head = (part * kLayLoads * 32 + lane) / per_head % a.n_kv_heads;
     uint2 u[kLayLoads];
     float sc[kLayLoads];
 #pragma unroll
@@ -449,8 +453,10 @@ __global__ void __launch_bounds__(kLayThreads) lay_out_int8_kernel(const Int8Lay
       if (c < valid) {
         if constexpr (sizeof(T) == 2) u[k] = *reinterpret_cast<const uint2*>(src + static_cast<int64_t>(c) * kPer);
         else u[k].x = *reinterpret_cast<const uint32_t*>(src + static_cast<int64_t>(c) * kPer);
-        sc[k] = scale[c * kPer % pitch / a.head_dim];
+        sc[k] = scale[head];
       }
+      head += head_step;
+      if (head >= a.n_kv_heads) head -= a.n_kv_heads;
     }
 #pragma unroll
     for (int k = 0; k < kLayLoads; ++k) {
