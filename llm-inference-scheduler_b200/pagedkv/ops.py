@@ -1058,10 +1058,13 @@ class StepTables(NamedTuple):
 def new_step_tables(n_seqs: int, n_tokens: int, device) -> StepTables:
     """Buffers of build_step_tables for up to n_seqs requests and n_tokens
     tokens, for a caller that fills the same ones every step (a captured one)."""
-    ctx, start, n_free = torch.empty(2 * n_seqs + 2, dtype=torch.int32, device=device).split(
+    # two allocations; the positions begin on a 16-byte boundary
+    ctx, start, n_free = torch.empty(2 * n_seqs + 2, dtype=torch.int32, device=device).split_with_sizes(
         (n_seqs, n_seqs + 1, 1))
-    return StepTables(ctx, start, torch.empty(n_tokens, dtype=torch.int64, device=device),
-                      torch.empty(n_tokens, dtype=torch.int64, device=device), n_free)
+    odd = n_tokens & 1
+    slot, _, pos = torch.empty(2 * n_tokens + odd, dtype=torch.int64, device=device).split_with_sizes(
+        (n_tokens, odd, n_tokens))
+    return StepTables(ctx, start, slot, pos, n_free)
 
 
 def build_step_tables(block_tables: torch.Tensor, free_blocks: torch.Tensor, n_free: torch.Tensor,
