@@ -251,8 +251,8 @@ struct PackedArgs {
   int key_cap;
   int key_limit;   // keys a sequence's table can hold
   int n_key_rows;  // rows of k / v
-  // splitting of long items over their keys (NULL: not split): zeroed counters
-  // (8 a segment) and partials for n_parts segments (packed_split_parts)
+  // splitting of long items over their keys: zeroed counters (8 a segment) and
+  // partials for n_parts segments (packed_split_parts; 0: none)
   int* part_count = nullptr;
   float* part_o = nullptr;   // 16-byte aligned
   float2* part_ml = nullptr;

@@ -330,9 +330,9 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
 // A chunk of few rows behind many cached keys would leave most SMs idle, or one of
 // them busy long after the others.  Where the caller brings room for partials,
 // items much longer than an SM's share of all key tiles are cut over their keys
-// into segments of that length, items of their own; each leaves its normalised O with its maximum and
-// sum, and the one that finishes last joins them in segment order.  16 rows
-// behind 32,768 keys (14 heads / 2 x 64): 226 us unsplit, 42 split; 512 behind
+// into segments of that length, items of their own; each leaves its normalised O
+// with its maximum and sum, and the one that finishes last joins them in segment
+// order.  16 rows behind 32,768 keys (14 heads / 2 x 64): 226 us unsplit, 42 split; 512 behind
 // 8,192: 95, 65; 16 chunks of about 500 of which two lie behind some 3,400 keys:
 // 79.7, 68.4.  Segments of half the share, of 1,024 keys at least or up to 32 an
 // item were no faster.
@@ -439,7 +439,9 @@ struct TcItem {
   int idx;       // index of this one (segment q of the same item: idx + (seg - q) n_kv_heads)
 };
 
-template <typename T, int D>
+// SPLIT: the caller brought room for partials (without it the code for them cost
+// the others 4%)
+template <typename T, int D, bool SPLIT>
 __global__ void __launch_bounds__(kTcThreads, 1)
     packed_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                      const __grid_constant__ CUtensorMap vmap, const TcParams p) {
@@ -531,11 +533,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int len = max(a.query_start_loc[tid + 1] - a.query_start_loc[tid], 0);
       order[rank] = tid;
       n_items[rank] = (min(len, a.n_tokens) + per_item - 1) / per_item;
-      if (a.part_count != nullptr) last_tiles[rank] = (key_span(a, tid, 0, len).keys + kN - 1) / kN;
+      if (SPLIT) last_tiles[rank] = (key_span(a, tid, 0, len).keys + kN - 1) / kN;
     }
     __syncthreads();
     if (warp == 0) {
-      if (a.part_count != nullptr) {
+      if (SPLIT) {
         // an SM's share of the key tiles of all items (a sequence's taken as
         // between those of its first and last) is a segment's length: there are
         // at most two SMs' worth more segments than items
@@ -569,7 +571,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       int run = 0;
       for (int b0 = 0; b0 < B; b0 += 32) {
         const int i = b0 + lane;
-        const int n = i < B ? n_items[i] * (a.part_count != nullptr ? segs_of(last_tiles[i], seg_len) : 1) : 0;
+        const int n = i < B ? n_items[i] * (SPLIT ? segs_of(last_tiles[i], seg_len) : 1) : 0;
         int x = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -596,7 +598,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     it.segs = 1;
     it.j0 = 0;
     it.j1 = INT_MAX;
-    int tile, segs = 1, last = 0;
+    int tile;
+    [[maybe_unused]] int segs = 1, last = 0;
     if (p.sorted) {
       int lo = 0, hi = B - 1;
       if (u >= first_item[B]) return false;
@@ -606,7 +609,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       it.s = order[lo];
       tile = first_item[lo + 1] - 1 - u;  // last tokens first
-      if (a.part_count != nullptr) {
+      if (SPLIT) {
         last = last_tiles[lo];
         segs = segs_of(last, seg_len);
         it.seg = tile % segs;
@@ -650,8 +653,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     bool ok = mbar_wait(&item_full[sl], (k >> 1) & 1);
     ok = __all_sync(0xffffffffu, ok);
     const int* w = items + sl * kTcItemInts;
-    it.s = w[0], it.g = w[1], it.tok0 = w[2], it.q_begin = w[3], it.n_new = w[4], it.prior = w[5], it.keys = w[6], it.row0 = w[7], it.j0 = w[8], it.j1 = w[9];
-    it.seg = w[10] & 255, it.segs = w[10] >> 8, it.idx = w[11];
+    it.s = w[0], it.g = w[1], it.tok0 = w[2], it.q_begin = w[3], it.n_new = w[4], it.prior = w[5], it.keys = w[6], it.row0 = w[7];
+    if constexpr (SPLIT) it.j0 = w[8], it.j1 = w[9], it.seg = w[10] & 255, it.segs = w[10] >> 8, it.idx = w[11];
     __syncwarp();
     if (lane == 0) mbar_arrive(&item_empty[sl]);
     if (!ok && lane == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
@@ -664,7 +667,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     return n > 0 ? min(it.prior + t0 + n, it.keys) : 0;
   };
   // key tiles of tile x in this item (segment)
-  auto item_tiles = [&](const TcItem& it, int x) { return max(0, min((tile_keys(it, x) + kN - 1) / kN, it.j1) - it.j0); };
+  auto item_tiles = [&](const TcItem& it, int x) {
+    const int n = (tile_keys(it, x) + kN - 1) / kN;
+    return SPLIT ? max(0, min(n, it.j1) - it.j0) : n;
+  };
 
   if (warp >= 8) {
     setmaxnreg_dec<kTcRegsOther>();
@@ -701,7 +707,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           int* w = items + sl * kTcItemInts;
           w[0] = it.s, w[1] = it.g, w[2] = have ? it.tok0 : -1, w[3] = it.q_begin, w[4] = it.n_new, w[5] = it.prior, w[6] = it.keys,
-          w[7] = it.row0, w[8] = it.j0, w[9] = it.j1, w[10] = it.seg | (it.segs << 8), w[11] = it.idx;
+          w[7] = it.row0;
+          if constexpr (SPLIT) w[8] = it.j0, w[9] = it.j1, w[10] = it.seg | (it.segs << 8), w[11] = it.idx;
           mbar_arrive(&item_full[sl]);
           if (!have) break;
         }
@@ -744,7 +751,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
               for (int h = 0; h < kHalves; ++h)
                 tma_load_3d(base + (kv ? Sh::kOffV : Sh::kOffK) + st * Sh::kKTile + h * Sh::kKHalf, kv ? &vmap : &kmap, full, h * 64, it.g,
-                            it.row0 + (it.j0 + j) * kN);
+                            it.row0 + ((SPLIT ? it.j0 : 0) + j) * kN);
             }
             __syncwarp();
           }
@@ -893,7 +900,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_wait_ld_regs(sr[0]);
 #pragma unroll
         for (int c4 = 1; c4 < kN / 32; ++c4) reg_after_wait(sr[c4]);
-        const int kbase = (it.j0 + j) * kN;
+        const int kbase = ((SPLIT ? it.j0 : 0) + j) * kN;
         if (kbase + kN > lim) {
 #pragma unroll
           for (int c = 0; c < kN; ++c)
@@ -982,7 +989,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       };
       // partials of segment q: four columns of a tile's 128 rows side by side
       auto part_slot = [&](int q) { return static_cast<int64_t>(it.idx + (it.seg - q) * a.n_kv_heads) * 2 + x; };
-      const bool whole = it.segs == 1;
+      const bool whole = !SPLIT || it.segs == 1;
       if (ntx > 0) {
         wait_pv(ntx - 1);
         __syncwarp();
@@ -1107,9 +1114,9 @@ int64_t tc_items(int n_seqs, int n_tokens, int n_q_heads, int n_kv_heads) {
   return (n_tokens / (2 * tokens) + static_cast<int64_t>(n_seqs)) * n_kv_heads;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool SPLIT>
 cudaError_t launch_tc(const PackedArgs& a, cudaStream_t stream) {
-  auto kern = packed_tc_kernel<T, D>;
+  auto kern = packed_tc_kernel<T, D, SPLIT>;
   static std::atomic<int> ready[64];  // per device: 0 not asked, SMs: ready, -1 the register split does not fit
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -1134,7 +1141,6 @@ cudaError_t launch_tc(const PackedArgs& a, cudaStream_t stream) {
   p.tokens = kTcM / p.group;
   p.sorted = a.n_seqs <= kTcMaxSorted;
   p.n_sms = state;
-  if (a.n_parts == 0) p.a.part_count = nullptr;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   CUtensorMap qm, km, vm;
   int rc = encode_rows_tensormap(&qm, a.q, a.q_stride, a.n_tokens, a.n_q_heads, D, a.dtype, p.group, p.tokens);
@@ -1143,7 +1149,7 @@ cudaError_t launch_tc(const PackedArgs& a, cudaStream_t stream) {
   if (rc != 0) return cudaErrorNotSupported;
   int64_t items = tc_items(a.n_seqs, a.n_tokens, a.n_q_heads, a.n_kv_heads);
   if (items > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  if (p.a.part_count != nullptr) items = a.n_parts;
+  if (SPLIT) items = a.n_parts;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(items));
   cfg.blockDim = dim3(kTcThreads);
@@ -1174,7 +1180,10 @@ cudaError_t launch_packed_attention(const PackedArgs& a, cudaStream_t stream) {
   auto go = [&](auto tag) {
     using T = decltype(tag);
     if constexpr (sizeof(T) == 2) {
-      if (tc_supported(a)) return a.head_dim == 64 ? launch_tc<T, 64>(a, stream) : launch_tc<T, 128>(a, stream);
+      if (tc_supported(a)) {
+        if (a.n_parts > 0) return a.head_dim == 64 ? launch_tc<T, 64, true>(a, stream) : launch_tc<T, 128, true>(a, stream);
+        return a.head_dim == 64 ? launch_tc<T, 64, false>(a, stream) : launch_tc<T, 128, false>(a, stream);
+      }
     }
     return a.head_dim == 64 ? launch_cores<T, 64>(a, stream) : launch_cores<T, 128>(a, stream);
   };
