@@ -34,8 +34,12 @@
 // that several CTAs share in the workspace, joined in CTA order by a second
 // launch.
 //
-// What bounds it: instructions.  At 256 sequences of about 1,024 tokens (14 / 2
-// heads, 74 MB) the bytes take 11.3 us at the copy rate.
+// What bounds it: HBM where heads are wide (64 sequences of 4,096 tokens, 32 / 8 x
+// 128: 92.9 us, 5.8 TB/s of 6.5 measured for a copy), the instructions of the two
+// kinds of tiles at 64 dims and 7 query heads a KV head (64 x 8,192 tokens, 14 / 2
+// x 64: 33.0 us, 4.1 TB/s), and for small steps the fixed part: about 2 us to the
+// first tile, 1.3 for the join in the CTA, 2.5 for the second launch (256 x 1,024:
+// 22.3 us for 67 MB; one sequence of 131,072: 15.7 us for 34 MB; of 16: 5.5 us).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -592,6 +596,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 // are on their way (running sums, four at a time, took 2.5 us more of 131,072
 // tokens' 15.7).  Empty sequences get zeros.  The lengths are read while the
 // decode kernel runs (it starts this one after its own wait for them).
+//
+// Up to kM8Few partials a thread takes all of them for its dims (256 x 1,024
+// tokens: 22.3 us; 37.9 with the other way for all, 24.9 with this way for up to
+// 16).
 constexpr int kM8Threads = 256, kM8Few = 6, kM8Ahead = 10;
 template <typename T, int D>
 __global__ void __launch_bounds__(kM8Threads) merge_int8_kernel(const D8Params p, int grid, int heads_per) {
@@ -802,7 +810,9 @@ cudaError_t launch_d8(const AttnArgs& a, const CUtensorMap* kmap, const CUtensor
 template <typename T>
 cudaError_t launch_d8_t(const AttnArgs& a, const CUtensorMap* km, const CUtensorMap* vm, void* ws, cudaStream_t stream) {
   // query heads per warp: 8, or 16 where the group has more (V's fragments are
-  // then converted once for both halves)
+  // then converted once for both halves).  64 sequences of 4,096 tokens with 8 and
+  // with 16: 14 / 2 x 64 21.6 and 31.8 us, 32 / 8 x 128 93 and 131; 32 / 2 x 128
+  // 46.5 and 44.5, 16 / 1 x 128 in fp32 33.1 and 30.9
   const bool two = a.n_q_heads / a.n_kv_heads > 8;
   constexpr bool f32 = std::is_same<T, float>::value;
   if (a.head_dim == 64)

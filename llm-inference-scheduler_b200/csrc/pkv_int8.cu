@@ -24,7 +24,9 @@
 // floor(n / b) + 2 bounds it, so sequence i's units start at
 // floor(start_i / b) + 2 i and a warp finds its sequence by a search on the
 // start positions: no prefix pass, no scratch.  Bound by the bytes of the
-// rows for prompts, by launch and round trips for decode steps.
+// rows for prompts (64 of 200 to 2,000 tokens, 8 x 128 in bf16, appended and
+// fetched: 460 MB in 108 us, 65% of the copy rate), by launch and round trips for
+// decode steps (256 single tokens, 2 x 64: 3.9 us, 7.1 with the fetch).
 #include <type_traits>
 
 #include "pkv_common.cuh"
@@ -398,7 +400,10 @@ __global__ void __launch_bounds__(kI8Warps * 32) fetch_int8_kernel(const Int8Row
 // the next multiple of 128 (the attention kernel's key tile): a tile holds no
 // stale bytes.  A warp takes up to kLayLoads stores a lane of a 16-row group's K or V at
 // a time, all its loads ahead of them.
-// Also clears the counters of the attention behind it.
+// Also clears the counters of the attention behind it.  Bound by the bytes for
+// long ones (64-bit divisions for every unit and a head index by division for
+// every load had made 32 sequences of 4,064 keys, 8 x 128, 109 us slower), by four
+// dependent round trips for short ones.
 constexpr int kLayThreads = 256, kLayLoads = 8;
 template <typename T>
 __global__ void __launch_bounds__(kLayThreads) lay_out_int8_kernel(const Int8LayArgs a) {
@@ -481,6 +486,8 @@ __global__ void __launch_bounds__(kLayThreads) lay_out_int8_kernel(const Int8Lay
 template <typename K>
 cudaError_t launch_rows(K f16, K bf16, K f32, Int8RowsArgs a, cudaStream_t stream) {
   // one head a warp while that leaves the SMs' warp slots short, up to four beyond
+  // (append of 64 prompts of 1,000 tokens, 8 x 128: 83.1 us with one, 68.4 with
+  // four; of 256 single tokens, 2 x 64: 3.9 and 4.8)
   const int64_t each = a.n_units * 2 * a.n_kv_heads;
   a.heads_per_warp = each < 32768 ? 1 : each < 65536 ? 2 : 4;
   if (a.heads_per_warp > a.n_kv_heads) a.heads_per_warp = a.n_kv_heads;

@@ -1,6 +1,13 @@
 // pkv_packed.cu -- causal attention with grouped heads over consecutive rows:
 // whole prompts packed one behind the other, or chunks behind cached keys that
 // were laid out row by row.
+//
+//   x_ij = scale q_i . k_j,  j <= prior + i,  o_i = sum_j softmax(x_i)_j v_j
+//
+// in one pass over the keys with a running maximum and sum (fp32).  fp16 and bf16
+// rows that TMA can read take the tensor-core tiles (packed_tc_kernel), fp32 rows
+// and those at other strides or alignments, or of more than 64 query heads to a
+// KV head, the CUDA-core tiles (packed_cores_kernel).
 #include <float.h>
 #include <limits.h>
 
@@ -98,7 +105,10 @@ __device__ __forceinline__ void pk_copy16(void* dst, const void* src, bool on) {
 // A thread takes 4 rows x 4 keys of S (keys tx + 16 c) and 4 rows x 4 (or 2 x 4)
 // dims of O, two products an instruction (the paired fp32 FMA): 8 16-byte reads
 // of shared memory for 32 of them, in both.  fp32 rows on 16-byte boundaries come
-// by cp.async, a key tile ahead; other rows element by element.
+// by cp.async, a key tile ahead; other rows element by element.  Bound by those
+// reads and the FMAs: 29 TFLOP/s for long fp32 prompts; three short ones (250, 17
+// and 93 tokens, 14 / 2 x 64) take 32 us, the four key tiles of the longest row
+// tile one after the other.
 template <typename T, int D>
 __global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedArgs a, int wide) {
   extern __shared__ __align__(16) float pk_smem[];
@@ -336,6 +346,12 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
 // 8,192: 95, 65; 16 chunks of about 500 of which two lie behind some 3,400 keys:
 // 79.7, 68.4.  Segments of half the share, of 1,024 keys at least or up to 32 an
 // item were no faster.
+//
+// What bounds it: at 64 dims the exponentials, two for every 128 FLOP of MMA (a
+// third of them are polynomials on the FMA pipe), at 128 dims the S -> P -> O chain
+// of short items.  One prompt of 16,384 tokens: 878 TFLOP/s (14 / 2 x 64), 1,218
+// (32 / 8 x 128); four of up to 8,191 tokens, 14 / 2 x 64: 180 us, 673 TFLOP/s;
+// twelve of up to 2,048, 32 / 8 x 128: 227 us, 804 TFLOP/s.
 //
 // Items are handed out while the kernel runs: a CTA starts with its own block
 // index and then takes the indices of blocks that have not started
