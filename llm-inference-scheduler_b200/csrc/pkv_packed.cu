@@ -106,8 +106,8 @@ __device__ __forceinline__ void pk_copy16(void* dst, const void* src, bool on) {
 // dims of O, two products an instruction (the paired fp32 FMA): 8 16-byte reads
 // of shared memory for 32 of them, in both.  fp32 rows on 16-byte boundaries come
 // by cp.async, a key tile ahead; other rows element by element.  Bound by those
-// reads and the FMAs: 29 TFLOP/s for long fp32 prompts; three short ones (250, 17
-// and 93 tokens, 14 / 2 x 64) take 32 us, the four key tiles of the longest row
+// reads and the FMAs: 28 TFLOP/s for long fp32 prompts; three short ones (250, 17
+// and 93 tokens, 14 / 2 x 64) take 28 us, the four key tiles of the longest row
 // tile one after the other.
 template <typename T, int D>
 __global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedArgs a, int wide) {
@@ -343,13 +343,13 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
 // into segments of that length, items of their own; each leaves its normalised O
 // with its maximum and sum, and the one that finishes last joins them in segment
 // order.  16 rows behind 32,768 keys (14 heads / 2 x 64): 226 us unsplit, 42 split; 512 behind
-// 8,192: 95, 65; 16 chunks of about 500 of which two lie behind some 3,400 keys:
-// 79.7, 68.4.  Segments of half the share, of 1,024 keys at least or up to 32 an
-// item were no faster.
+// 8,192: 95, 63; 16 chunks of about 500 of which two lie behind some 3,400 keys:
+// 79.7, 68.0 (with the laying out of the rows).  Segments of half the share, of
+// 1,024 keys at least or up to 32 an item were no faster.
 //
-// What bounds it: at 64 dims the exponentials, two for every 128 FLOP of MMA (a
+// What bounds it: at 64 dims the exponentials, one for every 256 FLOP of MMA (a
 // third of them are polynomials on the FMA pipe), at 128 dims the S -> P -> O chain
-// of short items.  One prompt of 16,384 tokens: 878 TFLOP/s (14 / 2 x 64), 1,218
+// of short items.  One prompt of 16,384 tokens: 886 TFLOP/s (14 / 2 x 64), 1,245
 // (32 / 8 x 128); four of up to 8,191 tokens, 14 / 2 x 64: 180 us, 673 TFLOP/s;
 // twelve of up to 2,048, 32 / 8 x 128: 227 us, 804 TFLOP/s.
 //
