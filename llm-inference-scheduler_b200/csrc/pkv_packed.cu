@@ -121,10 +121,11 @@ __global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedAr
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
-  const int h = blockIdx.y, g = h / (a.n_q_heads / a.n_kv_heads);
+  const unsigned back = gridDim.x - 1 - blockIdx.x, u = back / static_cast<unsigned>(a.n_q_heads);
+  const int h = static_cast<int>(back - u * a.n_q_heads), g = h / (a.n_q_heads / a.n_kv_heads);
   int s, tile;
-  // the last tiles (the longest of a sequence) first
-  if (!find_tile(a, static_cast<int64_t>(gridDim.x) - 1 - blockIdx.x, kPkM, s, tile)) return;
+  // the last tiles (the longest of a sequence) first, all heads of one together
+  if (!find_tile(a, u, kPkM, s, tile)) return;
   const int q_begin = a.query_start_loc[s], n_new = a.query_start_loc[s + 1] - q_begin;
   const KeySpan span = key_span(a, s, q_begin, n_new);
   const int q0 = tile * kPkM, rows = min(kPkM, n_new - q0);
@@ -292,7 +293,8 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   const int64_t tiles = a.n_tokens / kPkM + static_cast<int64_t>(a.n_seqs);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles), a.n_q_heads);
+  if (tiles * a.n_q_heads > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * a.n_q_heads));
   cfg.blockDim = dim3(kPkThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;

@@ -1023,13 +1023,21 @@ def _call(name: str, dev: int, *args) -> None:
 def _one_device(names: str, *tensors) -> int:
     """The CUDA device index that all tensors are on (None entries aside);
     `names` says what they are, in order, for the error."""
-    dev = tensors[0].get_device() if isinstance(tensors[0], torch.Tensor) else -1
-    for t in tensors:
-        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != dev or dev < 0):
-            for n, o in zip(names.split(), tensors):
-                if o is not None and _cuda(o, n).get_device() != dev:
-                    raise ValueError(f"pagedkv: `{n}` is on {o.device}, expected cuda:{dev}")
-    return dev
+    dev = -1
+    try:
+        dev = tensors[0].get_device()
+        for t in tensors:
+            if t is not None and t.get_device() != dev:
+                break
+        else:
+            if dev >= 0:
+                return dev
+    except AttributeError:  # not a tensor
+        pass
+    for n, o in zip(names.split(), tensors):
+        if o is not None and _cuda(o, n).get_device() != dev:
+            raise ValueError(f"pagedkv: `{n}` is on {o.device}, expected cuda:{dev}")
+    raise TypeError("pagedkv: a CUDA tensor is needed")
 
 
 def _check_err(err: torch.Tensor | None) -> None:
