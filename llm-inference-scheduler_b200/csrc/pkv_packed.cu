@@ -106,9 +106,11 @@ __device__ __forceinline__ void pk_copy16(void* dst, const void* src, bool on) {
 // dims of O, two products an instruction (the paired fp32 FMA): 8 16-byte reads
 // of shared memory for 32 of them, in both.  fp32 rows on 16-byte boundaries come
 // by cp.async, a key tile ahead; other rows element by element.  Bound by those
-// reads and the FMAs: 28 TFLOP/s for long fp32 prompts; three short ones (250, 17
-// and 93 tokens, 14 / 2 x 64) take 28 us, the four key tiles of the longest row
-// tile one after the other.
+// reads (55% of the shared-memory pipe's cycles), the FMAs (43%) and, with fewer
+// than two CTAs an SM, the latency between them: 37 TFLOP/s for a prompt of 4,096
+// tokens (14 / 2 x 64, fp32), 97 us for one of 1,000, 22 for three of 250, 17 and
+// 93.  Tiles of 32 or 16 queries were no faster for those (a key tile takes as
+// long) and up to 2.2 times slower for long ones.
 template <typename T, int D>
 __global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedArgs a, int wide) {
   extern __shared__ __align__(16) float pk_smem[];
@@ -118,7 +120,6 @@ __global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedAr
   float* kvs = qs + kTile;                  // [2 buffers][K, V][64][kLd]
   float* ps = kvs + 4 * kTile;              // [64][68] probabilities
   constexpr int kLp = kPkN + 4;
-  pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const unsigned back = gridDim.x - 1 - blockIdx.x, u = back / static_cast<unsigned>(a.n_q_heads);
@@ -245,6 +246,9 @@ __global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedAr
     }
     __syncthreads();  // the buffer is filled again next
   }
+  // (not before: the next launch's CTAs would share the SMs of these, two to one
+  // and none to another)
+  pdl_trigger();
   bool fine[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
