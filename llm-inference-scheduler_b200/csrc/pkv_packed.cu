@@ -361,8 +361,12 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
 //
 // Items are handed out while the kernel runs: a CTA starts with its own block
 // index and then takes the indices of blocks that have not started
-// (clusterlaunchcontrol.try_cancel), one item ahead, so tensor memory, barriers
-// and the item order are set up once per SM.  Indices run from the sequences with
+// (clusterlaunchcontrol.try_cancel), each once the item before has issued its last
+// loads: four key tiles of work hide the latency, and no CTA holds an item that
+// another could start (two
+// items ahead, as two slots allow: four prompts of 4,096 tokens, 8 / 8 x 64, 164 us
+// against 115; eight of 2,048, 32 / 8 x 128, 321 against 261).  So tensor memory, barriers and the
+// item order are set up once per SM.  Indices run from the sequences with
 // the most keys to those with the fewest, the last tokens of each first.
 constexpr int kTcM = 128, kTcThreads = 384;
 constexpr int kTcProducerWarp = 8, kTcQkWarp = 9, kTcSchedWarp = 10;  // warp 11: O
@@ -387,8 +391,8 @@ template <int D> struct TcShape {
   static constexpr int kOffV = kOffK + kStages * kKTile;
   static constexpr int kOffBar = kOffV + kStages * kKTile;
   // q_full, q_empty, K and V full / empty [stages], S full [2 tiles][bufs], P full and S free [bufs],
-  // o_done [2 tiles][bufs], item_full, item_empty [2], clc
-  static constexpr int kBars = 2 + 4 * kStages + 6 * kBufs + 4 + 1;
+  // o_done [2 tiles][bufs], item_full, item_empty [2], clc, loaded
+  static constexpr int kBars = 2 + 4 * kStages + 6 * kBufs + 4 + 1 + 1;
   static constexpr int kOffClc = (kOffBar + kBars * 8 + 15) / 16 * 16;
   static constexpr int kOffItem = kOffClc + 16;
   static constexpr int kOffTmem = kOffItem + 2 * kTcItemInts * 4;
@@ -488,6 +492,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* item_full = o_done + 2 * kBufs;
   uint64_t* item_empty = item_full + 2;
   uint64_t* clc_bar = item_empty + 2;
+  uint64_t* loaded = clc_bar + 1;  // an item's last K / V tile is on its way
   int* items = reinterpret_cast<int*>(base + Sh::kOffItem);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + Sh::kOffTmem);
   int* order = reinterpret_cast<int*>(base + Sh::kOffOrder);
@@ -519,6 +524,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&item_empty[i], 11);  // 8 softmax warps, producer, two issuers
     }
     mbar_init(clc_bar, 1);
+    mbar_init(loaded, 1);
     fence_barrier_init();
   }
   if (warp == kTcQkWarp) tmem_alloc(tmem_slot, kTcTmemCols);
@@ -705,6 +711,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int k = 0;; ++k) {
           TcItem it;
           bool have = false;
+          // taken late, so that a CTA with a long item leaves the next one to others
+          if (k >= 1 && more && !mbar_wait(loaded, (k - 1) & 1)) {
+            raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
+            more = false;
+          }
           while (more) {
             if (idx >= 0) have = find_item(idx, it);
             if (have) break;
@@ -780,6 +791,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (dead) break;
         }
         if (dead) break;
+        if (lane == 0) mbar_arrive(loaded);
       }
     } else {
       // ======================= MMA issuers (warp 9: S, warp 11: O) =======================
