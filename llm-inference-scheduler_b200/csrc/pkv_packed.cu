@@ -348,16 +348,17 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
 // items much longer than an SM's share of all key tiles are cut over their keys
 // into segments of that length, items of their own; each leaves its normalised O
 // with its maximum and sum, and the one that finishes last joins them in segment
-// order.  16 rows behind 32,768 keys (14 heads / 2 x 64): 226 us unsplit, 42 split; 512 behind
-// 8,192: 95, 63; 16 chunks of about 500 of which two lie behind some 3,400 keys:
-// 79.7, 68.0 (with the laying out of the rows).  Segments of half the share, of
-// 1,024 keys at least or up to 32 an item were no faster.
+// order.  16 rows behind 32,768 keys (14 heads / 2 x 64): 226 us unsplit, 42 split
+// (38 by now); 512 behind 8,192: 95, 63 (53); 16 chunks of about 500 of which two
+// lie behind some 3,400 keys: 79.7, 68.0 (58).  All with the laying out of the rows.
+// Segments of half the share, of 1,024 keys at least or up to 32 an item were no
+// faster.
 //
 // What bounds it: at 64 dims the exponentials, one for every 256 FLOP of MMA (a
 // third of them are polynomials on the FMA pipe), at 128 dims the S -> P -> O chain
-// of short items.  One prompt of 16,384 tokens: 886 TFLOP/s (14 / 2 x 64), 1,245
-// (32 / 8 x 128); four of up to 8,191 tokens, 14 / 2 x 64: 180 us, 673 TFLOP/s;
-// twelve of up to 2,048, 32 / 8 x 128: 227 us, 804 TFLOP/s.
+// of short items.  One prompt of 16,384 tokens: 933 TFLOP/s (14 / 2 x 64), 1,308
+// (32 / 8 x 128); four of up to 8,191 tokens, 14 / 2 x 64: 164 us, 738 TFLOP/s;
+// twelve of up to 2,048, 32 / 8 x 128: 218 us, 837 TFLOP/s.
 //
 // Items are handed out while the kernel runs: a CTA starts with its own block
 // index and then takes the indices of blocks that have not started
@@ -365,7 +366,7 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
 // loads: four key tiles of work hide the latency, and no CTA holds an item that
 // another could start (two
 // items ahead, as two slots allow: four prompts of 4,096 tokens, 8 / 8 x 64, 164 us
-// against 115; eight of 2,048, 32 / 8 x 128, 321 against 261).  So tensor memory, barriers and the
+// against 115; of up to 8,191, 14 / 2 x 64, 180 against 164).  So tensor memory, barriers and the
 // item order are set up once per SM.  Indices run from the sequences with
 // the most keys to those with the fewest, the last tokens of each first.
 constexpr int kTcM = 128, kTcThreads = 384;
