@@ -650,9 +650,9 @@ int pkv_paged_decode_attention_int8(void* out, int64_t out_row_stride, const voi
                                     int block_size, float scale, int dtype, void* workspace,
                                     size_t workspace_bytes, int* err_flags, pkv_stream_t stream);
 
-/* Scratch of the chunked prefill below (any initial contents): the visible rows of
- * every sequence as values and, for calls of few rows, the partial results of work
- * split over the keys. */
+/* Scratch of the chunked prefill below (any initial contents, one call at a time):
+ * the visible rows of every sequence as values and, for calls of few rows, the
+ * partial results of work split over the keys. */
 size_t pkv_prefill_int8_scratch_bytes(int n_seqs, int n_tokens, int max_blocks_per_seq, int n_q_heads,
                                       int n_kv_heads, int head_dim, int block_size, int dtype);
 

@@ -213,3 +213,27 @@ def test_in_place_outputs_are_refused():
     tables, pools, _ = chunk_call([20], 16, 14, 2, 64, torch.float16, 1)
     with pytest.raises(_lib.PagedKVError):
         ops.paged_prefill_attention_int8(q, *[t.cuda() for t in pools], ints(tables), ints([0, 20]), ints([0]), 20, 0.125, out=q)
+
+
+@pytest.mark.gpu
+def test_split_chunks_flag_bad_layouts():
+    """Starts that go back or pass the rows, lengths past the tables: flagged, and a good call after them is right."""
+    bs, hq, hkv, d = 16, 14, 2, 64
+    tables, pools, q = chunk_call([5030, 20, 5030], bs, hq, hkv, d, torch.float16, 50)
+    dev, qd, tab = [t.cuda() for t in pools], q.cuda(), ints(tables)
+    need = ops.prefill_int8_scratch_bytes(3, 50, tab.shape[1], hq, hkv, d, bs, torch.float16)
+    scratch = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    err = ops.new_error_flags("cuda")
+
+    def call(starts, prior):
+        err.zero_()
+        out = ops.paged_prefill_attention_int8(qd, *dev, tab, ints(starts), ints(prior), 50, 0.125, err=err, scratch=scratch)
+        return out, int(err)
+
+    good, flags = call([0, 20, 20, 50], [5000, 0, 5000])
+    assert flags == 0
+    assert call([0, 30, 20, 50], [5000, 0, 5000])[1] & _lib.FLAG_BAD_QUERY_LAYOUT
+    assert call([0, 20, 20, 70], [5000, 0, 5000])[1] & _lib.FLAG_BAD_QUERY_LAYOUT
+    assert call([0, 20, 20, 50], [2 ** 30, 0, 5000])[1] & _lib.FLAG_CONTEXT_EXCEEDS_TABLE
+    again, flags = call([0, 20, 20, 50], [5000, 0, 5000])
+    assert flags == 0 and torch.equal(again, good)
