@@ -44,7 +44,8 @@ __device__ __forceinline__ KeySpan key_span(const PackedArgs& a, int s, int q_be
 // arithmetic, untouched by any key it must not see.  The tiled kernels multiply
 // masked keys by a probability of zero, which is not zero where such a key's V
 // holds an infinity or NaN; a row that comes out not finite is computed again
-// here (and stays so if its own keys make it so).
+// here (and stays so if its own values make it so).  Not where its sum is NaN
+// already: masked scores never enter that, so its own q or keys made it so.
 template <typename T, int D>
 __device__ __noinline__ void packed_row_alone(const PackedArgs& a, int64_t row, int h, int64_t key0, int lim) {
   const int lane = threadIdx.x & 31, g = h / (a.n_q_heads / a.n_kv_heads);
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedAr
         if (row < rows) out[64 * c + 4 * tx + i] = Elem<T>::from_f(v[i]);
       }
     }
-    fine[r] = ok || row >= rows;
+    fine[r] = ok || row >= rows || !(l[r] < INFINITY);
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -455,6 +456,13 @@ __device__ __forceinline__ int clc_index(const void* result) {
       : "r"(smem_u32(result))
       : "memory");
   return ok ? static_cast<int>(x) : -1;
+}
+
+// the largest of three, NaN if one is
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 // an item: two tiles of one (sequence, KV head), or a segment of their keys
@@ -921,6 +929,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // would send its warp through the masking code at every step)
       const int lim = row_valid ? min(it.prior + tok + 1, kvx) : INT_MAX;
       float m_used = -INFINITY, l = 0.f;
+      bool odd = false;  // a NaN or +infinity among the visible scores: the row is NaN
       for (int j = 0; j < ntx; ++j) {
         // the step's number (A(j) and B(j) alternate while both tiles have key tiles), its S buffer
         const int n = n0 + (x == 0 ? (nto > 0 ? 2 * j : j) : (j < nto ? 2 * j + 1 : nto + j));
@@ -943,14 +952,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         float m8[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) m8[q] = fmaxf(__uint_as_float(sr[0][q]), __uint_as_float(sr[0][q + 8]));
+        for (int q = 0; q < 8; ++q) m8[q] = fmax3_nan(__uint_as_float(sr[0][q]), __uint_as_float(sr[0][q + 8]), -INFINITY);
 #pragma unroll
         for (int c = 16; c < kN; c += 16) {
 #pragma unroll
           for (int q = 0; q < 8; ++q)
-            m8[q] = fmax3(m8[q], __uint_as_float(sr[c >> 5][(c & 31) + q]), __uint_as_float(sr[(c + 8) >> 5][((c + 8) & 31) + q]));
+            m8[q] = fmax3_nan(m8[q], __uint_as_float(sr[c >> 5][(c & 31) + q]), __uint_as_float(sr[(c + 8) >> 5][((c + 8) & 31) + q]));
         }
-        const float mt = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7])) * sl2;
+        const float mt = fmax3_nan(fmax3_nan(m8[0], m8[1], m8[2]), fmax3_nan(m8[3], m8[4], m8[5]), fmax3_nan(m8[6], m8[7], -INFINITY)) * sl2;
+        odd = odd || !(mt < INFINITY);  // (the polynomials below would swallow a NaN)
         float factor = 1.f;
         if (mt > m_used + 8.f) {
           factor = exp2f(m_used - mt);
@@ -994,6 +1004,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_before();
         mbar_arrive(&p_full[b]);
       }
+      if (odd) l = NAN;
+      else if (m_used == -INFINITY) l = 0.f;  // nothing seen, or scores of -infinity alone
       // ---- epilogue: O / l -> out
       bool fine = true;
       const int64_t row = static_cast<int64_t>(it.q_begin) + tok;
@@ -1030,7 +1042,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         __syncwarp();
         tc_fence_after();
         const float inv = l > 0.f ? 1.f / l : l;  // NaN stays
-        float fsum = l;
+        float fsum = 0.f;
 #pragma unroll
         for (int c2 = 0; c2 < D / 32; ++c2) {
           uint32_t o[32];
@@ -1051,7 +1063,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
         tc_fence_before();  // O is read before the next item's PV (ordered by p_full)
-        if (whole) fine = !row_valid || fsum < INFINITY;
+        if (whole) fine = !row_valid || !(l < INFINITY) || (l > 0.f && fsum < INFINITY);
       }
       if (!whole) {
         // each warp on its own: its rows of all segments are in memory once their
@@ -1077,7 +1089,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             sum += w[q];
           }
           const float inv = sum > 0.f ? 1.f / sum : sum;  // NaN stays
-          float fsum = sum;
+          float fsum = 0.f;
           for (int c2 = 0; c2 < D / 32; ++c2) {
             float f[32];
 #pragma unroll
@@ -1113,7 +1125,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __syncwarp();
             store32(c2, f);
           }
-          fine = !row_valid || fsum < INFINITY;
+          fine = !row_valid || !(sum < INFINITY) || (sum > 0.f && fsum < INFINITY);
         }
       }
       cx += ntx;

@@ -237,3 +237,31 @@ def test_split_chunks_flag_bad_layouts():
     assert call([0, 20, 20, 50], [2 ** 30, 0, 5000])[1] & _lib.FLAG_CONTEXT_EXCEEDS_TABLE
     again, flags = call([0, 20, 20, 50], [5000, 0, 5000])
     assert flags == 0 and torch.equal(again, good)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d", [("f16", 64), ("bf16", 128), ("f32", 64)])
+def test_non_finite_values_of_a_rows_own(dtype, d):
+    """NaN in a key makes NaN of every later row of its sequence and heads; an infinity or
+    NaN in a value of its column there; no other row or column changes."""
+    hq, hkv, dt, starts = 6, 2, DT[dtype], [0, 90, 200]
+    x = torch.randn(200, hq + 2 * hkv, d, generator=torch.Generator().manual_seed(5)).to(dt)
+
+    def run(y):
+        y = y.cuda()
+        return ops.packed_prompt_attention(y[:, :hq], y[:, hq:hq + hkv], y[:, hq + hkv:], ints(starts), 0.125).cpu()
+
+    plain, bad = run(x), x.clone()
+    bad[40, hq, 3] = math.nan           # a key of KV head 0 in the first sequence
+    bad[130, hq + hkv + 1, 7] = math.inf  # a value of KV head 1 in the second
+    bad[150, hq + hkv + 1, 9] = math.nan
+    got, want = run(bad), plain.clone()
+    want[40:90, :3] = math.nan
+    want[130:200, 3:, 7] = math.inf
+    want[150:200, 3:, 9] = math.nan
+    nan = want.isnan()
+    assert torch.equal(got.isnan(), nan) and torch.equal(got.isinf(), want.isinf())
+    # bit for bit where no key tile holds a bad value of a key that the row must not see;
+    # rows of the second sequence are computed again on their own, within the bounds of any result
+    assert torch.equal(got[:90][~nan[:90]], plain[:90][~nan[:90]])
+    check(torch.where(nan | want.isinf(), plain, got), dt, x, hq, hkv, starts, 0.125)
