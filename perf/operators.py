@@ -17,7 +17,6 @@ absmax <= 127 * 2^e over the block's rows of that head, so quantising, rescaling
 exact but for the rounding to an integer.
 """
 
-import functools
 import math
 import os
 import random
@@ -32,7 +31,6 @@ MIN_EXP = -120  # smallest scale exponent of a block
 LARGEST = 3_500_000_000  # scores of a drawn attention case in its plain form
 
 
-@functools.cache  # a program imports the package once, not at every call
 def _ops():
     root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "llm-inference-scheduler_b200")
     if root not in sys.path:
