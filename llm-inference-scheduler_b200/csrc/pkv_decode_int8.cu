@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
               if (!(fabsf(up) < INFINITY)) up = 0.f;
               cf[c] = ex2_approx(-up);
               mu[nt][c] += up;
-              l[nt][c] *= cf[c];
+              if (!fresh) l[nt][c] *= cf[c];  // (up may be far below zero: 0 * inf would be NaN)
               mx[c] = up;
               cf[c] *= vf;
             }
@@ -567,7 +567,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       const float2 ml = *reinterpret_cast<const float2*>(sl + kHeads * D + 2 * hh);
       const float4 x = *reinterpret_cast<const float4*>(sl + hh * D + 4 * v);
       const float mn = one ? ml.x : fmaxf(mm, ml.x);
-      const float fa = ex2_approx(mm - mn), fb = ex2_approx(ml.x - mn) * ml.y;
+      // (nothing is held before the first, whose mn may be far below zero: 0 * inf would be NaN)
+      const float fa = one ? 0.f : ex2_approx(mm - mn), fb = ex2_approx(ml.x - mn) * ml.y;
       mm = mn;
       ll = ll * fa + fb;
       oo = make_float4(oo.x * fa + x.x * fb, oo.y * fa + x.y * fb, oo.z * fa + x.z * fb, oo.w * fa + x.w * fb);
@@ -642,7 +643,7 @@ __global__ void __launch_bounds__(kM8Threads) merge_int8_kernel(const D8Params p
     bool any = false;
     __device__ void add(float2 ml, float4 x) {
       const float mn = any ? fmaxf(m, ml.x) : ml.x;
-      const float fa = ex2_approx(m - mn), fb = ex2_approx(ml.x - mn) * ml.y;
+      const float fa = any ? ex2_approx(m - mn) : 0.f, fb = ex2_approx(ml.x - mn) * ml.y;
       m = mn;
       any = true;
       l = l * fa + fb;
