@@ -19,9 +19,14 @@
 // becomes the low byte of the fp16 1024 + 128 + x (a byte permute), and
 // subtracting 1152 is exact.  (fp8 bytes need the conversion pipe, which bounds
 // the fp8 kernel at about half of the HBM rate.)  The V scale goes into P as
-// 2^(c_b - E), E the largest exponent seen so far (a larger one rescales O,
-// exactly), and 2^E into O at the end; the row sum takes the unscaled p.  For
-// fp32 q, P is split into two fp16 parts (22 bits) and each product is two MMAs.
+// P' = p 2^(c_b + n), n per head such that the largest P' so far, the largest
+// product of a probability and a scale, lies in 2^6 .. 2^15: fp16 keeps 11 bits of
+// the keys down to 2^-20 of that one and an error of 2^-31 of it below.  (With n by
+// the largest scale alone, a loud block of no weight took the others' bits: 2.3% off
+// at a ratio of 2^20.)  n moves where P' passes 2^15 or the maximum moves, O with it,
+// exactly; the row sum takes p itself.  An error of 2^-11 a key is of the size of the
+// output's own rounding for 16-bit q; for fp32 q, P' is split into two fp16 parts
+// (22 bits) and each product is two MMAs.
 // Maximum, sums and O are fp32.
 //
 // Work split.  The 16-token tiles of all sequences are cut into one contiguous
@@ -55,6 +60,10 @@ constexpr int kD8MaxSeqs = 1024;   // per launch
 constexpr int kD8MaxCtas = 296;    // per launch and head group
 constexpr float kD8Log2e = 1.4426950408889634f;
 constexpr float kD8Slack = 8.f;    // the reference maximum moves by more than this (log2)
+// log2 of P' = p vs 2^gain: the largest is brought to 2^kD8LeadP when the gain is set
+// and never passes 2^kD8MostP (fp16 ends at 2^16)
+constexpr float kD8LeadP = 7.f, kD8MostP = 15.f;
+constexpr float kD8MostGain = 119.f;  // p 2^gain stays finite (p <= 2^8)
 
 struct D8Params {
   void* out;
@@ -100,6 +109,11 @@ __device__ __forceinline__ uint32_t sub1152(uint32_t h) {
 }
 __device__ __forceinline__ uint32_t i8_lo(uint32_t biased) { return sub1152(__byte_perm(biased, 0x64646464u, 0x4140)); }
 __device__ __forceinline__ uint32_t i8_hi(uint32_t biased) { return sub1152(__byte_perm(biased, 0x64646464u, 0x4342)); }
+
+// 2^n for whole n <= 127, exactly; 0 below the normal range
+__device__ __forceinline__ float exp2_whole(float n) {
+  return __int_as_float((static_cast<int>(fmaxf(n, -127.f)) + 127) << 23);
+}
 
 // last s in [0, n) with prefix[s] <= x
 __device__ __forceinline__ int d8_find(const int* prefix, int n, int x) {
@@ -316,8 +330,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
         for (int j = 0; j < KS; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
       }
-      float v_ref = 0.f, v_inv = 0.f;  // 2^E and 2^-E (0: no tile yet)
-      bool fresh = true;               // no tile of the segment yet
+      // gain: P' = p vs 2^gain goes into the products (vs: V's scale of the tile)
+      float gain[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) gain[nt][0] = gain[nt][1] = 0.f;
+      bool fresh = true;  // no tile of the segment yet
 
       int left = ctx - (pos - prefix[s]) * 16;  // tokens from this tile on
       for (; pos < seg_end; ++pos, ++i, left -= 16) {
@@ -368,7 +385,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           }
         // ---- x - mu of the lane's scores (tokens g, g + 8; heads 2t, 2t + 1)
         float2 x0[NT], x1[NT];
-        float top = -INFINITY;
+        float top = -INFINITY, top_w = -INFINITY;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float2 f = __fmul2_rn(make_float2(c_head[nt][0], c_head[nt][1]), make_float2(ks, ks));
@@ -384,15 +401,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
             if (g + 8 >= left) x1[nt] = none;
           }
         }
+        // the largest x - mu, and the largest of P' without vs
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) top = fmax3(top, fmaxf(x0[nt].x, x0[nt].y), fmaxf(x1[nt].x, x1[nt].y));
-        const bool wider = vs > v_ref;  // warp-uniform
-        if (__any_sync(0xffffffffu, top > kD8Slack) || wider || fresh) {
-          const float vf = wider ? v_ref * (1.f / vs) : 1.f;  // exact
-          if (wider) {
-            v_ref = vs;
-            v_inv = 1.f / vs;
-          }
+        for (int nt = 0; nt < NT; ++nt) {
+          const float2 m = make_float2(fmaxf(x0[nt].x, x1[nt].x), fmaxf(x0[nt].y, x1[nt].y));
+          const float2 w = __fadd2_rn(m, make_float2(gain[nt][0], gain[nt][1]));
+          top = fmax3(top, m.x, m.y);
+          top_w = fmax3(top_w, w.x, w.y);
+        }
+        const float v_exp = __uint_as_float(0x4b000000u | (__float_as_uint(vs) >> 23)) - (8388608.f + 127.f);  // vs < 2^(v_exp + 1)
+        if (__any_sync(0xffffffffu, top > kD8Slack || top_w + v_exp > kD8MostP - 1.f) || fresh) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float mx[2] = {fmaxf(x0[nt].x, x1[nt].x), fmaxf(x0[nt].y, x1[nt].y)}, cf[2];
@@ -400,14 +418,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
             for (int c = 0; c < 2; ++c) {
 #pragma unroll
               for (int off = 4; off < 32; off <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], off));
-              // the reference moves up by mx (the segment's first tile: to its maximum, unless that is not finite)
-              float up = fresh ? mx[c] : fmaxf(mx[c], 0.f);
+              // the reference moves up to mx, in whole steps (the segment's first tile: to its
+              // maximum, unless that is not finite)
+              float up = ceilf(fresh ? mx[c] : fmaxf(mx[c], 0.f));
               if (!(fabsf(up) < INFINITY)) up = 0.f;
-              cf[c] = ex2_approx(-up);
               mu[nt][c] += up;
-              if (!fresh) l[nt][c] *= cf[c];  // (up may be far below zero: 0 * inf would be NaN)
+              // gain: what it was, raised by what the older p fall by, or as low as this tile's largest P' asks for
+              const float want = kD8LeadP - ceilf(mx[c] - up) - v_exp;
+              const float to = fmaxf(fminf(fresh ? want : fminf(gain[nt][c] + up, want), kD8MostGain), -126.f);
+              cf[c] = exp2_whole(to - gain[nt][c] - up);
+              gain[nt][c] = to;
+              if (!fresh) l[nt][c] *= exp2_whole(-up);
               mx[c] = up;
-              cf[c] *= vf;
             }
             const float2 nu = make_float2(-mx[0], -mx[1]);
             x0[nt] = __fadd2_rn(x0[nt], nu);
@@ -424,7 +446,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           }
           fresh = false;
         }
-        const float2 vfac = make_float2(vs * v_inv, vs * v_inv);
+        const float2 vs2 = make_float2(vs, vs);
         uint32_t pb[NT][LIMBS][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -432,7 +454,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           const float2 p1 = make_float2(ex2_approx(x1[nt].x), ex2_approx(x1[nt].y));
           l[nt][0] += p0.x + p1.x;
           l[nt][1] += p0.y + p1.y;
-          const float2 e0 = __fmul2_rn(p0, vfac), e1 = __fmul2_rn(p1, vfac);
+          // (the gain first: its product with vs alone may pass fp32's range)
+          const float2 n = __fadd2_rn(make_float2(gain[nt][0], gain[nt][1]), make_float2(kFloatBase + 127.f, kFloatBase + 127.f));
+          const float2 g2 = make_float2(__int_as_float(__float_as_int(n.x) << 23), __int_as_float(__float_as_int(n.y) << 23));
+          const float2 e0 = __fmul2_rn(__fmul2_rn(p0, g2), vs2), e1 = __fmul2_rn(__fmul2_rn(p1, g2), vs2);
           float e[4] = {e0.x, e0.y, e1.x, e1.y};
           pb[nt][0][0] = movmatrix_t(pack2<__half>(e[0], e[1]));
           pb[nt][0][1] = movmatrix_t(pack2<__half>(e[2], e[3]));
@@ -490,14 +515,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           for (int c = 0; c < 2; ++c) {
             const int hh = 8 * nt + 2 * t + c;
             if (hh >= nh) continue;
-            const float f = v_ref / l[nt][c];
+            const float f = 1.f / l[nt][c], back = exp2_whole(-gain[nt][c]);
             T* orow = static_cast<T*>(p.out) + static_cast<int64_t>(s) * p.out_stride +
                       static_cast<int64_t>(head0 + hh) * D;
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
               const int d = (j >> 2) * 64 + 8 * g + 2 * (j & 3);
-              orow[d] = Elem<T>::from_f(o[nt][j][c] * f);
-              orow[d + 1] = Elem<T>::from_f(o[nt][j][c + 2] * f);
+              orow[d] = Elem<T>::from_f(o[nt][j][c] * f * back);
+              orow[d + 1] = Elem<T>::from_f(o[nt][j][c + 2] * f * back);
             }
           }
       } else {
@@ -510,12 +535,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const int hh = 8 * nt + 2 * t + c;
-            const float f = v_ref / l[nt][c];  // a partial holds its own softmax's O
+            const float f = 1.f / l[nt][c], back = exp2_whole(-gain[nt][c]);  // a partial holds its own softmax's O
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
               const int d = (j >> 2) * 64 + 8 * g + 2 * (j & 3);
-              slot[hh * D + d] = o[nt][j][c] * f;
-              slot[hh * D + d + 1] = o[nt][j][c + 2] * f;
+              slot[hh * D + d] = o[nt][j][c] * f * back;
+              slot[hh * D + d + 1] = o[nt][j][c + 2] * f * back;
             }
             if (g == 0) {
               slot[kHeads * D + 2 * hh] = mu[nt][c];
