@@ -400,14 +400,20 @@ __device__ __forceinline__ bool elect_one() {
 // integer n, held in t's low mantissa bits; f = x - n lies in [-1/2, 1/2].
 // 2^f is a degree-3 polynomial fitted by Remez exchange to minimise the
 // relative error on [-1/2, 1/2] (7.5e-5, against 4.9e-4 for rounding to
-// fp16); 2^n is applied by adding n to the exponent field.  x is clamped at
-// -125 so that the exponent field stays positive (p(f) can be below 1).
+// fp16); 2^n is applied by adding n to the exponent field.  x is clamped just
+// above -127, at the first value there whose p(f) is not below 1 (18 units above it
+// in the last place): the exponent field is then zero and the result 18 * 2^-149,
+// which rounds to 0 in bf16 as in fp16.  So a score of -infinity (a hidden key)
+// gets no weight at all; clamped at -125 it got 2^-125, a number in bf16, and a hidden
+// value of 2^127 entered the row.  Between the clamp and -126 results are off by at
+// most 2^-127.
+constexpr float kExp2Lowest = -0x1.fbffe4p+6f;
 constexpr float kExp2C0 = 0x1.fff692p-1f;
 constexpr float kExp2C1 = 0x1.62f31ap-1f;
 constexpr float kExp2C2 = 0x1.f0de1ap-3f;
 constexpr float kExp2C3 = 0x1.c3f760p-5f;
 __device__ __forceinline__ float exp2_poly3(float x) {
-  x = fmaxf(x, -125.f);
+  x = fmaxf(x, kExp2Lowest);
   const float t = __fadd_rn(x, 12582912.f);
   const float f = __fsub_rn(x, __fsub_rn(t, 12582912.f));
   const float p = fmaf(fmaf(fmaf(kExp2C3, f, kExp2C2), f, kExp2C1), f, kExp2C0);
@@ -417,8 +423,8 @@ __device__ __forceinline__ float exp2_poly3(float x) {
 // (__fadd2_rn / __ffma2_rn round each lane as __fadd_rn / fmaf do, so each
 // lane's result equals exp2_poly3 bit for bit) at half the issue slots
 __device__ __forceinline__ float2 exp2_poly3x2(float2 x) {
-  x.x = fmaxf(x.x, -125.f);
-  x.y = fmaxf(x.y, -125.f);
+  x.x = fmaxf(x.x, kExp2Lowest);
+  x.y = fmaxf(x.y, kExp2Lowest);
   const float2 big = make_float2(12582912.f, 12582912.f), nbig = make_float2(-12582912.f, -12582912.f);
   const float2 t = __fadd2_rn(x, big);
   const float2 n = __fadd2_rn(t, nbig);
