@@ -680,7 +680,8 @@ int pkv_paged_prefill_attention_int8(void* out, int64_t out_row_stride, const vo
  * fused projection will do); out must not overlap q, k or v.  head_dim 64 or 128,
  * scale > 0.  Rows before query_start_loc[0] and past query_start_loc[n_seqs] are
  * not written and enter no result.  A key that a row must not see never enters
- * it, whatever it holds.
+ * it, whatever it holds.  An infinity or NaN in a value that it sees makes that
+ * column of it infinite or NaN (NaN where the key's weight rounds to 0 in dtype).
  */
 int pkv_packed_prompt_attention(void* out, int64_t out_row_stride, const void* q,
                                 int64_t q_row_stride, const void* k, int64_t k_row_stride,

@@ -98,13 +98,14 @@ __device__ __forceinline__ uint32_t e4m3_even_h2(uint32_t x) {
   const uint32_t z = (x << 7) & 0x7f807f80u;  // sign lands on bit 14 / 30
   return z + (z & 0x40004000u);               // ... and is carried to bit 15 / 31
 }
-// Bounded wait: gives up after ~2^31 SM cycles (about a second) and returns
-// false, so a lost transaction can never hang the GPU.
+// Bounded wait: gives up after ~2^LOG_CYCLES SM cycles (2^31: about a second) and
+// returns false, so a lost transaction can never hang the GPU.
+template <int LOG_CYCLES = 31>
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
   if (mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
   while (!mbar_try_wait(bar, parity)) {
-    if (clock64() - t0 > (1ll << 31)) return false;
+    if (clock64() - t0 > (1ll << LOG_CYCLES)) return false;
   }
   return true;
 }

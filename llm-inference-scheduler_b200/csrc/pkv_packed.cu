@@ -40,42 +40,187 @@ __device__ __forceinline__ KeySpan key_span(const PackedArgs& a, int s, int q_be
   return k;
 }
 
-// One (query row, head) by a whole warp, keys 0 .. lim - 1 only: the row's own
-// arithmetic, untouched by any key it must not see.  The tiled kernels multiply
-// masked keys by a probability of zero, which is not zero where such a key's V
-// holds an infinity or NaN; a row that comes out not finite is computed again
-// here (and stays so if its own values make it so).  Not where its sum is NaN
-// already: masked scores never enter that, so its own q or keys made it so.
-template <typename T, int D>
-__device__ __noinline__ void packed_row_alone(const PackedArgs& a, int64_t row, int h, int64_t key0, int lim) {
-  const int lane = threadIdx.x & 31, g = h / (a.n_q_heads / a.n_kv_heads);
-  constexpr int kPer = D / 32;
-  const T* q = static_cast<const T*>(a.q) + row * a.q_stride + static_cast<int64_t>(h) * D;
-  float qv[kPer], acc[kPer];
+// ---- rows that come out not finite
+//
+// The tiled kernels multiply a hidden key's V by a probability of zero, which is
+// not zero where that V holds an infinity or NaN, and their unnormalised sums pass
+// fp32 for values near its end.  A row that comes out not finite is therefore
+// computed again by a warp, over its own keys only, unless its own values make it
+// so: its sum of probabilities is NaN (hidden scores never enter that), or a V that
+// it sees is not finite and none of the hidden ones in its last tiles is.  (Without
+// that second rule one NaN in the first V of a prompt of 8,191 tokens had every later
+// row computed again: 77 ms.  With it 0.2; and 8.8 where the NaN is hidden from the
+// last rows, four at a time, against 45 one by one.)
+
+// four or eight consecutive elements from a 16-byte boundary
+template <typename T>
+__device__ __forceinline__ void load16_f(const T* p, float* v) {
+  const uint4 w = *reinterpret_cast<const uint4*>(p);
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    qv[i] = Elem<T>::to_f(q[lane + 32 * i]);
-    acc[i] = 0.f;
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(u[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const T* e = reinterpret_cast<const T*>(u) + i;
+      v[i] = Elem<T>::to_f(*e);
+    }
   }
-  float m = -FLT_MAX, l = 0.f;
-  for (int j = 0; j < lim; ++j) {
-    const T* k = static_cast<const T*>(a.k) + (key0 + j) * a.k_stride + static_cast<int64_t>(g) * D;
-    const T* v = static_cast<const T*>(a.v) + (key0 + j) * a.v_stride + static_cast<int64_t>(g) * D;
-    float s = 0.f;
+}
+
+// (whole warp) keys from .. to - 1 of one sequence and KV head: the last of them whose
+// V is not finite, or the first; `none` if there is none.
+template <typename T, int D, bool VEC>
+__device__ __forceinline__ int value_not_finite(const PackedArgs& a, int g, int64_t key0, int from, int to, bool last, int none) {
+  const int lane = threadIdx.x & 31;
+  for (int i = 0; i < to - from; i += 32) {
+    const int key = last ? to - 1 - i - lane : from + i + lane;
+    bool bad = false;
+    if (key >= from && key < to) {
+      const T* v = static_cast<const T*>(a.v) + (key0 + key) * a.v_stride + static_cast<int64_t>(g) * D;
+      constexpr int kStep = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+#pragma unroll 8
+      for (int d = 0; d < D; d += kStep) {
+        float f[kStep];
+        if constexpr (VEC) load16_f<T>(v + d, f);
+        else f[0] = Elem<T>::to_f(v[d]);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) s = fmaf(qv[i], Elem<T>::to_f(k[lane + 32 * i]), s);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    s *= a.scale;
-    const float mn = fmaxf(m, s), c = expf(m - mn), p = expf(s - mn);
-    m = mn;
-    l = l * c + p;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * c + p * Elem<T>::to_f(v[lane + 32 * i]);
+        for (int e = 0; e < kStep; ++e) bad = bad || !(fabsf(f[e]) < INFINITY);
+      }
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, bad);
+    if (hit) {  // lane 0 has the end that is asked for
+      const int l = __ffs(hit) - 1;
+      return last ? to - 1 - i - l : from + i + l;
+    }
   }
-  T* out = static_cast<T*>(a.out) + row * a.out_stride + static_cast<int64_t>(h) * D;
+  return none;
+}
+
+// Up to kAlone (query row, head) pairs of one KV head by a whole warp, each over its
+// own keys 0 .. lim - 1 only: 32 keys at a time, the scores a key to a lane, the
+// values D / 32 dims to a lane (VEC: a step's loads ahead of its arithmetic).  Rows with
+// lim 0 are not there.  About 64 cycles a row and key (fp16, 64 dims).
+constexpr int kAlone = 4;
+template <typename T, int D, bool VEC>
+__device__ __forceinline__ void packed_rows_alone(const PackedArgs& a, const int64_t (&row)[kAlone], const int (&h)[kAlone],
+                                                  const int (&lim)[kAlone], int g, int64_t key0) {
+  const int lane = threadIdx.x & 31;
+  constexpr int kPer = D / 32, kStep = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  constexpr int kAhead = VEC ? 16 : 4;  // values on their way at a time
+  const T* kr = static_cast<const T*>(a.k) + key0 * a.k_stride + static_cast<int64_t>(g) * D;
+  const T* vr = static_cast<const T*>(a.v) + key0 * a.v_stride + static_cast<int64_t>(g) * D + lane * kPer;
+  const T* q[kAlone];
+  float acc[kAlone][kPer], m[kAlone], l[kAlone];  // l: this lane's keys
+  int most = 0;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) out[lane + 32 * i] = Elem<T>::from_f(acc[i] / l);
+  for (int r = 0; r < kAlone; ++r) {
+    q[r] = static_cast<const T*>(a.q) + row[r] * a.q_stride + static_cast<int64_t>(h[r]) * D;
+    m[r] = -FLT_MAX;
+    l[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) acc[r][i] = 0.f;
+    most = max(most, lim[r]);
+  }
+  for (int j0 = 0; j0 < most; j0 += 32) {
+    const int n = min(32, most - j0);
+    struct alignas(VEC ? kPer * sizeof(T) : sizeof(T)) Dims { T e[kPer]; } v[kAhead];
+    auto load_v = [&](int at) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        // (a key past the last is read as the last, and gets no weight)
+        const T* from = vr + static_cast<int64_t>(j0 + min(at + j, n - 1)) * a.v_stride;
+        if constexpr (VEC) {
+          v[j] = *reinterpret_cast<const Dims*>(from);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) v[j].e[i] = from[i];
+        }
+      }
+    };
+    load_v(0);
+    float p[kAlone];
+#pragma unroll
+    for (int r = 0; r < kAlone; ++r) p[r] = 0.f;
+    const T* k = kr + static_cast<int64_t>(j0 + min(lane, n - 1)) * a.k_stride;
+#pragma unroll 4
+    for (int d = 0; d < D; d += kStep) {
+      float kf[kStep], qf[kStep];
+      if constexpr (VEC) load16_f<T>(k + d, kf);
+      else kf[0] = Elem<T>::to_f(k[d]);
+#pragma unroll
+      for (int r = 0; r < kAlone; ++r) {
+        if constexpr (VEC) load16_f<T>(q[r] + d, qf);
+        else qf[0] = Elem<T>::to_f(q[r][d]);
+#pragma unroll
+        for (int e = 0; e < kStep; ++e) p[r] = fmaf(qf[e], kf[e], p[r]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kAlone; ++r) {
+      const float s = j0 + lane < lim[r] ? p[r] * a.scale : -INFINITY;
+      float mn = fmaxf(m[r], s);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      const float c = expf(m[r] - mn);
+      p[r] = expf(s - mn);
+      m[r] = mn;
+      l[r] = l[r] * c + p[r];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) acc[r][i] *= c;
+    }
+#pragma unroll 1
+    for (int at = 0; at < n; at += kAhead) {
+      if (at > 0) load_v(at);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+        for (int r = 0; r < kAlone; ++r) {
+          const float pj = __shfl_sync(0xffffffffu, p[r], (at + j) & 31);
+          if (j0 + at + j < lim[r]) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) acc[r][i] = fmaf(pj, Elem<T>::to_f(v[j].e[i]), acc[r][i]);
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kAlone; ++r) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+    if (lim[r] == 0) continue;
+    T* out = static_cast<T*>(a.out) + row[r] * a.out_stride + static_cast<int64_t>(h[r]) * D + lane * kPer;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) out[i] = Elem<T>::from_f(acc[r][i] / l[r]);
+  }
+}
+
+// (whole warp) `bad` lanes: a row of head h (all of one KV head) and `lim` keys came
+// out not finite with a sum that is.  A row's last key tile ends at most 127 + 127 keys
+// behind its last key (the last row of its query tile, the end of a key tile)
+template <typename T, int D, bool VEC>
+__device__ __noinline__ void redo_rows(const PackedArgs& a, bool bad, int64_t row, int h, int lim, int64_t key0) {
+  const int g = __shfl_sync(0xffffffffu, h, 0) / (a.n_q_heads / a.n_kv_heads);
+  const int low = __reduce_min_sync(0xffffffffu, bad ? lim : INT_MAX), high = __reduce_max_sync(0xffffffffu, bad ? lim : 0);
+  const int end = static_cast<int>(min((static_cast<int64_t>(high) + 254) / 128 * 128, a.n_key_rows - key0));
+  const int hidden = value_not_finite<T, D, VEC>(a, g, key0, low, end, true, -1);
+  const int seen = value_not_finite<T, D, VEC>(a, g, key0, 0, high, false, INT_MAX);
+  unsigned todo = __ballot_sync(0xffffffffu, bad && (lim <= hidden || lim <= seen));
+  while (todo) {
+    int64_t rows[kAlone];
+    int heads[kAlone], lims[kAlone];
+#pragma unroll
+    for (int r = 0; r < kAlone; ++r) {
+      const int b = todo ? __ffs(todo) - 1 : 0;
+      rows[r] = __shfl_sync(0xffffffffu, row, b);
+      heads[r] = __shfl_sync(0xffffffffu, h, b);
+      lims[r] = __shfl_sync(0xffffffffu, lim, b);
+      if (todo == 0) lims[r] = 0, rows[r] = rows[0], heads[r] = heads[0];
+      todo &= todo - 1;
+    }
+    packed_rows_alone<T, D, VEC>(a, rows, heads, lims, g, key0);
+  }
 }
 
 // ---- CUDA-core tiles: 64 queries x 64 keys, fp32 throughout
@@ -271,18 +416,22 @@ __global__ void __launch_bounds__(kPkThreads) packed_cores_kernel(const PackedAr
     }
     fine[r] = ok || row >= rows || !(l[r] < INFINITY);
   }
+  // rows 4 ty + r of the warp's two half-warps: lane 4 half + r takes its row's part
+  unsigned bad = 0;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const unsigned bad = __ballot_sync(0xffffffffu, !fine[r]);
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-      if (bad & (0xffffu << (16 * half))) {  // warp-uniform: row 4 ty + r of this half-warp
-        const int row = 4 * ((tid >> 5) * 2 + half) + r;
-        __syncwarp();
-        packed_row_alone<T, D>(a, static_cast<int64_t>(q_begin) + q0 + row, h, span.row0,
-                               min(span.prior + q0 + row + 1, span.keys));
-      }
+    const unsigned b = __ballot_sync(0xffffffffu, !fine[r]);
+    bad |= (b & 0xffffu ? 1u << r : 0u) | (b >> 16 ? 16u << r : 0u);
   }
+  if (bad == 0) return;  // (warp-uniform)
+  __syncwarp();
+  const int lane = tid & 31, my_row = 4 * (tid >> 5) * 2 + (lane & 7);
+  const int my_lim = min(span.prior + q0 + my_row + 1, span.keys);
+  const int64_t row0 = static_cast<int64_t>(q_begin) + q0 + my_row;
+  if constexpr (sizeof(T) == 4) {
+    if (wide) return redo_rows<T, D, true>(a, (bad >> lane) & 1, row0, h, my_lim, span.row0);
+  }
+  redo_rows<T, D, false>(a, (bad >> lane) & 1, row0, h, my_lim, span.row0);
 }
 
 template <typename T, int D>
@@ -380,6 +529,9 @@ constexpr int kTcMaxSegs = 16;      // segments of an item
 constexpr int kTcSegKeys = 1536;    // least keys of a segment
 constexpr int kTcSplitPerSm = 4;    // split calls of up to this many items an SM
 constexpr uint32_t kTcTmemCols = 512;
+// log2 of the cycles that a wait takes at most (9 seconds): the other warps wait while
+// one computes up to 32 rows on its own (redo_rows), some 2,000 cycles a key
+constexpr int kTcWait = 34;
 
 template <int D> struct TcShape {
   static constexpr int kN = D == 64 ? 128 : 64;         // keys per tile
@@ -687,7 +839,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   // item `k` (counted per CTA) as the scheduler published it; tok0 < 0: no more
   auto take_item = [&](int k, TcItem& it) -> bool {
     const int sl = k & 1;
-    bool ok = mbar_wait(&item_full[sl], (k >> 1) & 1);
+    bool ok = mbar_wait<kTcWait>(&item_full[sl], (k >> 1) & 1);
     ok = __all_sync(0xffffffffu, ok);
     const int* w = items + sl * kTcItemInts;
     it.s = w[0], it.g = w[1], it.tok0 = w[2], it.q_begin = w[3], it.n_new = w[4], it.prior = w[5], it.keys = w[6], it.row0 = w[7];
@@ -721,7 +873,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           TcItem it;
           bool have = false;
           // taken late, so that a CTA with a long item leaves the next one to others
-          if (k >= 1 && more && !mbar_wait(loaded, (k - 1) & 1)) {
+          if (k >= 1 && more && !mbar_wait<kTcWait>(loaded, (k - 1) & 1)) {
             raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
             more = false;
           }
@@ -731,7 +883,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // the next block that has not started, if there is one
             mbar_arrive_expect_tx(clc_bar, 16);
             clc_try_cancel(base + Sh::kOffClc, clc_bar);
-            if (!mbar_wait(clc_bar, clc_phase)) {
+            if (!mbar_wait<kTcWait>(clc_bar, clc_phase)) {
               raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
               more = false;
               break;
@@ -743,7 +895,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           idx = -1;
           const int sl = k & 1;
-          if (k >= 2 && !mbar_wait(&item_empty[sl], ((k >> 1) & 1) ^ 1)) {
+          if (k >= 2 && !mbar_wait<kTcWait>(&item_empty[sl], ((k >> 1) & 1) ^ 1)) {
             raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
             have = false;
           }
@@ -762,7 +914,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       TcItem it;
       for (int k = 0; take_item(k, it); ++k) {
         const int n_tiles = max(item_tiles(it, 0), item_tiles(it, 1));
-        if (k >= 1 && !__all_sync(0xffffffffu, mbar_wait(q_empty, (k - 1) & 1))) {
+        if (k >= 1 && !__all_sync(0xffffffffu, mbar_wait<kTcWait>(q_empty, (k - 1) & 1))) {
           if (lane == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
           break;
         }
@@ -783,7 +935,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             uint64_t* full = kv ? &v_full[st] : &k_full[st];
-            if (!__all_sync(0xffffffffu, mbar_wait(kv ? &v_empty[st] : &k_empty[st], ((c / kStages) & 1) ^ 1))) {
+            if (!__all_sync(0xffffffffu, mbar_wait<kTcWait>(kv ? &v_empty[st] : &k_empty[st], ((c / kStages) & 1) ^ 1))) {
               if (lane == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
               dead = true;
               break;
@@ -809,7 +961,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // shared memory is broadcast, so that the compiler knows the loops to be
       // uniform and keeps the MMAs' operands in uniform registers.
       constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-      auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait<kTcWait>(bar, parity)); };
       int st = 0, buf = 0;                 // K / V stage, S buffer
       uint32_t st_ph = 0, buf_ph = 0;      // their phases
       int turn[2] = {0, 0};                // the tile's next barrier of its ring
@@ -914,14 +1066,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     int n0 = 0;   // steps of both tiles so far
     bool dead = false;
     TcItem it;
-    for (int k = 0; take_item(k, it); ++k) {
+    unsigned again;  // lanes whose row may have to be computed again
+    int k = 0;
+    do {
+    again = 0;
+    for (; take_item(k, it); ++k) {
       const int kvx = tile_keys(it, x), ntx = item_tiles(it, x), nto = item_tiles(it, 1 - x);
       // PV number i of this item and tile has completed.  PVs signal a ring of
       // barriers: a wait tells a phase from the one before it only, and the S
       // that the caller has seen vouches for the PV a ring's length back.
       auto wait_pv = [&](int i) {
         const int w = cx + i;
-        if (!dead && !mbar_wait(&o_done[x * kBufs + w % kBufs], (w / kBufs) & 1)) dead = true;
+        if (!dead && !mbar_wait<kTcWait>(&o_done[x * kBufs + w % kBufs], (w / kBufs) & 1)) dead = true;
       };
       const int tok = it.tok0 + x * TT + rtok;
       const bool row_valid = rtok < TT && tok < it.n_new;
@@ -935,7 +1091,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int n = n0 + (x == 0 ? (nto > 0 ? 2 * j : j) : (j < nto ? 2 * j + 1 : nto + j));
         const int b = n % kBufs;
         const uint32_t t_s = tbase + b * kN + lane_off;
-        if (!dead && !mbar_wait(&s_full[x * kBufs + (cx + j) % kBufs], ((cx + j) / kBufs) & 1)) dead = true;
+        if (!dead && !mbar_wait<kTcWait>(&s_full[x * kBufs + (cx + j) % kBufs], ((cx + j) / kBufs) & 1)) dead = true;
         __syncwarp();
         tc_fence_after();
         uint32_t sr[kN / 32][32];
@@ -1041,7 +1197,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         wait_pv(ntx - 1);
         __syncwarp();
         tc_fence_after();
-        const float inv = l > 0.f ? 1.f / l : l;  // NaN stays
+        const float inv = l > 0.f ? 1.f / l : NAN;  // (0: scores of -infinity alone, or a segment without a say)
         float fsum = 0.f;
 #pragma unroll
         for (int c2 = 0; c2 < D / 32; ++c2) {
@@ -1063,7 +1219,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
         tc_fence_before();  // O is read before the next item's PV (ordered by p_full)
-        if (whole) fine = !row_valid || !(l < INFINITY) || (l > 0.f && fsum < INFINITY);
+        if (whole) fine = !row_valid || !(l > 0.f && l < INFINITY) || fsum < INFINITY;
       }
       if (!whole) {
         // each warp on its own: its rows of all segments are in memory once their
@@ -1088,7 +1244,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             w[q] = ml[q].y != 0.f ? ex2_approx(ml[q].x - top) * ml[q].y : 0.f;
             sum += w[q];
           }
-          const float inv = sum > 0.f ? 1.f / sum : sum;  // NaN stays
+          const float inv = sum > 0.f ? 1.f / sum : NAN;  // (0: scores of -infinity alone)
           float fsum = 0.f;
           for (int c2 = 0; c2 < D / 32; ++c2) {
             float f[32];
@@ -1125,21 +1281,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __syncwarp();
             store32(c2, f);
           }
-          fine = !row_valid || !(sum < INFINITY) || (sum > 0.f && fsum < INFINITY);
+          fine = !row_valid || !(sum > 0.f && sum < INFINITY) || fsum < INFINITY;
         }
       }
       cx += ntx;
       n0 += ntx + nto;
-      unsigned bad = __ballot_sync(0xffffffffu, !fine);
-      while (bad) {  // rows that a key they must not see may have spoiled
-        const int b = __ffs(bad) - 1;
-        bad &= bad - 1;
-        const int64_t brow = __shfl_sync(0xffffffffu, row, b);
-        const int bhead = __shfl_sync(0xffffffffu, head, b), blim = __shfl_sync(0xffffffffu, lim, b);
-        __syncwarp();
-        packed_row_alone<T, D>(a, brow, bhead, it.row0, blim);
+      // rows that a key they must not see may have spoiled: out of the loop over items
+      // and back into it (with the call inside, the whole loop was 5% slower)
+      again = __ballot_sync(0xffffffffu, !fine);
+      if (again) {
+        reinterpret_cast<int4*>(mine)[lane] = make_int4(static_cast<int>(row), head, lim, it.row0);
+        ++k;
+        break;
       }
     }
+    if (again) {
+      const int4 me = reinterpret_cast<const int4*>(base + Sh::kOffOut + warp * 2048)[lane];
+      redo_rows<T, D, true>(a, (again >> lane) & 1, me.x, me.y, me.z, me.w);
+    }
+    } while (again);
     if (dead && r == 0) raise_flag(a.err, PKV_FLAG_PIPELINE_TIMEOUT);
   }
   tc_fence_before();
