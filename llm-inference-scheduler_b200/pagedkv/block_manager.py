@@ -563,6 +563,13 @@ class PagedKVCache:
             self._workspace = torch.empty(need, dtype=torch.uint8, device=self.mgr.device)
         return self._workspace
 
+    def step_buffers(self) -> tuple:
+        """The buffers that the launches of a step use besides the pools, as they are now
+        (each is replaced by a larger one when a step needs that): a captured step
+        keeps them."""
+        return (self._workspace, self._schedule_buf, self._fp8_scratch, self._int8_workspace, self._int8_scratch,
+                self._counts, self._slots_int8)
+
     def forward_layer(self, layer: int, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
                       meta: StepMetadata, scale: float, out: torch.Tensor | None = None,
                       advance: bool = True) -> torch.Tensor:

@@ -34,10 +34,11 @@ Fixed shapes make a replay valid for any step that fits:
   each prefill sequence's last row, so the first B logits rows are the
   step's sequences in order;
 * the runner owns the decode schedule, the RoPE tables (sized for W * 16
-  positions) and the logits buffer; the cache's split-K workspace and fp8
-  prefill scratch are sized for the largest graph before the first capture
-  and held here, so a later reallocation by an eager step cannot free them
-  under a graph.
+  positions) and the logits buffer; the cache's split-K workspace, prefill
+  scratch and index rows are sized for the largest graph before the first
+  capture.  Eager steps may replace them by larger ones between two captures, so
+  each graph holds those that it was captured with (`held`), and no
+  reallocation frees one under a graph.
 
 Padding does not change the real rows: the attention kernels give padding
 rows no keys and no output, and every other operation of the step (GEMMs,
@@ -176,6 +177,7 @@ class StepGraphs:
         rows = max(R + P for R, P in keys)
         heads = max(R + self._layout(R, P)["NP"] for R, P in keys)
         self.graphs = {}
+        self.held: dict[tuple[int, int], tuple] = {}  # what each graph uses of the cache's buffers
         self.pool = torch.cuda.graph_pool_handle()
         self.meta_dev = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
         self.stage = [[torch.empty(nbytes, dtype=torch.uint8).pin_memory(), None] for _ in range(2)]
@@ -184,23 +186,19 @@ class StepGraphs:
         self.logits = torch.empty((heads, cfg.vocab_size), dtype=m.dtype, device=dev)
         Rm = max(R for R, _ in keys)
         self.schedule = ops.new_decode_schedule(Rm, self.W, dev)
-        self.workspace = kv.decode_workspace(Rm, cfg.num_attention_heads, cfg.head_dim)
-        self.scratch = None
+        kv.decode_workspace(Rm, cfg.num_attention_heads, cfg.head_dim)
         if mgr.fp8 and self.prefill_seqs:
             need = ops.prefill_fp8_scratch_bytes(self.prefill_seqs, self.W, mgr.num_kv_heads,
                                                  cfg.head_dim)
             if kv._fp8_scratch is None or kv._fp8_scratch.numel() < need:
                 kv._fp8_scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-            self.scratch = kv._fp8_scratch
         if mgr.int8:
-            # what the captured layers use of the cache's, held for the same reason
             tokens = max(self._layout(R, P)["T"] for R, P in keys)
             kv.counts(Rm + 1)
             if kv._slots_int8 is None or kv._slots_int8.shape[0] < tokens:
                 kv._slots_int8 = torch.arange(tokens, dtype=torch.int64, device=dev)
             for P in {P for _, P in keys}:  # (a larger one may need less: it is not split)
                 kv.int8_buffers(self.prefill_seqs if P else 0, P, self.W, cfg.num_attention_heads, m.dtype)
-            self.int8_held = (kv._int8_workspace, kv._int8_scratch, kv._counts, kv._slots_int8)
         cos, sin = m.rope.tables(self.W * mgr.block_size)
         self.cos, self.sin = cos, sin  # held: an eager step that grows the tables drops them
 
@@ -265,6 +263,7 @@ class StepGraphs:
         with torch.cuda.graph(g, pool=self.pool, capture_error_mode="thread_local"):
             self._step(R, P)
         self.graphs[(R, P)] = g
+        self.held[(R, P)] = self.kv.step_buffers()
 
     def capture_all(self) -> None:
         for key in sorted(self._key_set, key=lambda k: -(k[0] + k[1])):
