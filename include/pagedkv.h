@@ -578,8 +578,11 @@ int pkv_paged_prefill_attention_fp8(void* out, int64_t out_row_stride, const voi
  * Requests are served in order while blocks last.  One that is not (the free
  * list is short: PKV_FLAG_OUT_OF_BLOCKS; its tokens pass n_tokens:
  * PKV_FLAG_BAD_QUERY_LAYOUT) keeps its rows of the batch, with slots -1 and
- * context_lens 0, which every kernel here skips, and takes no block; nor do the
- * requests after it.  A negative length (PKV_FLAG_BAD_QUERY_LAYOUT) or one past
+ * context_lens 0, and takes no block; nor do the requests after it.  The appends
+ * write nothing for it, the decode calls, pkv_fetch_int8 and
+ * pkv_paged_prefill_attention_int8_served give zero rows.  The other chunk calls take
+ * no context_lens: what they give for its rows is of no use (its table holds no
+ * blocks for them).  A negative length (PKV_FLAG_BAD_QUERY_LAYOUT) or one past
  * the table (PKV_FLAG_CONTEXT_EXCEEDS_TABLE) counts as a request without tokens.
  * n_free_out must not be n_free.  Up to 16,384 requests.
  */
@@ -625,7 +628,7 @@ int pkv_reshape_and_cache_int8(const void* k, const void* v, int64_t k_row_strid
  * The last row_start_loc[i + 1] - row_start_loc[i] rows of each context as
  * values (byte * scale rounded to dtype), packed one sequence behind the other:
  * the gather of append_and_fetch (mini_engine/paged/block_manager.py:136-141).
- * k_out / v_out [n_rows][n_kv_heads][head_dim] with row strides in elements.
+ * Rows of a context of length 0 are zeros.  k_out / v_out [n_rows][n_kv_heads][head_dim] with row strides in elements.
  */
 int pkv_fetch_int8(void* k_out, void* v_out, int64_t k_row_stride, int64_t v_row_stride,
                    const void* k_pool, const void* v_pool, const float* k_scale,
@@ -669,6 +672,17 @@ int pkv_paged_prefill_attention_int8(void* out, int64_t out_row_stride, const vo
                                      int n_q_heads, int n_kv_heads, int head_dim, int block_size,
                                      float scale, int dtype, void* scratch, size_t scratch_bytes,
                                      int* err_flags, pkv_stream_t stream);
+
+/* The same for a step in which some sequences may not be served (pkv_build_step_tables
+ * on a short free list): where context_lens[s] is 0 the table of sequence s is not
+ * read and its rows are zeros (for finite q).  context_lens NULL: all are served. */
+int pkv_paged_prefill_attention_int8_served(
+    void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride, const void* k_pool,
+    const void* v_pool, const float* k_scale, const float* v_scale, int num_blocks,
+    const int32_t* block_tables, int64_t block_table_stride, int max_blocks_per_seq,
+    const int32_t* query_start_loc, const int32_t* num_prior, const int32_t* context_lens, int n_seqs,
+    int n_tokens, int n_q_heads, int n_kv_heads, int head_dim, int block_size, float scale, int dtype,
+    void* scratch, size_t scratch_bytes, int* err_flags, pkv_stream_t stream);
 
 /*
  * Causal attention with grouped heads over whole prompts packed one behind the

@@ -229,15 +229,13 @@ size_t pkv_prefill_int8_scratch_bytes(int n_seqs, int n_tokens, int max_blocks_p
   return prefill_scratch(n_seqs, n_tokens, max_blocks_per_seq, n_q_heads, n_kv_heads, head_dim, block_size, dtype).total;
 }
 
-int pkv_paged_prefill_attention_int8(void* out, int64_t out_row_stride, const void* q,
-                                     int64_t q_row_stride, const void* k_pool, const void* v_pool,
-                                     const float* k_scale, const float* v_scale, int num_blocks,
-                                     const int32_t* block_tables, int64_t block_table_stride,
-                                     int max_blocks_per_seq, const int32_t* query_start_loc,
-                                     const int32_t* num_prior, int n_seqs, int n_tokens,
-                                     int n_q_heads, int n_kv_heads, int head_dim, int block_size,
-                                     float scale, int dtype, void* scratch, size_t scratch_bytes,
-                                     int* err_flags, pkv_stream_t stream) {
+int pkv_paged_prefill_attention_int8_served(
+    void* out, int64_t out_row_stride, const void* q, int64_t q_row_stride, const void* k_pool,
+    const void* v_pool, const float* k_scale, const float* v_scale, int num_blocks,
+    const int32_t* block_tables, int64_t block_table_stride, int max_blocks_per_seq,
+    const int32_t* query_start_loc, const int32_t* num_prior, const int32_t* context_lens, int n_seqs,
+    int n_tokens, int n_q_heads, int n_kv_heads, int head_dim, int block_size, float scale, int dtype,
+    void* scratch, size_t scratch_bytes, int* err_flags, pkv_stream_t stream) {
   if (n_seqs < 0 || n_tokens < 0) return PKV_ERR_BAD_SHAPE;
   if (n_seqs == 0 || n_tokens == 0) return PKV_OK;
   int rc = check_int8(k_pool, v_pool, k_scale, v_scale, num_blocks, block_tables, block_table_stride,
@@ -265,6 +263,7 @@ int pkv_paged_prefill_attention_int8(void* out, int64_t out_row_stride, const vo
   y.max_blocks = max_blocks_per_seq;
   y.query_start_loc = query_start_loc;
   y.num_prior = num_prior;
+  y.context_lens = context_lens;
   y.n_seqs = n_seqs;
   y.num_blocks = num_blocks;
   y.block_size = block_size;
@@ -306,6 +305,21 @@ int pkv_paged_prefill_attention_int8(void* out, int64_t out_row_stride, const vo
   a.dtype = dtype;
   a.err = err_flags;
   return status(launch_packed_attention(a, st));
+}
+
+int pkv_paged_prefill_attention_int8(void* out, int64_t out_row_stride, const void* q,
+                                     int64_t q_row_stride, const void* k_pool, const void* v_pool,
+                                     const float* k_scale, const float* v_scale, int num_blocks,
+                                     const int32_t* block_tables, int64_t block_table_stride,
+                                     int max_blocks_per_seq, const int32_t* query_start_loc,
+                                     const int32_t* num_prior, int n_seqs, int n_tokens,
+                                     int n_q_heads, int n_kv_heads, int head_dim, int block_size,
+                                     float scale, int dtype, void* scratch, size_t scratch_bytes,
+                                     int* err_flags, pkv_stream_t stream) {
+  return pkv_paged_prefill_attention_int8_served(
+      out, out_row_stride, q, q_row_stride, k_pool, v_pool, k_scale, v_scale, num_blocks, block_tables,
+      block_table_stride, max_blocks_per_seq, query_start_loc, num_prior, nullptr, n_seqs, n_tokens, n_q_heads,
+      n_kv_heads, head_dim, block_size, scale, dtype, scratch, scratch_bytes, err_flags, stream);
 }
 
 int pkv_packed_prompt_attention(void* out, int64_t out_row_stride, const void* q,

@@ -319,6 +319,13 @@ __global__ void __launch_bounds__(kI8Warps * 32) fetch_int8_kernel(const Int8Row
       raise_flag(a.err, PKV_FLAG_BAD_QUERY_LAYOUT);
     return;
   }
+  if (w.ctx == 0) {  // an unserved sequence: zero rows, bs of them a unit
+    T* dst = static_cast<T*>(const_cast<void*>(isv ? a.v : a.k));
+    const int r1 = static_cast<int>(min(static_cast<int64_t>(w.n), (w.j + static_cast<int64_t>(1)) * bs));
+    for (int64_t r = static_cast<int64_t>(w.j) * bs; r < r1; ++r)
+      for (int e = h0 * D + lane; e < h1 * D; e += 32) dst[(w.row0 + r) * (isv ? a.v_stride : a.k_stride) + e] = Elem<T>::from_f(0.f);
+    return;
+  }
   const int from = w.ctx - w.n;  // first position fetched
   if (from < 0) {
     if (w.j == 0 && rem == 0 && lane == 0) raise_flag(a.err, PKV_FLAG_BAD_QUERY_LAYOUT);
@@ -398,7 +405,8 @@ __global__ void __launch_bounds__(kI8Warps * 32) fetch_int8_kernel(const Int8Row
 // into row s * cap + j of k_out / v_out [n_seqs * cap][n_kv_heads][D], so that a
 // sequence's keys are consecutive rows.  Rows past its last key are zeros up to
 // the next multiple of 128 (the attention kernel's key tile): a tile holds no
-// stale bytes.  A warp takes up to kLayLoads stores a lane of a 16-row group's K or V at
+// stale bytes.  All rows of a sequence that is not served are zeros, and so is what the
+// attention makes of them.  A warp takes up to kLayLoads stores a lane of a 16-row group's K or V at
 // a time, all its loads ahead of them.
 // Also clears the counters of the attention behind it.  Bound by the bytes for
 // long ones (64-bit divisions for every unit and a head index by division for
@@ -414,6 +422,7 @@ __global__ void __launch_bounds__(kLayThreads) lay_out_int8_kernel(const Int8Lay
        i += static_cast<int64_t>(gridDim.x) * gridDim.y * kLayThreads)
     a.zero[i] = 0;
   const int new_rows = a.query_start_loc[s + 1] - a.query_start_loc[s];
+  const bool served = a.context_lens == nullptr || a.context_lens[s] > 0;
   int64_t keys = static_cast<int64_t>(max(a.num_prior[s], 0)) + max(new_rows, 0);
   if (keys > static_cast<int64_t>(a.max_blocks) * bs) {
     if (blockIdx.x == 0 && threadIdx.x == 0) raise_flag(a.err, PKV_FLAG_CONTEXT_EXCEEDS_TABLE);
@@ -433,7 +442,7 @@ __global__ void __launch_bounds__(kLayThreads) lay_out_int8_kernel(const Int8Lay
     const bool isv = wp & 1;
     const int row0 = static_cast<int>(wp >> 1) * 16;
     int id = -1;
-    if (row0 < keys) {
+    if (row0 < keys && served) {
       id = a.block_tables[static_cast<int64_t>(s) * a.bt_stride + row0 / bs];
       if (id < 0 || id >= a.num_blocks) {
         if (lane == 0) raise_flag(a.err, PKV_FLAG_BLOCK_OUT_OF_RANGE);

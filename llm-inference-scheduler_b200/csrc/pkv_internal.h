@@ -222,6 +222,7 @@ struct Int8LayArgs {
   int max_blocks;
   const int32_t* query_start_loc;
   const int32_t* num_prior;
+  const int32_t* context_lens;  // NULL, or 0 for a sequence that is not served: its rows are zeros
   int n_seqs, num_blocks, block_size, n_kv_heads, head_dim;
   void* k_out;
   void* v_out;

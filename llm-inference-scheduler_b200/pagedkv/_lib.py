@@ -112,6 +112,9 @@ SIGNATURES: dict = {
     "pkv_prefill_int8_scratch_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I, _I]),
     "pkv_paged_prefill_attention_int8": (_I, [_P, _I64, _P, _I64, _P, _P, _P, _P, _I, _P, _I64, _I, _P,
                                               _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _SZ, _P, _P]),
+    "pkv_paged_prefill_attention_int8_served": (_I, [_P, _I64, _P, _I64, _P, _P, _P, _P, _I, _P, _I64, _I,
+                                                     _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _SZ, _P,
+                                                     _P]),
     "pkv_packed_prompt_attention": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I, _I, _I, _I, _I,
                                          _F, _I, _P, _P]),
 }

@@ -754,7 +754,7 @@ class PagedKVCache:
                                        meta.query_start_loc, mgr.err)
             ops.paged_prefill_attention_int8(q[nd:], *pools, tabs[nd:], meta.query_start_loc,
                                              meta.num_prior_dev[nd:], meta.max_query_len, scale,
-                                             out=out[nd:], err=mgr.err, scratch=scratch)
+                                             out=out[nd:], err=mgr.err, scratch=scratch, context_lens=ctx[nd:])
         if advance and layer == mgr.num_layers - 1:
             self._advance(meta)
         return out

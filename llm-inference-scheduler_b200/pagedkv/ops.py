@@ -1092,7 +1092,8 @@ def build_step_tables(block_tables: torch.Tensor, free_blocks: torch.Tensor, n_f
 
     A request the free list is too short for sets PKV_FLAG_OUT_OF_BLOCKS in
     err; it and those after it get slots -1 and context length 0 and take no
-    block.  Reference: scheduler.py:79-156 and block_manager.py:121-131 (host)."""
+    block (their rows stay in query_start_loc: pass context_lens to
+    paged_prefill_attention_int8; the other chunk calls give nothing of use for them).  Reference: scheduler.py:79-156 and block_manager.py:121-131 (host)."""
     dev = _one_device("block_tables free_blocks n_free num_prior num_new err", block_tables, free_blocks,
                       n_free, num_prior, num_new, err)
     _check_tables(block_tables)
@@ -1194,8 +1195,9 @@ def fetch_int8(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor
                err: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The last row_start_loc[i + 1] - row_start_loc[i] rows of each context as
     values of `dtype`: (K, V), each [n_rows, Hkv, D], one sequence behind the
-    other (rows past row_start_loc[-1] are left as allocated).  Reference: the
-    gather of append_and_fetch, block_manager.py:136-141."""
+    other (rows past row_start_loc[-1] are left as allocated; rows of a context of
+    length 0 are zeros).  Reference: the gather of append_and_fetch,
+    block_manager.py:136-141."""
     dev = _one_device("k_pool v_pool k_scale v_scale block_tables context_lens row_start_loc err", k_pool, v_pool,
                       k_scale, v_scale, block_tables, context_lens, row_start_loc, err)
     nb, bs, hkv, d = _check_int8_pools(k_pool, v_pool, k_scale, v_scale)
@@ -1278,19 +1280,23 @@ def paged_prefill_attention_int8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: 
                                  block_tables: torch.Tensor, query_start_loc: torch.Tensor,
                                  num_prior: torch.Tensor, max_query_len: int, scale: float,
                                  out: torch.Tensor | None = None, err: torch.Tensor | None = None,
-                                 scratch: torch.Tensor | None = None) -> torch.Tensor:
+                                 scratch: torch.Tensor | None = None,
+                                 context_lens: torch.Tensor | None = None) -> torch.Tensor:
     """paged_prefill_attention over int8 pools with a scale per (block, KV
     head): query i of sequence s sees keys 0 .. num_prior[s] + i.  The visible
     rows are laid out as values of q's dtype in `scratch`
     (prefill_int8_scratch_bytes; allocated here when None), which the packed
     attention kernel then reads.  max_query_len is taken as the other prefill
-    calls take it; this path does not need it."""
-    dev = _one_device("q k_pool v_pool k_scale v_scale block_tables query_start_loc num_prior scratch out err", q,
-                      k_pool, v_pool, k_scale, v_scale, block_tables, query_start_loc, num_prior, scratch, out,
-                      err)
+    calls take it; this path does not need it.  context_lens: build_step_tables',
+    where some requests may not be served (length 0: zero rows, the table is not read)."""
+    dev = _one_device("q k_pool v_pool k_scale v_scale block_tables query_start_loc num_prior scratch out err "
+                      "context_lens", q, k_pool, v_pool, k_scale, v_scale, block_tables, query_start_loc,
+                      num_prior, scratch, out, err, context_lens)
     nb, bs, hkv, d = _check_int8_pools(k_pool, v_pool, k_scale, v_scale)
     _check_err(err)
     n_seqs = _check_rows_of(block_tables, num_prior, query_start_loc, "query_start_loc")
+    if context_lens is not None:
+        _int_row(context_lens, "context_lens", n_seqs)
     T, hq, dq = q.shape
     if dq != d or hq % hkv:
         raise ValueError("pagedkv: q / pools shapes disagree")
@@ -1301,11 +1307,11 @@ def paged_prefill_attention_int8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: 
         scratch = torch.empty(
             prefill_int8_scratch_bytes(n_seqs, T, block_tables.shape[1], hq, hkv, d, bs, q.dtype),
             dtype=torch.uint8, device=q.device)
-    _call("pkv_paged_prefill_attention_int8", dev, out.data_ptr(), _row_stride(out, "out"), q.data_ptr(),
+    _call("pkv_paged_prefill_attention_int8_served", dev, out.data_ptr(), _row_stride(out, "out"), q.data_ptr(),
           _row_stride(q, "q"), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
           v_scale.data_ptr(), nb, block_tables.data_ptr(), block_tables.stride(0),
-          block_tables.shape[1], query_start_loc.data_ptr(), num_prior.data_ptr(), n_seqs, T, hq, hkv,
-          d, bs, float(scale), dtype_code(q.dtype), scratch.data_ptr(), _bytes_of(scratch, "scratch"),
+          block_tables.shape[1], query_start_loc.data_ptr(), num_prior.data_ptr(), _ptr(context_lens), n_seqs, T,
+          hq, hkv, d, bs, float(scale), dtype_code(q.dtype), scratch.data_ptr(), _bytes_of(scratch, "scratch"),
           _ptr(err))
     return out
 
