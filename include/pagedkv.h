@@ -584,7 +584,8 @@ int pkv_paged_prefill_attention_fp8(void* out, int64_t out_row_stride, const voi
  * no context_lens: what they give for its rows is of no use (its table holds no
  * blocks for them).  A negative length (PKV_FLAG_BAD_QUERY_LAYOUT) or one past
  * the table (PKV_FLAG_CONTEXT_EXCEEDS_TABLE) counts as a request without tokens.
- * n_free_out must not be n_free.  Up to 16,384 requests.
+ * No output may overlap n_free, num_prior, num_new or free_blocks
+ * (PKV_ERR_UNSUPPORTED).  Up to 16,384 requests.
  */
 int pkv_build_step_tables(int32_t* block_tables, int64_t block_table_stride, int max_blocks_per_seq,
                           const int32_t* free_blocks, int n_free_blocks, const int32_t* n_free,

@@ -41,7 +41,6 @@ int pkv_build_step_tables(int32_t* block_tables, int64_t block_table_stride, int
                           int n_tokens, int* err_flags, pkv_stream_t stream) {
   if (n_seqs < 0 || n_tokens < 0 || n_free_blocks < 0 || block_size <= 0) return PKV_ERR_BAD_SHAPE;
   if (!n_free || !n_free_out || !query_start_loc) return PKV_ERR_NULL_POINTER;
-  if (n_free == n_free_out) return PKV_ERR_UNSUPPORTED;  // read by every CTA while one writes
   if (n_seqs > 0) {
     if (!block_tables || !num_prior || !num_new || !context_lens) return PKV_ERR_NULL_POINTER;
     if (max_blocks_per_seq <= 0 || block_table_stride < max_blocks_per_seq ||
@@ -51,6 +50,17 @@ int pkv_build_step_tables(int32_t* block_tables, int64_t block_table_stride, int
   }
   if (n_free_blocks > 0 && !free_blocks) return PKV_ERR_NULL_POINTER;
   if (n_tokens > 0 && (!slot_mapping || !positions)) return PKV_ERR_NULL_POINTER;
+  // every CTA reads the inputs while others write: no output may lie over an input
+  const struct { const void* p; size_t bytes; } ins[] = {
+      {n_free, 4}, {num_prior, 4 * static_cast<size_t>(n_seqs)}, {num_new, 4 * static_cast<size_t>(n_seqs)},
+      {free_blocks, 4 * static_cast<size_t>(n_free_blocks)}}, outs[] = {
+      {n_free_out, 4}, {context_lens, 4 * static_cast<size_t>(n_seqs)}, {query_start_loc, 4 * (static_cast<size_t>(n_seqs) + 1)},
+      {slot_mapping, 8 * static_cast<size_t>(n_tokens)}, {positions, 8 * static_cast<size_t>(n_tokens)}};
+  for (const auto& o : outs)
+    for (const auto& i : ins) {
+      const uintptr_t x = reinterpret_cast<uintptr_t>(o.p), y = reinterpret_cast<uintptr_t>(i.p);
+      if (x < y + i.bytes && y < x + o.bytes) return PKV_ERR_UNSUPPORTED;
+    }
   StepTablesArgs a{};
   a.block_tables = block_tables;
   a.bt_stride = block_table_stride;

@@ -1088,7 +1088,9 @@ def build_step_tables(block_tables: torch.Tensor, free_blocks: torch.Tensor, n_f
     which BlockManager.allocate pops).  num_prior, num_new: int32 [B].
     n_tokens: rows of the batch (at least the sum of num_new; further rows get
     slot -1).  The free count after the step is in the result's n_free, another
-    tensor than the one passed in; pass it to the next step.
+    tensor than the one passed in; pass it to the next step.  out: buffers of
+    new_step_tables; none may overlap num_prior, num_new, n_free or free_blocks
+    (refused: every CTA reads those while others write).
 
     A request the free list is too short for sets PKV_FLAG_OUT_OF_BLOCKS in
     err; it and those after it get slots -1 and context length 0 and take no
