@@ -85,3 +85,24 @@ def test_loud_blocks_of_no_weight(dtype, hq, hkv, d, ratio, order):
         o, tol = weighted_tolerance(dt, q[i:i + 1], k, v, vscale, 0.125)
         off = (out[i:i + 1].double() - o).abs()
         assert bool((off <= tol).all()), f"context {c} off by up to {float((off / tol).max()):.2f} of the bound"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("where", ["first", "last", "all"])
+@pytest.mark.parametrize("dtype,hq,hkv,d", [("f16", 14, 2, 64), ("bf16", 16, 1, 128), ("f32", 14, 2, 64)])
+def test_blocks_of_zeros(dtype, hq, hkv, d, where):
+    """Blocks whose rows are all zeros have the least scale, 2^-120: as any other block."""
+    bs, dt, ctx = 16, DT[dtype], [7, 40, 1500, 9000]
+    tables, nb = layout(ctx, bs, 3)
+    (kp, ks), (vp, vs) = random_pool(nb, bs, hkv, d, 1), random_pool(nb, bs, hkv, d, 2)
+    for t, c in zip(tables, ctx):
+        n = -(-c // bs)
+        zero = t[:n] if where == "all" else t[:(n + 2) // 3] if where == "first" else t[n // 2:n]
+        kp[zero], vp[zero], ks[zero], vs[zero] = 0, 0, 2.0 ** -120, 2.0 ** -120
+    q = torch.randn(len(ctx), hq, d, generator=torch.Generator().manual_seed(4)).to(dt)
+    out = decode(q, kp, vp, ks, vs, tables, ctx, 0.125)
+    for i, c in enumerate(ctx):
+        k, v = values(kp, ks, tables[i], c, bs), values(vp, vs, tables[i], c, bs)
+        vscale = vs[tables[i][:-(-c // bs)]].double().repeat_interleave(bs, 0)[:c]
+        o, tol = weighted_tolerance(dt, q[i:i + 1], k, v, vscale, 0.125)
+        assert bool(((out[i:i + 1].double() - o).abs() <= tol).all())
