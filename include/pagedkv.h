@@ -603,7 +603,8 @@ int pkv_build_step_tables(int32_t* block_tables, int64_t block_table_stride, int
  * that head; byte = x / s rounded to nearest even; value = byte * s (exact in
  * fp16 range, bf16 and fp32).  Infinities are stored as +-127 and NaN as 0, and
  * neither enters absmax.  In fp16, rows of more than 65,024 in magnitude may come
- * back as infinities (64 * 1,024 is past 65,504).  q, out and new rows are in `dtype` (fp32, fp16 or
+ * back as infinities (64 * 1,024 is past 65,504); in bf16 and fp32, more than
+ * 127 * 2^121 (64 * 2^122 is past the largest).  q, out and new rows are in `dtype` (fp32, fp16 or
  * bf16).  head_dim 64 or 128, block_size a multiple of 16, pools 16-byte aligned
  * (else PKV_ERR_UNSUPPORTED / PKV_ERR_MISALIGNED).
  */

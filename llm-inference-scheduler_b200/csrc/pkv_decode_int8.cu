@@ -40,11 +40,12 @@
 // launch.
 //
 // What bounds it: HBM where heads are wide (64 sequences of 4,096 tokens, 32 / 8 x
-// 128: 92.9 us, 5.8 TB/s of 6.5 measured for a copy), the instructions of the two
+// 128: 93.5 us, 5.8 TB/s of 6.5 measured for a copy), the instructions of the two
 // kinds of tiles at 64 dims and 7 query heads a KV head (64 x 8,192 tokens, 14 / 2
-// x 64: 33.0 us, 4.1 TB/s), and for small steps the fixed part: about 2 us to the
-// first tile, 1.3 for the join in the CTA, 2.5 for the second launch (256 x 1,024:
-// 22.3 us for 67 MB; one sequence of 131,072: 15.7 us for 34 MB; of 16: 5.5 us).
+// x 64: 34.0 us, 4.0 TB/s; 64 x 4,096 22.0, with fp32 q 23.0), and for small steps
+// the fixed part: about 2 us to the first tile, 1.3 for the join in the CTA, 2.5 for
+// the second launch (256 x 1,024: 22.9 us for 67 MB; one sequence of 131,072: 16.0 us
+// for 34 MB; of 16: 5.3 us).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -619,13 +620,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 // it, in order.  Four dims of one head to a thread; a sequence that many CTAs
 // share (a long one) is read by all the CTA's threads, kLanes partials of a head
 // side by side: its weights are made while up to kM8Ahead of a thread's partials
-// are on their way (running sums, four at a time, took 2.5 us more of 131,072
-// tokens' 15.7).  Empty sequences get zeros.  The lengths are read while the
+// are on their way (running sums, four at a time: 18.2 us instead of 15.7 for
+// 131,072 tokens).  Empty sequences get zeros.  The lengths are read while the
 // decode kernel runs (it starts this one after its own wait for them).
 //
-// Up to kM8Few partials a thread takes all of them for its dims (256 x 1,024
-// tokens: 22.3 us; 37.9 with the other way for all, 24.9 with this way for up to
-// 16).
+// Up to kM8Few partials a thread takes all of them for its dims (256 x 1,024 tokens
+// when this was chosen: 22.3 us; 37.9 with the other way for all, 24.9 with this way
+// for up to 16).
 constexpr int kM8Threads = 256, kM8Few = 6, kM8Ahead = 10;
 template <typename T, int D>
 __global__ void __launch_bounds__(kM8Threads) merge_int8_kernel(const D8Params p, int grid, int heads_per) {

@@ -25,8 +25,8 @@
 // floor(start_i / b) + 2 i and a warp finds its sequence by a search on the
 // start positions: no prefix pass, no scratch.  Bound by the bytes of the
 // rows for prompts (64 of 200 to 2,000 tokens, 8 x 128 in bf16, appended and
-// fetched: 460 MB in 108 us, 65% of the copy rate), by launch and round trips for
-// decode steps (256 single tokens, 2 x 64: 3.9 us, 7.1 with the fetch).
+// fetched: 460 MB in 105 us, 67% of the copy rate), by launch and round trips for
+// decode steps (256 single tokens, 2 x 64: 3.9 us, 7.4 with the fetch).
 #include <type_traits>
 
 #include "pkv_common.cuh"
@@ -196,8 +196,8 @@ __global__ void __launch_bounds__(kI8Warps * 32) append_int8_kernel(const Int8Ro
   // units of four consecutive elements: cpr to a row
   const int cpr = D / 4, total = (end - held) * cpr;
   // new rows that one load of 16 bytes a lane, at most kI8Regs times, can bring:
-  // they stay in registers between absmax and rounding (every block of 16 or 32
-  // rows here but fp32 ones of 128 dims); others are read twice
+  // they stay in registers between absmax and rounding (4 KB: 16 rows of 128 dims or
+  // 32 of 64 in 16 bits, 16 of 64 in fp32); larger blocks are read twice
   constexpr int kPer = 16 / sizeof(T), kLog = sizeof(T) == 2 ? 3 : 2;
   const int chunks = total * 4 / kPer, row_log = (D == 64 ? 6 : 7) - kLog;  // 2^row_log chunks to a row
   bool once = (isv ? a.v_vec16 : a.k_vec16) && chunks <= 32 * kI8Regs;

@@ -479,6 +479,13 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
 //   O += P V   (M 128, N = D, K 128 keys; P from tensor memory)
 // O is rescaled only when the running maximum grows by more than 2^8.
 //
+// Roundings.  S, the maximum, the row sum and O are fp32.  P goes into the second
+// product in q's type, since both operands of an MMA have one (fp16: 2^-11 of a
+// probability, bf16: 2^-8), and a third of the exponentials are polynomials good to
+// 7.5e-5, below that; the row sum takes P before its rounding.  Outputs are then off
+// by 1.3 times the output's own rounding (fp16 2.5e-4, bf16 2.0e-3 against 2.0e-4 and
+// 1.6e-3 for fp32 probabilities).  P in two parts would be two MMAs for one.
+//
 // Steps A(0), B(0), A(1), B(1), .. (query tile, key tile) go through a ring of S
 // buffers in tensor memory, which O leaves 384 columns (D = 64) or 256 of: three
 // buffers of 128 keys, or four of 64.  P of a step overwrites its own S, so a
@@ -507,8 +514,10 @@ cudaError_t launch_cores(const PackedArgs& a, cudaStream_t stream) {
 // What bounds it: at 64 dims the exponentials, one for every 256 FLOP of MMA (a
 // third of them are polynomials on the FMA pipe), at 128 dims the S -> P -> O chain
 // of short items.  One prompt of 16,384 tokens: 933 TFLOP/s (14 / 2 x 64), 1,308
-// (32 / 8 x 128); four of up to 8,191 tokens, 14 / 2 x 64: 164 us, 738 TFLOP/s;
-// twelve of up to 2,048, 32 / 8 x 128: 218 us, 837 TFLOP/s.
+// (32 / 8 x 128); four of up to 8,191 tokens, 14 / 2 x 64: 167 us, 727 TFLOP/s;
+// twelve of up to 2,048, 32 / 8 x 128: 222 us, 822 TFLOP/s.  No unit is full there
+// (issue slots 59% and 48%, exponentials 56% and 36%, tensor pipe 38% and 49% of the
+// launch): items' starts, diagonals and ends cost what long prompts do not show.
 //
 // Items are handed out while the kernel runs: a CTA starts with its own block
 // index and then takes the indices of blocks that have not started
