@@ -47,7 +47,8 @@ __device__ __forceinline__ KeySpan key_span(const PackedArgs& a, int s, int q_be
 // fp32 for values near its end.  A row that comes out not finite is therefore
 // computed again by a warp, over its own keys only, unless its own values make it
 // so: its sum of probabilities is NaN (hidden scores never enter that), or a V that
-// it sees is not finite and none of the hidden ones in its last tiles is.  (Without
+// it sees is not finite and none of the hidden ones in its last tiles is (then sums
+// that pass fp32 stay infinite in its other columns too).  (Without
 // that second rule one NaN in the first V of a prompt of 8,191 tokens had every later
 // row computed again: 77 ms.  With it 0.2; and 8.8 where the NaN is hidden from the
 // last rows, four at a time, against 45 one by one.)
